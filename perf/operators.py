@@ -112,7 +112,7 @@ def _prepare_slots(case, g, host):
     state = dict(case, states=tensors, source=order[0], list=order[1:1 + case["forks"]])
     if own:  # where the states lie: a cache makes this once
         from bitnet_c_b200.csrc import ops
-        state["where"] = ops.slot_rows(tensors)
+        state["where"] = ops.StateSlots(tensors)
     return state
 
 
