@@ -21,15 +21,15 @@ PAGE = 64  # tokens per page of the cache
 def listed():
     return [
         # two completions of one prompt in a small model: the last page, 16 planes, latency
-        dict(name="copy last page, 2 forks", op="copy", planes=16, heads=8, dim=64, vdim=64, dtype="bfloat16", moves=2, rows=37, forks=True),
+        dict(name="copy last page 2 forks", op="copy", planes=16, heads=8, dim=64, vdim=64, dtype="bfloat16", moves=2, rows=37, forks=True),
         # sixteen completions in the 8B sizes
-        dict(name="copy last page, 16 forks", op="copy", planes=32, heads=8, dim=128, vdim=128, dtype="bfloat16", moves=16, rows=51, forks=True),
+        dict(name="copy last page 16 forks", op="copy", planes=32, heads=8, dim=128, vdim=128, dtype="bfloat16", moves=16, rows=51, forks=True),
         # whole pages of the 8B sizes moved to the front of the pool: the bandwidth of a copy
         dict(name="copy whole pages", op="copy", planes=32, heads=8, dim=128, vdim=128, dtype="bfloat16", moves=64, rows=64, forks=False),
         # states of a few layers whose rows are no multiple of 16 bytes, one more completion
-        dict(name="slots, odd rows", op="slots", tensors=12, floats=771, forks=1),
+        dict(name="slots odd rows", op="slots", tensors=12, floats=771, forks=1),
         # recurrent states of 24 layers (16 heads of 128 x 128) for seven more completions
-        dict(name="slots, recurrent states", op="slots", tensors=24, floats=262144, forks=7),
+        dict(name="slots recurrent states", op="slots", tensors=24, floats=262144, forks=7),
         # four completions of a short prompt in the 1B sizes: launches and latency
         dict(name="attend 4 of one short prompt", op="attend", prompts=1, each=4, shared=200, tail=40, heads=32, kv_heads=8, dim=64),
         # eight prompts with eight completions each, 8B sizes, prompts of unequal lengths
@@ -37,13 +37,13 @@ def listed():
         # many completions of one long prompt
         dict(name="attend 64 of one long prompt", op="attend", prompts=1, each=64, shared=8192, tail=500, heads=32, kv_heads=8, dim=128),
         # one sequence, the small vocabulary, top-k: latency
-        dict(name="sample 1 row, top-k", op="sample", rows=1, vocab=32000, dtype="float32", filters="top_k", spread=3.0),
+        dict(name="sample 1 row top-k", op="sample", rows=1, vocab=32000, dtype="float32", filters="top_k", spread=3.0),
         # a batch of 8 with a nucleus and min-p
-        dict(name="sample 8 rows, top-p", op="sample", rows=8, vocab=128256, dtype="float32", filters="top_p", spread=3.0),
+        dict(name="sample 8 rows top-p", op="sample", rows=8, vocab=128256, dtype="float32", filters="top_p", spread=3.0),
         # many users, each with parameters of their own
-        dict(name="sample 64 rows, own params", op="sample", rows=64, vocab=128256, dtype="float32", filters="rows", spread=3.0),
+        dict(name="sample 64 rows own params", op="sample", rows=64, vocab=128256, dtype="float32", filters="rows", spread=3.0),
         # a flat distribution (an early checkpoint, a high temperature) over an odd vocabulary in bfloat16: many ties, wide nuclei
-        dict(name="sample 200 flat rows, bf16", op="sample", rows=200, vocab=50257, dtype="bfloat16", filters="rows", spread=1.0),
+        dict(name="sample 200 flat rows bf16", op="sample", rows=200, vocab=50257, dtype="bfloat16", filters="rows", spread=1.0),
     ]
 
 
