@@ -31,6 +31,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 SOURCES: Dict[str, str] = {
     "embed": "embed.cu",
     "cache_rows": "cache_rows.cu",
+    "cache_pages": "cache_pages.cu",
     "norm": "norm.cu",
     "rope": "rope.cu",
     "act": "act.cu",

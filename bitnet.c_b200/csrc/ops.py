@@ -7,6 +7,7 @@ back to the CPU: tensors that are not on a CUDA device are refused.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import functools
 from ctypes import c_float, c_int, c_void_p
@@ -43,6 +44,14 @@ def _stream() -> c_void_p:
         return c_void_p(torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice()))
     except AttributeError:  # a torch without these entry points
         return c_void_p(torch.cuda.current_stream().cuda_stream)
+
+
+def _on(device: torch.device):
+    """A context in which ``device`` is the current one (a switch costs microseconds: none where it is already)."""
+    return _HERE if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
+
+
+_HERE = contextlib.nullcontext()
 
 
 def _need(t: torch.Tensor, name: str, dtype=None, dims: Optional[int] = None) -> None:
@@ -1606,6 +1615,73 @@ def zero_slot(rows: torch.Tensor, slot: int) -> None:
     """Slot ``slot`` of all tensors that ``rows`` (of ``slot_rows``) was made from is set to zero, in one launch."""
     _need(rows, "rows", torch.int64, 2)
     _check(_fn("cache_rows", "bn_zero_slot")(_ptr(rows), int(rows.shape[0]), int(slot), _stream()), "zero_slot")
+
+
+# ---- pages and slots copied -----------------------------------------------------------------
+def _page_moves(moves, pages: int):
+    """``copy_pages``' moves as the kernel takes them: groups of (source, rows, number of destinations) and their destinations; refuses what does not
+    name pages of the cache, and destinations that another move reads or writes."""
+    groups, sources = {}, set()
+    for src, dst, rows in moves:
+        if not (0 <= src < pages and 0 <= dst < pages):
+            raise KernelError(f"copy_pages: page {src if not 0 <= src < pages else dst} is outside the {pages} pages of the cache")
+        if not 0 < rows <= PAGE:
+            raise KernelError(f"copy_pages: {rows} rows of a page of {PAGE}")
+        groups.setdefault((src, rows), []).append(dst)
+        sources.add(src)
+    to = [d for g in groups.values() for d in g]
+    if len(set(to)) != len(to) or not sources.isdisjoint(to):
+        raise KernelError("copy_pages: a page that is written must be written once and not read")
+    return [x for (src, rows), dst in groups.items() for x in (src, rows, len(dst))], to
+
+
+def copy_pages(k: torch.Tensor, v: Optional[torch.Tensor], moves) -> None:
+    """For every move (source page, destination page, rows) the first ``rows`` rows of every head of the source page are copied to the destination page, in
+    all planes, of keys and of values.  ``k`` [planes, pages, heads, 64, numbers] of any type, ``v`` the same with a width of its own, or None;
+    ``moves`` is a sequence on the host, read before the call returns.  A page that is written is written once and not read."""
+    _need(k, "k", dims=5)
+    if k.shape[3] != PAGE:
+        raise KernelError(f"copy_pages: k {tuple(k.shape)} is not [planes, pages, heads, {PAGE}, numbers]")
+    if v is not None:
+        _need(v, "v", dims=5)
+        if v.shape[:2] != k.shape[:2] or v.shape[3] != PAGE or v.device != k.device:
+            raise KernelError(f"copy_pages: v {tuple(v.shape)} on {v.device} does not go with k {tuple(k.shape)} on {k.device}")
+    groups, to = _page_moves(moves, k.shape[1])
+    if not to or 0 in k.shape:
+        return
+    g, d = (c_int * len(groups))(*groups), (c_int * len(to))(*to)
+    with _on(k.device):
+        # keys and values with different numbers of heads are copied one after the other
+        for one, other in ([(k, v)] if v is None or v.shape[2] == k.shape[2] else [(k, None), (v, None)]):
+            _check(_fn("cache_pages", "bn_copy_pages")(
+                _ptr(one), _ptr(other), int(one.shape[0]), int(one.shape[1]), int(one.shape[2]), int(one.shape[4] * one.element_size()),
+                int(other.shape[4] * other.element_size()) if other is not None else 0, g, len(groups) // 3, d, len(to), _stream()), "copy_pages")
+
+
+class StateSlots:
+    """Where the states of a cache lie, for ``copy_slots``: tensors ``[slots, ...]`` of one device, contiguous, with the same number of slots."""
+
+    def __init__(self, tensors):
+        self.tensors = list(tensors)  # kept alive: their addresses are passed on
+        for t in self.tensors:
+            _need(t, "state")
+            if t.dim() < 1 or t.shape[0] != self.tensors[0].shape[0] or t.device != self.tensors[0].device:
+                raise KernelError("copy_slots: states must have the same number of slots and lie on one device")
+        self.n_slots = self.tensors[0].shape[0] if self.tensors else 0
+        where = [x for t in self.tensors for x in (t.data_ptr(), t.stride(0) * t.element_size() if t.numel() else 0)]
+        self.where = (ctypes.c_longlong * len(where))(*where)
+
+
+def copy_slots(states: StateSlots, source: int, slots) -> None:
+    """Slot ``source`` of all tensors of ``states`` is copied to each of ``slots`` (a sequence on the host), in one launch."""
+    slots = list(slots)
+    if len(set(slots)) != len(slots) or source in slots or not all(0 <= s < states.n_slots for s in (source, *slots)):
+        raise KernelError(f"copy_slots: slot {source} to {slots} of {states.n_slots}")
+    if not slots or not states.tensors:
+        return
+    with _on(states.tensors[0].device):
+        _check(_fn("cache_pages", "bn_copy_slots")(states.where, len(states.tensors), states.n_slots, int(source), (c_int * len(slots))(*slots), len(slots),
+                                                   _stream()), "copy_slots")
 
 
 # ---- mLSTM ----------------------------------------------------------------------------------
