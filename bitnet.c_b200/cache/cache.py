@@ -138,7 +138,44 @@ class KvGroup:
         self.dirty.discard(slot)
 
     def tokens_held(self) -> int:
-        return sum(len(h) for h in self.held.values()) * PAGE
+        return (self.pool.n_pages - self.pool.n_free) * PAGE
+
+    def fork(self, slot: int, length: int, new_slots: Sequence[int]) -> List[Tuple[int, int, int]]:
+        """Let each of ``new_slots`` hold what the sequence of ``length`` tokens in ``slot`` holds: its full pages too, of the last
+        one, if it is not full, a page of its own.  Returns what is to be copied, as ``ops.copy_pages`` takes it."""
+        full, rest = divmod(length, PAGE)
+        held = self.held.get(slot, {})
+        shared = {i: p for i, p in held.items() if i < full}
+        part = held.get(full) if rest else None
+        own = self.pool.alloc(len(new_slots) if part is not None else 0)
+        for n, new in enumerate(new_slots):
+            self.pool.share(list(shared.values()))
+            mine = self.held[new] = dict(shared)
+            if part is not None:
+                mine[full] = own[n]
+            for i, p in mine.items():
+                self.host_table[new, i] = p
+            self.dirty.add(new)
+        return [(part, p, rest) for p in own]
+
+    def compact(self) -> List[Tuple[int, int, int]]:
+        """Renumber the held pages so that they are the first ones; returns what is to be copied."""
+        held = sorted({p for h in self.held.values() for p in h.values()})
+        gaps = [p for p in range(len(held)) if not self.pool.holders(p)]
+        moved = dict(zip([p for p in held if p >= len(held)], gaps))
+        if moved:
+            self.pool.renumber({p: moved.get(p, p) for p in held})
+            for slot, h in self.held.items():
+                for i, p in h.items():
+                    if p in moved:
+                        h[i] = self.host_table[slot, i] = moved[p]
+                        self.dirty.add(slot)
+        return [(old, new, PAGE) for old, new in moved.items()]
+
+    def copy(self, moves: List[Tuple[int, int, int]]) -> None:
+        if moves and self.k is not None:
+            from ..csrc import ops
+            ops.copy_pages(self.k, self.v, moves)
 
 
 class Cache:
@@ -210,6 +247,7 @@ class Cache:
                 self.states[i] = torch.zeros((n_slots,) + tuple(r.shape), dtype=r.dtype, device=device)
                 if isinstance(i, tuple):
                     self._named.setdefault(i[0], {})[i[1]] = self.states[i]
+        self._state_slots = None  # the same for copying a slot of all of them, made when a sequence is first forked
         self._state_rows = None  # where the states lie, for zeroing a slot of all of them in one launch
         if self.states and torch.device(device).type == "cuda":
             from ..csrc import ops
@@ -227,6 +265,44 @@ class Cache:
             for t in self.states.values():
                 t[slot].zero_()
         return slot
+
+    def fork(self, slot: int, n: int = 1) -> List[int]:
+        """``n`` new sequences that go on from where the one in ``slot`` is: their slots.  They share its full pages (a page is free again when
+        its last holder has given it back); the rows of its last page, if that is not full, and its states are copied, in one launch
+        for every group of runs and one for all states.  If the slots or pages for them are not there, nothing has changed."""
+        length = self.slots.length(slot)  # raises if not open
+        if n < 1:
+            raise CacheError(f"a sequence is forked into at least one, not {n}")
+        if n > self.slots.n_free:
+            raise CacheFull(f"{n} slots wanted, {self.slots.n_free} of {self.slots.n_slots} free")
+        new = [self.slots.open() for _ in range(n)]
+        try:
+            moves = [g.fork(slot, length, new) for g in self.groups]
+        except CacheFull:
+            for s in new:
+                self.close(s)
+            raise
+        for s in new:
+            self.slots.set_length(s, length)
+        for g, m in zip(self.groups, moves):
+            g.copy(m)
+        if self.states:
+            from ..csrc import ops
+            if self._state_slots is None:
+                self._state_slots = ops.StateSlots(self.states.values())
+            ops.copy_slots(self._state_slots, slot, new)
+        return new
+
+    def compact(self) -> int:
+        """Move pages so that the held ones of each group are its first, ``g.k[:, :n]`` and ``g.v[:, :n]`` for ``n`` of them: what is to be saved, or
+        sent elsewhere, is then one slice.  Returns the number of pages that were moved.  Sequences keep their slots, what they hold and whom
+        they share it with; recorded steps stay valid (page tables are data)."""
+        moved = 0
+        for g in self.groups:
+            moves = g.compact()
+            g.copy(moves)
+            moved += len(moves)
+        return moved
 
     def close(self, slot: int) -> None:
         """The sequence has ended: its pages and its slot are free for the next one."""
@@ -326,20 +402,22 @@ class Cache:
         return sum(g.bytes_per_token(item) for g in self.groups)
 
     def check(self) -> None:
-        """Invariants: no slot or page lost, held twice or freed twice; tables agree."""
+        """Invariants: no slot or page lost, freed twice or held by more than the pool knows of; only full pages are shared, as the same page of
+        every sequence that holds them; tables agree."""
         self.slots.check()
         active = set(self.slots.active())
         for g in self.groups:
             g.pool.check()
-            seen: Dict[int, int] = {}
+            seen: Dict[int, List[Tuple[int, int]]] = {}
             for slot, held in g.held.items():
                 if slot not in active and held:
                     raise CacheError(f"closed slot {slot} still holds pages")
                 for i, p in held.items():
-                    if p in seen:
-                        raise CacheError(f"page {p} is held by slots {seen[p]} and {slot}")
-                    seen[p] = slot
+                    seen.setdefault(p, []).append((slot, i))
                     if g.host_table[slot, i] != p:
                         raise CacheError(f"page table of slot {slot} disagrees at index {i}")
+            for p, by in seen.items():
+                if len(by) != g.pool.holders(p) or len({i for _s, i in by}) != 1 or (len(by) > 1 and any((i + 1) * PAGE > self.slots.length(s) for s, i in by)):
+                    raise CacheError(f"page {p} is held by (slot, index) {by}, counted {g.pool.holders(p)} times")
             if len(seen) + g.pool.n_free != g.pool.n_pages:
                 raise CacheError("pages are lost: held + free != total")

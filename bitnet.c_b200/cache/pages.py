@@ -27,14 +27,15 @@ def pages_for(n_tokens: int) -> int:
 
 
 class PagePool:
-    """Free list over ``n_pages`` page ids.  Every id is either free or held, never both."""
+    """Free list over ``n_pages`` page ids.  Every id is either free or held, never both; a page that several sequences share is held
+    once by each, and free again when the last of them has given it back."""
 
     def __init__(self, n_pages: int):
         if n_pages <= 0:
             raise CacheError(f"a page pool needs at least one page, got {n_pages}")
         self.n_pages = n_pages
         self._free: List[int] = list(range(n_pages - 1, -1, -1))  # pop() hands out 0 first
-        self._held = [False] * n_pages
+        self._held = [0] * n_pages  # how often each page is held
 
     @property
     def n_free(self) -> int:
@@ -49,8 +50,26 @@ class PagePool:
         for p in out:
             if self._held[p]:
                 raise CacheError(f"page {p} was on the free list while held")
-            self._held[p] = True
+            self._held[p] = 1
         return out
+
+    def holders(self, page: int) -> int:
+        return self._held[page]
+
+    def share(self, pages: List[int]) -> None:
+        """Held pages are held once more each."""
+        for p in pages:
+            if not 0 <= p < self.n_pages or not self._held[p]:
+                raise CacheError(f"page {p} cannot be shared: nothing holds it")
+            self._held[p] += 1
+
+    def renumber(self, new_id: Dict[int, int]) -> None:
+        """Held pages change their ids (the free ones are then handed out lowest first): ``new_id`` names every held page."""
+        held = [0] * self.n_pages
+        for old, new in new_id.items():
+            held[new] = self._held[old]
+        self._held = held
+        self._free = [p for p in range(self.n_pages - 1, -1, -1) if not held[p]]
 
     def free(self, pages: List[int]) -> None:
         for p in pages:
@@ -58,15 +77,17 @@ class PagePool:
                 raise CacheError(f"page {p} does not exist")
             if not self._held[p]:
                 raise CacheError(f"page {p} is freed twice")
-            self._held[p] = False
-            self._free.append(p)
+            self._held[p] -= 1
+            if not self._held[p]:
+                self._free.append(p)
 
     def check(self) -> None:
         """Every page is exactly once either free or held."""
         if len(set(self._free)) != len(self._free):
             raise CacheError("a page is on the free list twice")
+        free = set(self._free)
         for p in range(self.n_pages):
-            if self._held[p] == (p in set(self._free)):
+            if (self._held[p] > 0) == (p in free):
                 raise CacheError(f"page {p} is {'both held and free' if self._held[p] else 'lost'}")
 
 

@@ -95,3 +95,65 @@ def test_copy_slots_more_tensors_than_one_launch_takes(cuda_device):
     want = [t[7].clone() for t in tensors]
     ops.copy_slots(ops.StateSlots(tensors), 7, [i for i in range(300) if i != 7])
     assert all(torch.equal(t, w.expand(300, 3)) for t, w in zip(tensors, want))
+
+
+# ---- forks of a cache ------------------------------------------------------------------------------
+def seen_by(cache, group, slot):
+    """Keys and values of the sequence in ``slot``, through the page table on the device: [planes, heads, positions, numbers]."""
+    n = cache.length(slot)
+    pages = group.page_table[slot, :(n + PAGE - 1) // PAGE].long()
+    rows = lambda t: torch.cat([t[:, p] for p in pages], 2)[:, :, :n].clone()
+    return rows(group.k), rows(group.v)
+
+
+@pytest.mark.parametrize("length", [1, 64, 100, 193])
+def test_fork_and_compact_keep_what_sequences_see(cuda_device, length):
+    from bitnet_c_b200.cache import Cache
+    from bitnet_c_b200.parts import KvRequest, StateRequest
+    requests = [KvRequest(2, 16), KvRequest(2, 16), KvRequest(1, 32, v_head_dim=48)]
+    states = [None, StateRequest((3, 5)), {"a": StateRequest((7,)), "b": StateRequest((2, 4), torch.float32)}]
+    c = Cache(requests, [None] * 3, states, 40 * 64, 1000, torch.bfloat16, torch.device(cuda_device), max_seqs=8)
+    other = c.open()
+    c.reserve(other, 130)
+    c.advance(other, 130)
+    a = c.open()
+    c.reserve(a, length)
+    c.advance(a, length)
+    for i, g in enumerate(c.groups):
+        g.k.copy_(filled(tuple(g.k.shape), g.k.dtype, cuda_device, i))
+        g.v.copy_(filled(tuple(g.v.shape), g.v.dtype, cuda_device, i + 9))
+    for i, t in enumerate(c.states.values()):
+        t.copy_(filled(tuple(t.shape), t.dtype, cuda_device, i))
+    c.sync()
+    forks = c.fork(a, 3)
+    forks += c.fork(forks[1])
+    c.sync()
+    c.check()
+    want = [seen_by(c, g, a) for g in c.groups]
+    at_rest = [seen_by(c, g, other) for g in c.groups]
+
+    def same(slots):
+        for s in slots:
+            for g, w in zip(c.groups, want):
+                assert all(torch.equal(x, y) for x, y in zip(seen_by(c, g, s), w))
+            assert all(torch.equal(t[s], t[a]) for t in c.states.values())
+
+    same(forks)
+    # the last page of each is its own
+    if length % PAGE:
+        g = c.groups[0]
+        g.k[:, int(g.page_table[forks[0], length // PAGE])] = 0
+        want_of_first = seen_by(c, g, forks[0])
+        assert not torch.equal(want_of_first[0], want[0][0])
+        same(forks[1:])
+    c.close(forks.pop(0))
+    c.close(a)
+    left = [seen_by(c, g, forks[0]) for g in c.groups]
+    moved = c.compact()
+    c.sync()
+    c.check()
+    assert moved > 0 or length % PAGE == 0
+    for g, w, r in zip(c.groups, left, at_rest):
+        for s in forks:
+            assert all(torch.equal(x, y) for x, y in zip(seen_by(c, g, s), w))
+        assert all(torch.equal(x, y) for x, y in zip(seen_by(c, g, other), r))
