@@ -48,6 +48,7 @@ SOURCES: Dict[str, str] = {
     "linear_tc": "linear_tc.cu",
     "gemm_tc": "gemm_tc.cu",
     "sampling": "sampling.cu",
+    "sampling_filtered": "sampling_filtered.cu",
     "argmax_noalloc": "argmax_noalloc.cu",
     "unit_norm": "unit_norm.cu",
     "mlstm": "mlstm.cu",

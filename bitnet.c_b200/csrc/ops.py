@@ -2635,6 +2635,64 @@ def sample_topp(logits: torch.Tensor, temperature: float, topp: float, rng_state
     return out
 
 
+def sample_filtered(logits: torch.Tensor, temperature, top_k=0, top_p=1.0, min_p=0.0, *, u: Optional[torch.Tensor] = None,
+                    rng_state: Optional[torch.Tensor] = None, index: Optional[torch.Tensor] = None,
+                    out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """One token per row of ``logits`` (float32 or bfloat16, rows may lie apart), int32 on the device; -1 for a row without a number above -inf.
+
+    In sorted order (falling logits, equal ones by rising index, NaN as -inf, -inf never chosen) with weights exp((logit - max) / temperature):
+    the first ``top_k`` (0: all); of them up to the first whose running sum exceeds ``top_p`` of their sum (outside (0, 1): all); of those
+    the ones of at least ``min_p`` times the largest weight; then the first whose running sum exceeds u times the sum of what is left.  A
+    temperature of 0 takes the first maximum; where there are logits of +inf, they share everything equally.
+    Each parameter is a number or a tensor with one per row (``top_k`` int32, the others float32; numbers are rounded to float32).
+    The random numbers are ``u`` [rows] in [0, 1), or row r draws from (and advances) the xorshift64* state ``rng_state[index[r]]`` (or [r])."""
+    _need_rows(logits, "logits")
+    n, vocab = logits.shape
+    device = logits.device
+
+    def given(x, name, dtype):
+        if not isinstance(x, torch.Tensor):
+            return None, (int(x) if dtype is torch.int32 else float(x))
+        _need(x, name, dtype, 1)
+        if x.shape[0] != n or x.device != device:
+            raise KernelError(f"sample_filtered: {name} {tuple(x.shape)} on {x.device} does not go with {n} rows on {device}")
+        return x, 0
+
+    temperatures, t = given(temperature, "temperature", torch.float32)
+    top_ks, k = given(top_k, "top_k", torch.int32)
+    top_ps, p = given(top_p, "top_p", torch.float32)
+    min_ps, m = given(min_p, "min_p", torch.float32)
+    if not t >= 0.0:
+        raise KernelError(f"sample_filtered: temperature={t} must not be negative")
+    k = min(max(k, 0), 0x7fffffff)
+    if (u is None) == (rng_state is None):
+        raise KernelError("sample_filtered: either u or rng_state")
+    if u is not None:
+        given(u, "u", torch.float32)
+        if index is not None:
+            raise KernelError("sample_filtered: index goes with rng_state")
+    else:
+        _need(rng_state, "rng_state", torch.int64, 1)
+        if index is not None:
+            given(index, "index", torch.int32)
+        elif rng_state.shape[0] < n:
+            raise KernelError("sample_filtered: one generator state per row is needed")
+    out = out if out is not None else torch.empty(n, dtype=torch.int32, device=device)
+    _need(out, "out", torch.int32, 1)
+    if out.shape[0] < n or out.device != device:
+        raise KernelError(f"sample_filtered: out {tuple(out.shape)} on {out.device} does not hold {n} tokens")
+    if n == 0:
+        return out
+    if vocab == 0:
+        raise KernelError("sample_filtered: no logits")
+    with _on(device):
+        _check(_fn("sampling_filtered", "bn_sample_filtered")(
+            _ptr(logits), _code(logits), ctypes.c_longlong(logits.stride(0) if n > 1 else vocab), int(n), int(vocab), c_float(t), _ptr(temperatures), k,
+            _ptr(top_ks), c_float(p), _ptr(top_ps), c_float(m), _ptr(min_ps), _ptr(u), _ptr(rng_state), _ptr(index), _ptr(out), _stream()),
+            "sample_filtered")
+    return out
+
+
 def repeat_penalty(logits: torch.Tensor, recent: torch.Tensor, recent_len: torch.Tensor, penalty: float,
                    index: Optional[torch.Tensor] = None) -> None:
     """In place: for each distinct id among the first recent_len[s] entries of recent[s] (s = index[r]
