@@ -90,9 +90,37 @@ struct DtArgs {
   int* tickets;    // [n_seqs][gridDim.y], zero before and after
   __nv_bfloat16* out;
   int out_stride;
+  // with JOIN: what attention_shared.cu found for pages that a sequence shares with others
+  const int4* shared;     // per sequence: pages covered there (its first ones), the first of its results, their number
+  const float* shared_o;  // [results][n_heads][head_dim], unnormalised
+  const float* shared_ml; // [results][n_heads][2]: maximum and sum, as part_ml
+  int n_shared;           // results that there are
 };
 
-template <int HD, int DT_STAGES>
+// A row's element d from this kernel's keys (maximum m, sum den, unnormalised num) and from the shared ones: num and den over both, by the larger maximum.
+__device__ __forceinline__ float dt_join(const DtArgs& a, const int4& sh, int h, int d, float m, float den, float num) {
+  if (sh.y < 0 || sh.y + sh.z > a.n_shared) return num / den;  // (a list that does not go with this launch: nothing is read past its end)
+  const float* ml = a.shared_ml + ((size_t)sh.y * a.n_heads + h) * 2;
+  const float* o = a.shared_o + ((size_t)sh.y * a.n_heads + h) * a.head_dim + d;
+  float top = m;
+#pragma unroll 4
+  for (int p = 0; p < sh.z; ++p) top = fmaxf(top, __ldcg(ml + (size_t)p * a.n_heads * 2));
+  const float own = (m == -INFINITY) ? 0.f : exp2f(m - top);
+  den *= own;
+  num *= own;
+#pragma unroll 4
+  for (int p = 0; p < sh.z; ++p) {
+    const float2 one = __ldcg(reinterpret_cast<const float2*>(ml + (size_t)p * a.n_heads * 2));
+    const float w = (one.x == -INFINITY) ? 0.f : exp2f(one.x - top);
+    den += w * one.y;
+    num += w * __ldcg(o + (size_t)p * a.n_heads * a.head_dim);
+  }
+  return num / den;
+}
+
+// JOIN: the first pages of a sequence are attended to by the kernel in front of this one (attention_shared.cu), which lets this one start as soon as
+// the kernel before it has completed: this block walks the sequence's other pages meanwhile and waits where it joins the results.
+template <int HD, int DT_STAGES, bool JOIN>
 __global__ void __launch_bounds__(DT_THREADS)
 attention_decode_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, DtArgs a) {
   pdl_launch_dependents();  // the next kernel in the stream may begin its prologue
@@ -137,14 +165,15 @@ attention_decode_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
   const int h0 = kvh * group + gb * DT_ROWS;
   const int G = min(DT_ROWS, group - gb * DT_ROWS);
   const int pos = a.tok_pos[b];
-  const int lo = a.window > 0 ? max(0, pos - a.window + 1) : 0;
+  const int4 sh = JOIN ? a.shared[b] : make_int4(0, 0, 0, 0);
+  const int lo = JOIN ? min(sh.x, pos / BN_PAGE) * BN_PAGE : a.window > 0 ? max(0, pos - a.window + 1) : 0;
   // pages that hold a visible key, and this block's run of them
   const int p_lo = lo / BN_PAGE, p_hi = pos / BN_PAGE;
   // The blocks of a sequence share its visible pages evenly (as many as the launch gives each
   // sequence, whatever the bound it was sized for); a sequence too short for a split to pay is the
   // first block's alone.
   const int vis = p_hi - p_lo + 1;
-  const int ppb = vis < DT_SPLIT_MIN_PAGES ? vis : min(a.pages_per_block, (vis + nz - 1) / nz);
+  const int ppb = vis < DT_SPLIT_MIN_PAGES ? vis : JOIN ? (vis + nz - 1) / nz : min(a.pages_per_block, (vis + nz - 1) / nz);
   const int my_lo = p_lo + zi * ppb;
   const int my_hi = min(p_hi, my_lo + ppb - 1);
   const int z_lo = 0, z_hi = (vis - 1) / ppb;  // splits with a visible page
@@ -196,7 +225,7 @@ attention_decode_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
   for (int p = tid; p < DT_ROWS * HD / 8; p += DT_THREADS) reinterpret_cast<uint4*>(q_tile)[p] = make_uint4(0u, 0u, 0u, 0u);
   for (int p = tid; p < 2 * HD / 8; p += DT_THREADS) reinterpret_cast<uint4*>(new_kv)[p] = make_uint4(0u, 0u, 0u, 0u);
   BN_TRACE_ONLY(if (tr) tr[2] = global_timer();)
-  pdl_wait();  // the kernel before this one has completed: the q|k|v rows are there
+  if (!JOIN) pdl_wait();  // the kernel before this one has completed: the q|k|v rows are there
   BN_TRACE_ONLY(if (tr) tr[3] = global_timer();)
   __syncthreads();
 
@@ -407,6 +436,7 @@ attention_decode_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
       }
     }
   }
+  if (JOIN) pdl_wait();  // the shared pages' results are there
   if (failed) {
     // a page never arrived: loads that were requested may still be landing in this block's shared
     // memory, so give them a bounded time and leave without a result (the status word says so)
@@ -458,7 +488,8 @@ attention_decode_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
 #pragma unroll
     for (int w = 0; w < 4; ++w) acc += wsc[w * DT_ROWS + g] * o_part[(size_t)(w * DT_ROWS + g) * OSTRIDE + d];
     if (alone)  // the only split of this sequence: normalise and store
-      a.out[(size_t)b * a.out_stride + (size_t)(h0 + g) * head_dim + d] = __float2bfloat16_rn(acc / ml_fin[g * 2 + 1]);
+      a.out[(size_t)b * a.out_stride + (size_t)(h0 + g) * head_dim + d] =
+          __float2bfloat16_rn(JOIN ? dt_join(a, sh, h0 + g, d, ml_fin[g * 2], ml_fin[g * 2 + 1], acc) : acc / ml_fin[g * 2 + 1]);
     else if (clustered) o_fin[g * HD + d] = acc;
     else a.part_o[(((size_t)b * n_heads + h0 + g) * n_splits + zi) * head_dim + d] = acc;
   }
@@ -495,7 +526,7 @@ attention_decode_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
         den += w * lz[z];
         num += w * v[z];
       }
-      a.out[(size_t)b * a.out_stride + (size_t)(h0 + g) * head_dim + d] = __float2bfloat16_rn(num / den);
+      a.out[(size_t)b * a.out_stride + (size_t)(h0 + g) * head_dim + d] = __float2bfloat16_rn(JOIN ? dt_join(a, sh, h0 + g, d, m, den, num) : num / den);
     }
     BN_TRACE_ONLY(if (tr) tr[10] = global_timer();)
     dt_cluster_sync();  // no block leaves while another still reads its result
@@ -536,7 +567,8 @@ attention_decode_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
     const float* po = a.part_o + ((size_t)b * n_heads + h0 + g) * n_splits * head_dim;
     float m = ml_fin[g * 2], num = 0.f;
     for (int z = z_lo; z <= z_hi; ++z) num += exp2f(__ldcg(ml + 2 * z) - m) * __ldcg(po + (size_t)z * head_dim + d);
-    a.out[(size_t)b * a.out_stride + (size_t)(h0 + g) * head_dim + d] = __float2bfloat16_rn(num / ml_fin[g * 2 + 1]);
+    a.out[(size_t)b * a.out_stride + (size_t)(h0 + g) * head_dim + d] =
+        __float2bfloat16_rn(JOIN ? dt_join(a, sh, h0 + g, d, m, ml_fin[g * 2 + 1], num) : num / ml_fin[g * 2 + 1]);
   }
   BN_TRACE_ONLY(if (tr) tr[10] = global_timer();)
 }
@@ -569,23 +601,19 @@ static constexpr size_t dt_smem_bytes() {
   return 1024 + (size_t)DT_STAGES * 2 * BN_PAGE * HD * 2 + (size_t)DT_ROWS * HD * 2 + 2 * HD * 2 +
          (4 * DT_ROWS * 2 + DT_ROWS * 2) * sizeof(float) + DT_STAGES * 8 + HD * sizeof(float) + 4 * DT_ROWS * sizeof(float);
 }
-template <int HD, int DT_STAGES>
+template <int HD, int DT_STAGES, bool JOIN>
 static int launch_dt2(const CUtensorMap& mk, const CUtensorMap& mv, const DtArgs& a, dim3 grid, dim3 cluster, cudaStream_t stream) {
   size_t smem = dt_smem_bytes<HD, DT_STAGES>();
-  static bool configured = false;
-  if (!configured) {
-    cudaError_t e = cudaFuncSetAttribute(attention_decode_tc_kernel<HD, DT_STAGES>,
-                                         cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return BN_ERR_LAUNCH + (int)e;
-    configured = true;
-  }
+  static BnGrant grant;
+  const cudaError_t g = grant.ask((const void*)attention_decode_tc_kernel<HD, DT_STAGES, JOIN>, smem, sizeof(int));
+  if (g != cudaSuccess) return BN_ERR_LAUNCH + (int)g;
   if (a.cluster) {
-    cudaError_t e = bn_launch_cluster(attention_decode_tc_kernel<HD, DT_STAGES>, grid, dim3(DT_THREADS), smem, stream,
+    cudaError_t e = bn_launch_cluster(attention_decode_tc_kernel<HD, DT_STAGES, JOIN>, grid, dim3(DT_THREADS), smem, stream,
                                       cluster, mk, mv, a);
     if (e != cudaSuccess) return BN_ERR_LAUNCH + (int)e;
     return BN_OK;
   }
-  BN_LAUNCH((attention_decode_tc_kernel<HD, DT_STAGES>), grid, DT_THREADS, smem, stream, mk, mv, a);
+  BN_LAUNCH((attention_decode_tc_kernel<HD, DT_STAGES, JOIN>), grid, DT_THREADS, smem, stream, mk, mv, a);
   return BN_OK;
 }
 // How many blocks of a ring depth fit on the device at once (asked of the runtime once per kernel).
@@ -595,8 +623,8 @@ static long long dt_slots() {
   if (!slots) {
     size_t smem = dt_smem_bytes<HD, DT_STAGES>();
     int per_sm = 0, dev = 0, sms = 0;
-    cudaFuncSetAttribute(attention_decode_tc_kernel<HD, DT_STAGES>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, attention_decode_tc_kernel<HD, DT_STAGES>, DT_THREADS, smem) != cudaSuccess ||
+    cudaFuncSetAttribute(attention_decode_tc_kernel<HD, DT_STAGES, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, attention_decode_tc_kernel<HD, DT_STAGES, false>, DT_THREADS, smem) != cudaSuccess ||
         cudaGetDevice(&dev) != cudaSuccess ||
         cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || per_sm <= 0 || sms <= 0)
       slots = 2 * 148;
@@ -610,14 +638,14 @@ static long long dt_slots() {
 // share the SM (shared memory is the limit at head size 128): when that saves a wave of blocks it
 // wins although each block runs about an eighth slower (40 heads of 128, 2,000 positions, 8
 // sequences = 320 blocks: 77 us with three stages in two waves, 53 us with two stages in one).
-template <int HD>
+template <int HD, bool JOIN>
 static int launch_dt(const CUtensorMap& mk, const CUtensorMap& mv, const DtArgs& a, dim3 grid, dim3 cluster, cudaStream_t stream) {
-  if (a.pages_per_block <= 2) return launch_dt2<HD, 2>(mk, mv, a, grid, cluster, stream);
+  if (a.pages_per_block <= 2) return launch_dt2<HD, 2, JOIN>(mk, mv, a, grid, cluster, stream);
   const long long blocks = (long long)grid.x * grid.y * grid.z;
   const long long s3 = dt_slots<HD, 3>(), s2 = dt_slots<HD, 2>();
   const long long w3 = (blocks + s3 - 1) / s3, w2 = (blocks + s2 - 1) / s2;
-  if (w2 * 115 < w3 * 100) return launch_dt2<HD, 2>(mk, mv, a, grid, cluster, stream);
-  return launch_dt2<HD, 3>(mk, mv, a, grid, cluster, stream);
+  if (w2 * 115 < w3 * 100) return launch_dt2<HD, 2, JOIN>(mk, mv, a, grid, cluster, stream);
+  return launch_dt2<HD, 3, JOIN>(mk, mv, a, grid, cluster, stream);
 }
 
 // qkv: [n_seqs, q_stride] bfloat16 rows with the raw query heads first, the key heads at element
@@ -642,7 +670,8 @@ static int dt_run(const void* qkv, int q_stride, int k_off, int v_off, void* out
                   int rotary_dims, float theta_scale, const int* tok_pos, const int* slots,
                   const int* page_table, int pt_stride, void* k_cache, void* v_cache,
                   int n_cache_pages, int* status, float* part_o, float* part_ml, int n_splits, int pages_per_block, int* tickets,
-                  int n_tickets, const int* items, int n_items, int item_group, cudaStream_t stream) {
+                  int n_tickets, const int* items, int n_items, int item_group, const int* shared, const float* shared_o, const float* shared_ml,
+                  int n_shared, cudaStream_t stream) {
   if (n_seqs <= 0) return BN_OK;
   if (items != nullptr) {
     if (n_items <= 0 || item_group < 1 || item_group > 8 || n_items % item_group || n_seqs > 65535) return BN_ERR_BAD_ARG;
@@ -671,6 +700,7 @@ static int dt_run(const void* qkv, int q_stride, int k_off, int v_off, void* out
   a.cluster = (n_splits > 1 && n_splits <= 8) ? 1 : 0;  // few splits: one cluster per (sequence, head group)
   a.pages_per_block = pages_per_block; a.tickets = tickets; a.out = (__nv_bfloat16*)out; a.out_stride = out_stride;
   a.items = items;
+  a.shared = (const int4*)shared; a.shared_o = shared_o; a.shared_ml = shared_ml; a.n_shared = n_shared;
   dim3 grid(n_seqs, n_kv_heads * gblocks, n_splits), cluster(1, 1, n_splits);
   if (items != nullptr) {
     BN_TRACE_ONLY(a.trace = nullptr;)
@@ -681,9 +711,13 @@ static int dt_run(const void* qkv, int q_stride, int k_off, int v_off, void* out
   if (!tma_map_bf16_pages(&mk, k_cache, n_cache_pages, (unsigned long long)n_kv_heads * BN_PAGE, head_dim, BN_PAGE) ||
       !tma_map_bf16_pages(&mv, v_cache, n_cache_pages, (unsigned long long)n_kv_heads * BN_PAGE, head_dim, BN_PAGE))
     return BN_ERR_BAD_ARG;
-  if (head_dim <= 64) return launch_dt<64>(mk, mv, a, grid, cluster, stream);
-  if (head_dim <= 128) return launch_dt<128>(mk, mv, a, grid, cluster, stream);
-  return launch_dt<256>(mk, mv, a, grid, cluster, stream);
+  if (shared != nullptr) {
+    if (head_dim <= 64) return launch_dt<64, true>(mk, mv, a, grid, cluster, stream);
+    return launch_dt<128, true>(mk, mv, a, grid, cluster, stream);
+  }
+  if (head_dim <= 64) return launch_dt<64, false>(mk, mv, a, grid, cluster, stream);
+  if (head_dim <= 128) return launch_dt<128, false>(mk, mv, a, grid, cluster, stream);
+  return launch_dt<256, false>(mk, mv, a, grid, cluster, stream);
 }
 extern "C" int bn_attention_decode_tc(const void* qkv, int q_stride, int k_off, int v_off, void* out, int out_stride,
                                       int n_seqs, int n_heads, int n_kv_heads, int head_dim, float scale, int window,
@@ -693,7 +727,7 @@ extern "C" int bn_attention_decode_tc(const void* qkv, int q_stride, int k_off, 
                                       int n_tickets, cudaStream_t stream) {
   return dt_run(qkv, q_stride, k_off, v_off, out, out_stride, n_seqs, n_heads, n_kv_heads, head_dim, scale, window, rotary_dims,
                 theta_scale, tok_pos, slots, page_table, pt_stride, k_cache, v_cache, n_cache_pages, status, part_o, part_ml,
-                n_splits, pages_per_block, tickets, n_tickets, nullptr, 0, 0, stream);
+                n_splits, pages_per_block, tickets, n_tickets, nullptr, 0, 0, nullptr, nullptr, nullptr, 0, stream);
 }
 extern "C" int bn_attention_decode_tc_items(const void* qkv, int q_stride, int k_off, int v_off, void* out, int out_stride,
                                             int n_seqs, int n_heads, int n_kv_heads, int head_dim, float scale, int window,
@@ -704,5 +738,20 @@ extern "C" int bn_attention_decode_tc_items(const void* qkv, int q_stride, int k
   if (!items) return BN_ERR_BAD_ARG;
   return dt_run(qkv, q_stride, k_off, v_off, out, out_stride, n_seqs, n_heads, n_kv_heads, head_dim, scale, window, rotary_dims,
                 theta_scale, tok_pos, slots, page_table, pt_stride, k_cache, v_cache, n_cache_pages, status, part_o, part_ml,
-                1, 1, tickets, n_tickets, items, n_items, item_group, stream);
+                1, 1, tickets, n_tickets, items, n_items, item_group, nullptr, nullptr, nullptr, 0, stream);
+}
+// With the first shared[4 b] pages of each sequence b attended to by attention_shared.cu, launched directly in front (it lets this kernel start early): its
+// results shared[4 b + 1] .. + shared[4 b + 2] - 1 of shared_o / shared_ml are joined with those of the other pages, of which there is at least one (the
+// new token's).  n_splits blocks share a sequence's other pages, about
+// pages_per_block each.  No window, no rotation (the rows are rotated), head_dim at most 128.
+extern "C" int bn_attention_decode_tc_join(const void* qkv, int q_stride, int k_off, int v_off, void* out, int out_stride,
+                                           int n_seqs, int n_heads, int n_kv_heads, int head_dim, float scale, const int* tok_pos, const int* slots,
+                                           const int* page_table, int pt_stride, void* k_cache, void* v_cache,
+                                           int n_cache_pages, int* status, float* part_o, float* part_ml, int n_splits, int pages_per_block, int* tickets,
+                                           int n_tickets, const int* shared, const float* shared_o, const float* shared_ml, int n_shared,
+                                           cudaStream_t stream) {
+  if (!shared || !shared_o || !shared_ml || n_shared <= 0 || head_dim > 128 || (((uintptr_t)shared) & 15) || (((uintptr_t)shared_ml) & 7)) return BN_ERR_BAD_ARG;
+  return dt_run(qkv, q_stride, k_off, v_off, out, out_stride, n_seqs, n_heads, n_kv_heads, head_dim, scale, 0, 0, 1.0f, tok_pos, slots,
+                page_table, pt_stride, k_cache, v_cache, n_cache_pages, status, part_o, part_ml, n_splits, pages_per_block, tickets, n_tickets,
+                nullptr, 0, 0, shared, shared_o, shared_ml, n_shared, stream);
 }

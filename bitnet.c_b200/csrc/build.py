@@ -38,6 +38,7 @@ SOURCES: Dict[str, str] = {
     "attention": "attention.cu",
     "attention_decode": "attention_decode.cu",
     "attention_decode_tc": "attention_decode_tc.cu",
+    "attention_shared": "attention_shared.cu",
     "attention_prefill": "attention_prefill.cu",
     "attention_prefill_tc": "attention_prefill_tc.cu",
     "linear": "linear.cu",

@@ -1090,6 +1090,144 @@ def attention_decode_fused(qkv: torch.Tensor, k_off: int, v_off: int, out: torch
 
 
 # ---- matrix products ----------------------------------------------------------------------
+SHARED_ROWS = 128  # query rows of a block of attention_shared.cu (AS_ROWS)
+SHARED_MIN_PAGES = 2  # pages that a block of it walks at least, where a run has that many
+
+
+class SharedPlan:
+    """Which sequences of a decode step share which pages, as ``attention_decode_shared`` takes it: made by ``shared_plan``, good while no sequence
+    takes a new page (one that only fills its last page changes nothing).
+
+    ``first_own[b]``: so many of sequence b's first pages are read together with others'.  ``runs``: (sequences, first page, pages) of what is shared."""
+
+    def __init__(self, pages, n_heads: int, n_kv_heads: int, head_dim: int, device, sms: Optional[int] = None):
+        if n_kv_heads <= 0 or n_heads % n_kv_heads or n_heads // n_kv_heads > SHARED_ROWS or head_dim % 16 or not 0 < head_dim <= 128:
+            raise KernelError(f"shared_plan: heads {n_heads}/{n_kv_heads} of {head_dim} are not supported")
+        if any(len(p) == 0 for p in pages):
+            raise KernelError("shared_plan: a sequence without a page has no new token")
+        self.n_seqs, self.n_heads, self.n_kv_heads, self.head_dim = len(pages), n_heads, n_kv_heads, head_dim
+        self.device = torch.device(device)
+        self.runs, self.first_own = shared_runs([p[:-1] for p in pages])  # the last page takes the new token: it is nobody else's
+        self.own_pages = max((len(p) - f for p, f in zip(pages, self.first_own)), default=0)
+        self._lay_out(sms if sms is not None else n_sms(self.device))
+        self.table = torch.tensor(self.host, dtype=torch.int32)
+        if self.device.type == "cuda" and self.n_items:
+            self.table = self.table.pin_memory().to(self.device, non_blocking=True)
+
+    def _lay_out(self, sms: int) -> None:
+        """The list of work, ``host``: items (first member, members, first page, pages), members (sequence, place of its results), and of every sequence
+        (pages read together, first place, places, 0)."""
+        most = SHARED_ROWS // (self.n_heads // self.n_kv_heads)  # sequences of a block
+        tiles = [(members[i:i + most], first, n) for members, first, n in self.runs for i in range(0, len(members), most)]
+        # two blocks fit an SM: as many as run at once share all pages evenly
+        budget = max(1, 2 * sms // self.n_kv_heads)
+        each = max(SHARED_MIN_PAGES, -(-sum(n for _m, _f, n in tiles) // budget))
+        work = []
+        for members, first, n in tiles:
+            pieces = -(-n // each)
+            work += [(members, first + n * i // pieces, n * (i + 1) // pieces - n * i // pieces) for i in range(pieces)]
+        work.sort(key=lambda w: -w[2])  # the longest start first
+        count = [0] * self.n_seqs
+        for members, _first, _n in work:
+            for b in members:
+                count[b] += 1
+        place, at = [], 0
+        for c in count:
+            place.append(at)
+            at += c
+        self.n_parts, self.n_items = at, len(work)
+        items, entries, sequences = [], [], [x for b in range(self.n_seqs) for x in (self.first_own[b], place[b], count[b], 0)]
+        for members, first, n in work:
+            items += (len(entries) // 2, len(members), first, n)
+            for b in members:
+                entries += (b, place[b])
+                place[b] += 1
+        self.n_members = len(entries) // 2
+        self.host = items + sequences + entries  # (rows of four first: they are read 16 bytes at a time)
+        self.at = (0, len(items) + len(sequences), len(items))  # items, members, sequences
+
+
+def shared_runs(pages):
+    """Runs of pages that several sequences begin with alike: ([(sequences, first page, pages)], how many of each sequence's first pages lie in them).
+    Sequences forked from forks share several runs, one behind the other."""
+    runs, first_own = [], [0] * len(pages)
+
+    def walk(members, depth):
+        buckets = {}
+        for b in members:
+            if len(pages[b]) > depth:
+                buckets.setdefault(pages[b][depth], []).append(b)
+        for bucket in buckets.values():
+            if len(bucket) < 2:
+                continue
+            rest = [pages[b][depth:] for b in bucket]
+            low, high = min(rest), max(rest)  # what these two begin with alike, all do
+            n = next((i for i, (x, y) in enumerate(zip(low, high)) if x != y), min(len(low), len(high)))
+            runs.append((bucket, depth, n))
+            for b in bucket:
+                first_own[b] = depth + n
+            walk(bucket, depth + n)
+
+    walk(range(len(pages)), 0)
+    return runs, first_own
+
+
+def shared_plan(pages, n_heads: int, n_kv_heads: int, head_dim: int, device) -> SharedPlan:
+    """The plan of a decode step in which sequence b holds the pages ``pages[b]``, in order, up to the one that its new token goes to."""
+    return SharedPlan([list(p) for p in pages], n_heads, n_kv_heads, head_dim, device)
+
+
+def attention_decode_shared(qkv: torch.Tensor, k_off: int, v_off: int, out: torch.Tensor, n_seqs: int, n_heads: int, n_kv_heads: int, head_dim: int,
+                            scale: float, tok_pos: torch.Tensor, slots: torch.Tensor, page_table: torch.Tensor, k_cache: torch.Tensor,
+                            v_cache: torch.Tensor, plan: SharedPlan) -> torch.Tensor:
+    """``attention_decode_fused`` for sequences that share pages: pages that several of them begin with are read once for all (``plan``, of
+    ``shared_plan``), each sequence's own pages as ever, and the two are joined, in two launches.  ``qkv`` holds rotated q|k|v rows; the new key and
+    value are written into the cache at ``tok_pos``.  No window; heads of at most 128."""
+    _need(qkv, "qkv", torch.bfloat16, 2)
+    _need(out, "out", torch.bfloat16, 2)
+    for t, nm in ((tok_pos, "tok_pos"), (slots, "slots")):
+        _need(t, nm, torch.int32, 1)
+    _need(page_table, "page_table", torch.int32, 2)
+    _need(k_cache, "k_cache", torch.bfloat16, 4)
+    _need(v_cache, "v_cache", torch.bfloat16, 4)
+    device = qkv.device
+    if any(t.device != device for t in (out, tok_pos, slots, page_table, k_cache, v_cache)):
+        raise KernelError(f"attention_decode_shared: everything must lie on {device}")
+    if tuple(k_cache.shape[1:]) != (n_kv_heads, PAGE, head_dim) or k_cache.shape != v_cache.shape:
+        raise KernelError(f"attention_decode_shared: cache {tuple(k_cache.shape)} is not [pages, {n_kv_heads}, {PAGE}, {head_dim}]")
+    if (plan.n_seqs, plan.n_heads, plan.n_kv_heads, plan.head_dim) != (n_seqs, n_heads, n_kv_heads, head_dim) or (plan.n_items and plan.table.device != device):
+        raise KernelError(f"attention_decode_shared: the plan is for {plan.n_seqs} sequences, heads {plan.n_heads}/{plan.n_kv_heads} of {plan.head_dim} on "
+                          f"{plan.table.device}")
+    if min(k_off, v_off) < 0 or max(k_off, v_off) + n_kv_heads * head_dim > qkv.shape[1] or n_heads * head_dim > qkv.shape[1] or (k_off | v_off | qkv.shape[1]) % 8:
+        raise KernelError("attention_decode_shared: offsets run past the row, or row and offsets are no multiples of 8")
+    if (out.shape[0] < n_seqs or out.shape[1] != n_heads * head_dim or tok_pos.shape[0] < n_seqs or slots.shape[0] < n_seqs or qkv.shape[0] < n_seqs
+            or max(plan.first_own, default=0) >= page_table.shape[1]):
+        raise KernelError("attention_decode_shared: out, qkv, tok_pos, slots or page_table does not fit")
+    if not scale > 0:
+        raise KernelError(f"attention_decode_shared: scale={scale} must be positive")
+    with _on(device):
+        if not plan.n_items:
+            return attention_decode_fused(qkv, k_off, v_off, out, n_seqs, n_heads, n_kv_heads, head_dim, scale, 0, 0, 1.0, tok_pos, slots, page_table,
+                                          k_cache, v_cache, plan.own_pages * PAGE)
+        n_splits, pages_per_block = decode_grid(plan.own_pages * PAGE, n_seqs, n_heads, n_kv_heads)
+        _scr, counters = _split_scratch(device)
+        floats = lambda n: torch.empty(n, dtype=torch.float32, device=device)  # noqa: E731
+        shared_o, shared_ml = floats(plan.n_parts * n_heads * head_dim), floats(plan.n_parts * n_heads * 2)
+        part_o, part_ml = floats(n_seqs * n_heads * n_splits * head_dim), floats(n_seqs * n_heads * n_splits * 2)
+        items, members, sequences = (c_void_p(plan.table.data_ptr() + 4 * i) for i in plan.at)
+        status = _ptr(tc_status(device))
+        _check(_fn("attention_shared", "bn_attention_shared")(
+            _ptr(qkv), int(qkv.shape[1]), int(n_seqs), int(n_heads), int(n_kv_heads), int(head_dim), c_float(scale), items, plan.n_items, members,
+            plan.n_members, _ptr(slots), _ptr(page_table), int(page_table.shape[1]), _ptr(k_cache), _ptr(v_cache), int(k_cache.shape[0]), _ptr(shared_o),
+            _ptr(shared_ml), plan.n_parts, status, _stream()), "attention_decode_shared")
+        _check(_fn("attention_decode_tc", "bn_attention_decode_tc_join")(
+            _ptr(qkv), int(qkv.shape[1]), int(k_off), int(v_off), _ptr(out), int(out.shape[1]), int(n_seqs), int(n_heads), int(n_kv_heads), int(head_dim),
+            c_float(scale), _ptr(tok_pos), _ptr(slots), _ptr(page_table), int(page_table.shape[1]), _ptr(k_cache), _ptr(v_cache),
+            int(k_cache.shape[0]), status, _ptr(part_o), _ptr(part_ml), int(n_splits), int(pages_per_block), _ptr(counters), int(counters.numel()),
+            sequences, _ptr(shared_o), _ptr(shared_ml), plan.n_parts, _stream()), "attention_decode_shared")
+    return out
+
+
 SKINNY_MAX_ROWS = 16  # float32: warp-per-column kernel up to this many rows
 MMA_MAX_ROWS = 64  # bfloat16: the streaming kernels (linear_tc.cu, linear_mma.cu) up to this many rows; the library
 # product is faster beyond (5.5 against 5.8 ms for a decode step of 96 sequences at 32 layers of width 4096)
@@ -1172,7 +1310,8 @@ def check_tc_status(device) -> None:
                 5: "attention_prefill_tc: a wait inside the kernel gave up",
                 6: "linear_tc: a slice of partial sums from another block of the cluster never arrived",
                 7: "gemm_tc: a wait inside the kernel gave up",
-                8: "linear_split: a wait inside the kernel gave up"}.get(code, f"code {code}")
+                8: "linear_split: a wait inside the kernel gave up",
+                9: "attention_shared: a wait inside the kernel gave up"}.get(code, f"code {code}")
         raise KernelError(f"{what}; the result of that launch is not valid")
 
 
