@@ -247,6 +247,7 @@ class Cache:
                 self.states[i] = torch.zeros((n_slots,) + tuple(r.shape), dtype=r.dtype, device=device)
                 if isinstance(i, tuple):
                     self._named.setdefault(i[0], {})[i[1]] = self.states[i]
+        self.turns = 0  # goes up when a sequence is forked or ends: who shares what with whom may then be another
         self._state_slots = None  # the same for copying a slot of all of them, made when a sequence is first forked
         self._state_rows = None  # where the states lie, for zeroing a slot of all of them in one launch
         if self.states and torch.device(device).type == "cuda":
@@ -284,6 +285,7 @@ class Cache:
             raise
         for s in new:
             self.slots.set_length(s, length)
+        self.turns += 1
         for g, m in zip(self.groups, moves):
             g.copy(m)
         if self.states:
@@ -310,6 +312,7 @@ class Cache:
         for g in self.groups:
             g.release(slot)
         self.slots.close(slot)
+        self.turns += 1
 
     def length(self, slot: int) -> int:
         return self.slots.length(slot)
@@ -356,6 +359,14 @@ class Cache:
             g.page_table.index_copy_(0, idx.to(self.device, non_blocking=True),
                                      staged.to(self.device, non_blocking=True))
             g.dirty.clear()
+
+    def shares_pages(self) -> bool:
+        """Whether any page is held by more than one sequence."""
+        return any(g.pool.n_shared for g in self.groups)
+
+    def pages_of(self, entry: int, slot: int, n: int) -> List[int]:
+        """The first ``n`` pages of the sequence in ``slot``, in order, in the group of schedule entry ``entry`` (one that keeps all of a sequence)."""
+        return self.groups[self._plane[entry][0]].host_table[slot, :n].tolist()
 
     # ---- views ----------------------------------------------------------------------------
     def view(self, entry: int) -> Optional[KvView]:

@@ -36,6 +36,7 @@ class PagePool:
         self.n_pages = n_pages
         self._free: List[int] = list(range(n_pages - 1, -1, -1))  # pop() hands out 0 first
         self._held = [0] * n_pages  # how often each page is held
+        self.n_shared = 0  # pages that are held more than once
 
     @property
     def n_free(self) -> int:
@@ -62,6 +63,7 @@ class PagePool:
             if not 0 <= p < self.n_pages or not self._held[p]:
                 raise CacheError(f"page {p} cannot be shared: nothing holds it")
             self._held[p] += 1
+            self.n_shared += self._held[p] == 2
 
     def renumber(self, new_id: Dict[int, int]) -> None:
         """Held pages change their ids (the free ones are then handed out lowest first): ``new_id`` names every held page."""
@@ -78,6 +80,7 @@ class PagePool:
             if not self._held[p]:
                 raise CacheError(f"page {p} is freed twice")
             self._held[p] -= 1
+            self.n_shared -= self._held[p] == 1
             if not self._held[p]:
                 self._free.append(p)
 
@@ -85,6 +88,8 @@ class PagePool:
         """Every page is exactly once either free or held."""
         if len(set(self._free)) != len(self._free):
             raise CacheError("a page is on the free list twice")
+        if self.n_shared != sum(h > 1 for h in self._held):
+            raise CacheError(f"{self.n_shared} shared pages counted, there are {sum(h > 1 for h in self._held)}")
         free = set(self._free)
         for p in range(self.n_pages):
             if (self._held[p] > 0) == (p in free):

@@ -5,6 +5,7 @@ Option names and meanings are the reference's where it has them: ``-p``, ``--pro
 ``--quiet``, ``--token-ids``, ``--benchmark-runs``, ``--benchmark-warmup-runs``, with the same defaults
 (256 tokens, temperature 0 = greedy, top-p 0.9, seed 42, repeat penalty 1.1 over 64 tokens).  The model
 is a folder with ``config.json`` and ``model.safetensors`` instead of a GGUF file.  New here:
+``--topk``, ``--minp`` and ``--completions`` (several of one prompt);
 ``--random-weights`` writes such a folder from ``--config`` and ``--weight-seed``; ``--dtype`` picks
 bfloat16 or true float32; ``--prompt-token-ids`` may be given several times for a batch.  Options of
 the reference that select CPU threads, other backends, quantized caches, speculative decoding, chat
@@ -48,6 +49,10 @@ def build_parser() -> argparse.ArgumentParser:
     ap.add_argument("-n", dest="n_tokens", type=int, default=256, help="number of tokens to generate (default 256; 0 = prompt only)")
     ap.add_argument("--temp", type=float, default=0.0, help="temperature (default 0.0 = greedy)")
     ap.add_argument("--topp", type=float, default=0.9, help="top-p sampling, used when temperature > 0 (default 0.9)")
+    ap.add_argument("--topk", type=int, default=0, help="keep the k most probable tokens, used when temperature > 0 (default 0 = all)")
+    ap.add_argument("--minp", type=float, default=0.0,
+                    help="keep tokens of at least this share of the most probable one's probability, used when temperature > 0 (default 0 = all)")
+    ap.add_argument("--completions", type=int, default=1, help="completions of every prompt; the prompt is run once (default 1)")
     ap.add_argument("--seed", type=int, default=42, help="random seed (default 42)")
     ap.add_argument("--maxseq", type=int, default=0, help="max sequence length (default: model max)")
     ap.add_argument("--repeat-penalty", type=float, default=1.1, help="repetition penalty over the last 64 tokens (default 1.1)")
@@ -84,6 +89,8 @@ def main(argv=None) -> int:
             cfg = json.load(f)
         bn.write_random_model(args.model, cfg, args.weight_seed if args.weight_seed is not None else args.seed,
                               dtype=args.dtype)
+    if args.no_prefill and args.completions != 1:
+        raise SystemExit("--no-prefill feeds every prompt by itself: it does not go with --completions")
     if args.prompt is not None and not args.prompt_token_ids:
         raise SystemExit("-p needs a tokenizer and none ships with this library; give --prompt-token-ids a,b,c")
     if not args.prompt_token_ids:
@@ -124,14 +131,15 @@ def main(argv=None) -> int:
         else:
             results = bn.generate(model, prompts, max_new, temperature=args.temp, top_p=args.topp, seed=args.seed,
                                   repeat_penalty=args.repeat_penalty, stop_ids=stop_ids,
-                                  callback=emit if args.token_ids and measured else None, loop_abort=args.loop_abort)
+                                  callback=emit if args.token_ids and measured else None, loop_abort=args.loop_abort,
+                                  top_k=args.topk, min_p=args.minp, completions=args.completions)
         torch.cuda.synchronize()
         total_ms = (time.time() - t1) * 1e3
         n_out = sum(len(r.tokens) for r in results)
         if measured:
             print(f"Generation complete tokens={n_out} tok/s={n_out / max(total_ms, 1e-9) * 1e3:.2f} "
                   f"prompt_tokens={sum(len(p) for p in prompts)} total_ms={total_ms:.1f} load_ms={load_ms:.1f} "
-                  f"requests={len(prompts)} dtype={args.dtype}", file=sys.stderr, flush=True)
+                  f"requests={len(results)} dtype={args.dtype}", file=sys.stderr, flush=True)
     if model.diagnostics is not None:
         for line in model.diagnostics.profile_lines():
             print(line, file=sys.stderr)
@@ -162,7 +170,7 @@ def _generate_no_prefill(bn, model, prompts, max_new, args, stop_ids, emit):
     S = model.spec.max_positions
     need = sum(pages_for(min(len(p) + m, S)) * PAGE for p, m in zip(prompts, max_new))
     cache = model.new_cache(max_tokens=max(need, PAGE), max_seqs=len(prompts))
-    params = SamplingParams(temperature=args.temp, top_p=args.topp, seed=args.seed, repeat_penalty=args.repeat_penalty)
+    params = SamplingParams(temperature=args.temp, top_p=args.topp, seed=args.seed, repeat_penalty=args.repeat_penalty, top_k=args.topk, min_p=args.minp)
     stops = tuple(model.spec.stop_ids) if stop_ids is None else tuple(stop_ids)
     return generate(OneByOne(model, cache, params), prompts, max_new, stop_ids=stops,
                     callback=emit if args.token_ids else None, loop_abort=args.loop_abort)

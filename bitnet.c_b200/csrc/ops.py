@@ -1090,6 +1090,7 @@ def attention_decode_fused(qkv: torch.Tensor, k_off: int, v_off: int, out: torch
 
 
 # ---- matrix products ----------------------------------------------------------------------
+USE_SHARED_PAGES = True  # decode steps of sequences that share pages read them once for all (tests switch it)
 SHARED_ROWS = 128  # query rows of a block of attention_shared.cu (AS_ROWS)
 SHARED_MIN_PAGES = 2  # pages that a block of it walks at least, where a run has that many
 
@@ -1098,30 +1099,44 @@ class SharedPlan:
     """Which sequences of a decode step share which pages, as ``attention_decode_shared`` takes it: made by ``shared_plan``, good while no sequence
     takes a new page (one that only fills its last page changes nothing).
 
-    ``first_own[b]``: so many of sequence b's first pages are read together with others'.  ``runs``: (sequences, first page, pages) of what is shared."""
+    ``first_own[b]``: so many of sequence b's first pages are read together with others'.  ``runs``: (sequences, first page, pages) of what is shared.
+    ``room`` = (items, places) pads the list of work to that size, for a recorded step whose list is data; ``fits`` is then false if it is too long for it."""
 
-    def __init__(self, pages, n_heads: int, n_kv_heads: int, head_dim: int, device, sms: Optional[int] = None):
+    def __init__(self, pages, n_heads: int, n_kv_heads: int, head_dim: int, device, sms: Optional[int] = None, room=None):
         if n_kv_heads <= 0 or n_heads % n_kv_heads or n_heads // n_kv_heads > SHARED_ROWS or head_dim % 16 or not 0 < head_dim <= 128:
             raise KernelError(f"shared_plan: heads {n_heads}/{n_kv_heads} of {head_dim} are not supported")
         if any(len(p) == 0 for p in pages):
             raise KernelError("shared_plan: a sequence without a page has no new token")
         self.n_seqs, self.n_heads, self.n_kv_heads, self.head_dim = len(pages), n_heads, n_kv_heads, head_dim
+        self.heads = (n_heads, n_kv_heads, head_dim)
         self.device = torch.device(device)
         self.runs, self.first_own = shared_runs([p[:-1] for p in pages])  # the last page takes the new token: it is nobody else's
         self.own_pages = max((len(p) - f for p, f in zip(pages, self.first_own)), default=0)
-        self._lay_out(sms if sms is not None else n_sms(self.device))
-        self.table = torch.tensor(self.host, dtype=torch.int32)
-        if self.device.type == "cuda" and self.n_items:
-            self.table = self.table.pin_memory().to(self.device, non_blocking=True)
+        self.fits = self._lay_out(sms if sms is not None else n_sms(self.device), room)
+        self.table = None
 
-    def _lay_out(self, sms: int) -> None:
-        """The list of work, ``host``: items (first member, members, first page, pages), members (sequence, place of its results), and of every sequence
-        (pages read together, first place, places, 0)."""
+    def upload(self, to: Optional[torch.Tensor] = None) -> "SharedPlan":
+        """Bring the list of work to the device (into ``to``, if given)."""
+        host = torch.tensor(self.host, dtype=torch.int32)
+        if self.device.type == "cuda":
+            host = host.pin_memory()
+        self.table = host.to(self.device, non_blocking=True) if to is None else to
+        if to is not None:
+            to[:host.numel()].copy_(host, non_blocking=True)
+        return self
+
+    def _lay_out(self, sms: int, room) -> bool:
+        """The list of work, ``host``: items (first member, members, first page, pages), of every sequence (pages read together, first place of its
+        results, places, 0), and members (sequence, place)."""
         most = SHARED_ROWS // (self.n_heads // self.n_kv_heads)  # sequences of a block
         tiles = [(members[i:i + most], first, n) for members, first, n in self.runs for i in range(0, len(members), most)]
         # two blocks fit an SM: as many as run at once share all pages evenly
         budget = max(1, 2 * sms // self.n_kv_heads)
-        each = max(SHARED_MIN_PAGES, -(-sum(n for _m, _f, n in tiles) // budget))
+        longest = max((n for _m, _f, n in tiles), default=1)
+        each = min(longest, max(SHARED_MIN_PAGES, -(-sum(n for _m, _f, n in tiles) // budget)))
+        if room is not None:
+            while each < longest and (sum(-(-n // each) for _m, _f, n in tiles) > room[0] or sum(-(-n // each) * len(m) for m, _f, n in tiles) > room[1]):
+                each = min(longest, 2 * each)
         work = []
         for members, first, n in tiles:
             pieces = -(-n // each)
@@ -1142,9 +1157,15 @@ class SharedPlan:
             for b in members:
                 entries += (b, place[b])
                 place[b] += 1
-        self.n_members = len(entries) // 2
+        if room is not None:
+            if self.n_items > room[0] or self.n_parts > room[1]:
+                return False
+            items += [0] * (4 * (room[0] - self.n_items))  # items without members: nothing to do
+            entries += [0] * (2 * (room[1] - self.n_parts))
+            self.n_items, self.n_parts = room
         self.host = items + sequences + entries  # (rows of four first: they are read 16 bytes at a time)
         self.at = (0, len(items) + len(sequences), len(items))  # items, members, sequences
+        return True
 
 
 def shared_runs(pages):
@@ -1174,7 +1195,12 @@ def shared_runs(pages):
 
 def shared_plan(pages, n_heads: int, n_kv_heads: int, head_dim: int, device) -> SharedPlan:
     """The plan of a decode step in which sequence b holds the pages ``pages[b]``, in order, up to the one that its new token goes to."""
-    return SharedPlan([list(p) for p in pages], n_heads, n_kv_heads, head_dim, device)
+    return SharedPlan([list(p) for p in pages], n_heads, n_kv_heads, head_dim, device).upload()
+
+
+def shared_pays(plan: SharedPlan) -> bool:
+    """Whether ``attention_decode_shared`` gains anything over every sequence reading its pages for itself."""
+    return bool(plan.runs)
 
 
 def attention_decode_shared(qkv: torch.Tensor, k_off: int, v_off: int, out: torch.Tensor, n_seqs: int, n_heads: int, n_kv_heads: int, head_dim: int,
@@ -1195,9 +1221,9 @@ def attention_decode_shared(qkv: torch.Tensor, k_off: int, v_off: int, out: torc
         raise KernelError(f"attention_decode_shared: everything must lie on {device}")
     if tuple(k_cache.shape[1:]) != (n_kv_heads, PAGE, head_dim) or k_cache.shape != v_cache.shape:
         raise KernelError(f"attention_decode_shared: cache {tuple(k_cache.shape)} is not [pages, {n_kv_heads}, {PAGE}, {head_dim}]")
-    if (plan.n_seqs, plan.n_heads, plan.n_kv_heads, plan.head_dim) != (n_seqs, n_heads, n_kv_heads, head_dim) or (plan.n_items and plan.table.device != device):
+    if (plan.n_seqs, plan.n_heads, plan.n_kv_heads, plan.head_dim) != (n_seqs, n_heads, n_kv_heads, head_dim) or plan.table is None or plan.table.device != device:
         raise KernelError(f"attention_decode_shared: the plan is for {plan.n_seqs} sequences, heads {plan.n_heads}/{plan.n_kv_heads} of {plan.head_dim} on "
-                          f"{plan.table.device}")
+                          f"{plan.device}")
     if min(k_off, v_off) < 0 or max(k_off, v_off) + n_kv_heads * head_dim > qkv.shape[1] or n_heads * head_dim > qkv.shape[1] or (k_off | v_off | qkv.shape[1]) % 8:
         raise KernelError("attention_decode_shared: offsets run past the row, or row and offsets are no multiples of 8")
     if (out.shape[0] < n_seqs or out.shape[1] != n_heads * head_dim or tok_pos.shape[0] < n_seqs or slots.shape[0] < n_seqs or qkv.shape[0] < n_seqs
@@ -1218,7 +1244,7 @@ def attention_decode_shared(qkv: torch.Tensor, k_off: int, v_off: int, out: torc
         status = _ptr(tc_status(device))
         _check(_fn("attention_shared", "bn_attention_shared")(
             _ptr(qkv), int(qkv.shape[1]), int(n_seqs), int(n_heads), int(n_kv_heads), int(head_dim), c_float(scale), items, plan.n_items, members,
-            plan.n_members, _ptr(slots), _ptr(page_table), int(page_table.shape[1]), _ptr(k_cache), _ptr(v_cache), int(k_cache.shape[0]), _ptr(shared_o),
+            plan.n_parts, _ptr(slots), _ptr(page_table), int(page_table.shape[1]), _ptr(k_cache), _ptr(v_cache), int(k_cache.shape[0]), _ptr(shared_o),
             _ptr(shared_ml), plan.n_parts, status, _stream()), "attention_decode_shared")
         _check(_fn("attention_decode_tc", "bn_attention_decode_tc_join")(
             _ptr(qkv), int(qkv.shape[1]), int(k_off), int(v_off), _ptr(out), int(out.shape[1]), int(n_seqs), int(n_heads), int(n_kv_heads), int(head_dim),

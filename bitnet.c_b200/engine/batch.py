@@ -52,6 +52,8 @@ class StepContext:
     # (``ops.decode_items``), in groups of ``decode_item_group``; None: every sequence alike
     decode_items: Optional[torch.Tensor] = None
     decode_item_group: int = 0
+    # a decode step of sequences that share pages (``ops.SharedPlan``); None: every sequence reads its pages for itself
+    shared: Optional[object] = None
     host_new: List[int] = field(default_factory=list)  # the same facts on the host, for parts that
     host_pos0: List[int] = field(default_factory=list)  # loop over sequences there
     host_slots: List[int] = field(default_factory=list)

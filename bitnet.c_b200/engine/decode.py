@@ -22,9 +22,13 @@ from typing import List, Optional, Sequence
 import numpy as np
 import torch
 
-from ..cache import Cache
+from ..cache import PAGE, Cache
+from ..csrc import ops
 from ..sampling import Sampler
 from .batch import StepContext
+
+
+SHARED_PLACES = 24  # results of shared pages per sequence that a recorded step has room for (ops.SharedPlan cuts its runs into fewer pieces to fit)
 
 
 class DecodeRunner:
@@ -52,15 +56,23 @@ class DecodeRunner:
         self.host_items: Optional[List[int]] = None  # what the device buffer holds
         self.items_for = None  # (bucket, page counts) that ``next_items`` was made for
         self.next_items: List[int] = []
-        self.graphs = {}  # length bucket -> recorded graph
+        # Sequences that share pages: what is shared is data in a buffer of fixed size (``ops.SharedPlan``), the longest run of own
+        # pages a bucket like that of the lengths.
+        heads = model.shared_heads()
+        self.shared_room = None
+        if heads is not None:
+            self.shared_room = (2 * ops.n_sms(dev) // heads[0][1] + B, SHARED_PLACES * B)
+            self.shared_table = torch.zeros(4 * self.shared_room[0] + 4 * B + 2 * self.shared_room[1], dtype=torch.int32, device=dev)
+        self.shared_for = None  # (slots, page counts, the cache's turns) that ``ctx.shared`` was made for
+        self.graphs = {}  # (length bucket, bucket of own pages where pages are shared) -> recorded graph
         self.pool = pool
-        self.warmed = False
+        self.warmed = set()  # whether a step with and without shared pages has run
         self.host_slots: Optional[List[int]] = None
         self.host_rows: Optional[List[int]] = None
         self.host_pos: Optional[List[int]] = None
         self.expect_tokens: Optional[List[int]] = None
         self.uploads = 0
-        self.launches_per_step = 0
+        self.launches_per_step = {}
 
     def _body(self) -> None:
         logits = self.model.forward(self.cache, self.ctx)
@@ -80,40 +92,61 @@ class DecodeRunner:
             self.uploads += 1
             self.h2d_bytes += host.numel() * 4
         self.host_slots, self.host_rows = slots, rows
-        from ..csrc import ops
         bucket = 1024
         while bucket < max(positions) + 1:
             bucket *= 2
         self.ctx.max_len = min(bucket, self.cache.max_positions)
+        self._shared_pages(slots, positions)
+        kind = self.ctx.shared is not None
         self._work_list(positions)
-        if not self.warmed:
+        if kind not in self.warmed:
             # the first step runs directly: kernels and libraries finish their lazy set-up,
             # which must not happen under capture
             before = ops.LAUNCHES
             self._body()
-            self.launches_per_step = ops.LAUNCHES - before
-            self.warmed = True
+            self.launches_per_step[kind] = ops.LAUNCHES - before
+            self.warmed.add(kind)
         else:
-            g = self.graphs.get(self.ctx.max_len)
+            key = (self.ctx.max_len, self.ctx.shared.own_pages if kind else 0)
+            g = self.graphs.get(key)
             if g is None:
                 g = torch.cuda.CUDAGraph()
                 before = ops.LAUNCHES
                 with torch.cuda.graph(g, pool=self.pool):
                     self._body()
                 ops.LAUNCHES = before  # recording launches nothing
-                self.graphs[self.ctx.max_len] = g
+                self.graphs[key] = g
             self.model.note_pass()
             g.replay()
-            ops.LAUNCHES += self.launches_per_step  # the replay launches every recorded kernel
+            ops.LAUNCHES += self.launches_per_step[kind]  # the replay launches every recorded kernel
         self.host_pos = [p + 1 for p in positions]
         self.expect_tokens = None  # known once the caller has read ``sampled``
         return self.sampled
 
+    def _shared_pages(self, slots: Sequence[int], positions: Sequence[int]) -> None:
+        """Bring what the sequences share up to date: it changes when one of them takes a new page, and when one is forked or ends."""
+        if self.shared_room is None:
+            return
+        now = (slots, [p // PAGE + 1 for p in positions], self.cache.turns) if self.cache.shares_pages() else None
+        if now == self.shared_for:
+            return
+        self.shared_for = now
+        before, self.ctx.shared = self.ctx.shared, None
+        plan = self.model.shared_pages(self.cache, slots, positions, room=self.shared_room) if now is not None else None
+        if plan is not None:
+            bucket = 4
+            while bucket < plan.own_pages:
+                bucket *= 2
+            plan.own_pages = bucket
+            if before is None or before.host != plan.host:
+                self.h2d_bytes += 4 * len(plan.host)
+                plan.upload(self.shared_table)
+            plan.table = self.shared_table
+            self.ctx.shared = plan
+
     def _work_list(self, positions: Sequence[int]) -> None:
         """Bring the work list of this step's bucket up to date (the grid's shape was fixed when the
         bucket was first met)."""
-        from ..cache.pages import PAGE
-        from ..csrc import ops
         bucket, B = self.ctx.max_len, self.batch
         pages = [p // PAGE + 1 for p in positions]
         group = self.item_group.get(bucket)

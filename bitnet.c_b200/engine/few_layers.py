@@ -102,7 +102,7 @@ class FewLayers:
     def takes(self, model, cache, ctx):
         """What ``run`` needs for a step of these tokens: the layers, where their matrices lie, and where their keys and values lie.  None if the step does not go this
         way; every switch that sends a part elsewhere sends the step there too."""
-        if not (ctx.n_tokens <= ops.TC_MAX_ROWS and ctx.diag is None and ops.PROFILE is None and ops.USE_TCGEN05 and ops.USE_FUSED_NORM
+        if not (ctx.n_tokens <= ops.TC_MAX_ROWS and ctx.diag is None and ctx.shared is None and ops.PROFILE is None and ops.USE_TCGEN05 and ops.USE_FUSED_NORM
                 and (ctx.decode or (ctx.wide_tile_seq is not None and ops.USE_TCGEN05_ATTENTION))):
             return None
         layers = _layers(model)

@@ -56,6 +56,14 @@ class Engine:
         """A new batch begins; row r of the batch is request ``first_index + r``."""
         raise NotImplementedError
 
+    def prefill(self, seqs: Sequence[SeqStep]) -> None:
+        """Run one step that wants no logits."""
+        raise NotImplementedError
+
+    def fork(self, slot: int, n: int) -> List[int]:
+        """``n`` more sequences that go on from where the one in ``slot`` is: their slots."""
+        raise NotImplementedError
+
     def step_and_sample(self, seqs: Sequence[SeqStep], rows: Sequence[int]) -> List[int]:
         """Run one step (logits wanted at each sequence's last token) and sample one token per
         sequence; ``rows[i]`` is the batch row of ``seqs[i]``."""
@@ -66,14 +74,17 @@ class Engine:
 
 
 def plan_batch(prompts: Sequence[Sequence[int]], max_new: Sequence[int], start: int, free_tokens: int,
-               max_batch: int, max_positions: int) -> int:
+               max_batch: int, max_positions: int, completions: int = 1) -> int:
     """How many requests from ``start`` on form the next batch: as many as fit, in order, counting
-    for each the pages its prompt and its new tokens can come to hold."""
+    for each the pages its prompt and its new tokens can come to hold.  Every ``completions`` requests in a row have one prompt; those of them
+    that are in the batch hold the full pages of all of it but its last token once."""
     n, used = 0, 0
     for i in range(start, len(prompts)):
         if n >= max_batch:
             break
         need = pages_for(min(len(prompts[i]) + max_new[i], max_positions)) * PAGE
+        if i % completions and i > start:
+            need -= (len(prompts[i]) - 1) // PAGE * PAGE
         if used + need > free_tokens:
             break
         used += need
@@ -95,12 +106,38 @@ def closes_a_loop(sampled: Sequence[int]) -> bool:
     return len(sampled) >= 2 * n and list(sampled[-n:]) == list(sampled[-2 * n:-n])
 
 
+def _fork_prompts(engine: Engine, live: Sequence[int], feed, completions: int):
+    """The slots of requests of which several have one prompt: all of a prompt but its last token is run once, and what that left is forked;
+    each request then brings the last token itself, and samples from logits of its own."""
+    siblings = {}
+    for i in live:
+        siblings.setdefault(i // completions, []).append(i)
+    slots = {group[0]: engine.open() for group in siblings.values()}
+    heads = [SeqStep(slots[g[0]], feed[g[0]][:-1], []) for g in siblings.values() if len(g) > 1 and len(feed[g[0]]) > 1]
+    if heads:
+        engine.prefill(heads)
+    for group in siblings.values():
+        if len(group) > 1:
+            slots.update(zip(group[1:], engine.fork(slots[group[0]], len(group) - 1)))
+            for i in group:
+                feed[i] = feed[i][-1:]
+    return slots
+
+
 def generate(engine: Engine, prompts: Sequence[Sequence[int]], max_new_tokens, stop_ids: Sequence[int] = (),
              callback: Optional[Callable[[int, int], bool]] = None, max_batch: Optional[int] = None,
-             loop_abort: bool = False) -> List[Completion]:
+             loop_abort: bool = False, completions: int = 1) -> List[Completion]:
     """Serve every prompt.  ``max_new_tokens`` is one number or one per prompt; ``callback(request,
     token)`` is called for every emitted token and stops that request when it returns true;
-    ``loop_abort`` ends a request whose last four sampled tokens repeat the four before them."""
+    ``loop_abort`` ends a request whose last four sampled tokens repeat the four before them.
+    ``completions``: so many requests are made of every prompt (prompt i's are requests i * completions and on, each with random numbers
+    of its own); the prompt is run once and its sequence forked."""
+    if completions < 1:
+        raise ValueError(f"completions={completions} must be at least 1")
+    if completions > 1:
+        if not isinstance(max_new_tokens, int):
+            max_new_tokens = [m for m in max_new_tokens for _ in range(completions)]
+        prompts = [p for p in prompts for _ in range(completions)]
     n_req = len(prompts)
     max_new = [int(max_new_tokens)] * n_req if isinstance(max_new_tokens, int) else [int(m) for m in max_new_tokens]
     if len(max_new) != n_req:
@@ -117,7 +154,7 @@ def generate(engine: Engine, prompts: Sequence[Sequence[int]], max_new_tokens, s
     start = 0
     while start < n_req:
         limit = min(max_batch or engine.max_batch(), engine.max_batch())
-        count = plan_batch(prompts, max_new, start, engine.free_tokens(), limit, engine.max_positions)
+        count = plan_batch(prompts, max_new, start, engine.free_tokens(), limit, engine.max_positions, completions)
         ids = list(range(start, start + count))
         start += count
         # -n 0: nothing is generated and nothing needs to run (the reference prefills without
@@ -129,9 +166,12 @@ def generate(engine: Engine, prompts: Sequence[Sequence[int]], max_new_tokens, s
         if not live:
             continue
         engine.start_batch(ids[0], [prompts[i] for i in ids])
-        slots = {i: engine.open() for i in live}
         length = {i: len(prompts[i]) for i in live}
         feed = {i: list(prompts[i]) for i in live}  # the prompts go in one step
+        if completions == 1:
+            slots = {i: engine.open() for i in live}
+        else:
+            slots = _fork_prompts(engine, live, feed, completions)
         while live:
             seqs = [SeqStep(slots[i], feed[i], [len(feed[i]) - 1]) for i in live]
             rows = [i - ids[0] for i in live]

@@ -14,7 +14,7 @@ from typing import Any, Dict, List, Optional, Sequence
 
 import torch
 
-from ..cache import Cache, CacheFull
+from ..cache import PAGE, Cache, CacheFull
 from ..config import ConfigError, ModelSpec, architecture_of, read_config_json
 from ..csrc import build as kernel_build
 from ..csrc import ops
@@ -102,6 +102,26 @@ class Model:
         """The most thread blocks any part launches per sequence in a decode step (0: no part takes
         a work list); what ``DecodeRunner`` sizes a batch's work list by."""
         return max((b.decode_blocks_per_sequence() for b in self.blocks), default=0)
+
+    def shared_heads(self):
+        """((query heads, key/value heads, head size), a schedule entry that has them) if there is a mixer that can read pages that sequences share
+        once for all of them; of several kinds of heads the first in the schedule."""
+        for i, e in enumerate(self.spec.schedule):
+            asks = getattr(getattr(self.blocks[e.block], "mixer", None), "shared_heads", None)
+            heads = asks() if asks is not None and e.cache_of is None else None
+            if heads is not None:
+                return heads, i
+        return None
+
+    def shared_pages(self, cache: Cache, slots: Sequence[int], lengths: Sequence[int], room=None):
+        """For a decode step of these sequences (``lengths``: before it): the plan of what they share, not yet on the device, or None if that is nothing, too
+        little to pay, or nothing that a mixer of this model can make use of."""
+        found = self.shared_heads() if cache.shares_pages() and ops.USE_SHARED_PAGES else None
+        if found is None:
+            return None
+        heads, entry = found
+        plan = ops.SharedPlan([cache.pages_of(entry, s, n // PAGE + 1) for s, n in zip(slots, lengths)], *heads, self.device, room=room)
+        return plan if plan.fits and ops.shared_pays(plan) else None
 
     def kernel_families(self) -> List[str]:
         # (a model in bfloat16 may have parameters that stay float32: their products of many rows are linear_split's)
@@ -245,6 +265,9 @@ class Model:
         try:
             cache.sync()
             ctx = pack_step(seqs, lengths, self.device)
+            if ctx.decode:
+                plan = self.shared_pages(cache, [s.slot for s in seqs], lengths)
+                ctx.shared = plan.upload() if plan is not None else None
             logits = self.forward(cache, ctx)
         except BaseException:
             for s in seqs:  # the step did not happen: its pages go back, the lengths stay

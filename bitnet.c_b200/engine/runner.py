@@ -60,6 +60,12 @@ class ModelEngine(Engine):
             self._check_kernels()
         self.cache.close(slot)
 
+    def prefill(self, seqs: Sequence[SeqStep]) -> None:
+        self.model.step(self.cache, seqs)
+
+    def fork(self, slot: int, n: int) -> List[int]:
+        return self.cache.fork(slot, n)
+
     def start_batch(self, first_index: int, prompts: Sequence[Sequence[int]]) -> None:
         """A new batch: its sampler rows are seeded and filled.  The sampler's device buffers are
         kept from batch to batch while they are large enough, so that the recorded decode graphs
@@ -129,24 +135,31 @@ def generate_with_model(model: Model, prompts: Sequence[Sequence[int]], max_new_
                         repeat_penalty: float = 1.0, repeat_window: int = 64,
                         stop_ids: Optional[Sequence[int]] = None, max_batch: Optional[int] = None,
                         cache: Optional[Cache] = None, max_tokens: Optional[int] = None,
-                        callback=None, loop_abort: bool = False) -> List[Completion]:
-    """Generate for every prompt (lists of token ids).  ``stop_ids`` default to the model's
+                        callback=None, loop_abort: bool = False, top_k: int = 0, min_p: float = 0.0,
+                        completions: int = 1) -> List[Completion]:
+    """Generate for every prompt (lists of token ids), ``completions`` times for each (prompt i's are results i * completions and on: its
+    prompt is run once, and what its completions share of the cache is held and read once).  ``stop_ids`` default to the model's
     end-of-sequence ids.  The cache is sized for the whole call unless ``max_tokens`` or a
     ``cache`` is given; requests that do not fit together run in batches one after another.
     ``loop_abort``: the reference's loop detector (off by default here)."""
     from ..cache.pages import PAGE, pages_for
     params = SamplingParams(temperature=temperature, top_p=top_p, seed=seed, repeat_penalty=repeat_penalty,
-                            repeat_window=repeat_window)
+                            repeat_window=repeat_window, top_k=top_k, min_p=min_p)
     n = len(prompts)
     mx = [int(max_new_tokens)] * n if isinstance(max_new_tokens, int) else [int(m) for m in max_new_tokens]
     if cache is None:
         S = model.spec.max_positions
+        copies = max(1, completions)
+        # of every completion the pages it can come to hold; the full ones of its prompt (all but the last token) are held once
+        whole = [pages_for(min(len(p) + m, S)) * PAGE for p, m in zip(prompts, mx)]
+        more = [w - max(0, len(p) - 1) // PAGE * PAGE for w, p in zip(whole, prompts)]
         if max_batch:
-            per = sorted((pages_for(min(len(p) + m, S)) * PAGE for p, m in zip(prompts, mx)), reverse=True)
+            # (a batch may begin anywhere among a prompt's completions)
+            per = sorted((x for w, m in zip(whole, more) for x in [w] + [m if max_batch >= copies else w] * (copies - 1)), reverse=True)
             need = sum(per[:max_batch])
         else:
-            need = sum(pages_for(min(len(p) + m, S)) * PAGE for p, m in zip(prompts, mx))
-        cache = model.new_cache(max_tokens=max_tokens or max(need, PAGE), max_seqs=max_batch or max(n, 1))
+            need = sum(w + (copies - 1) * m for w, m in zip(whole, more))
+        cache = model.new_cache(max_tokens=max_tokens or max(need, PAGE), max_seqs=max_batch or max(n * copies, 1))
     stops = tuple(model.spec.stop_ids) if stop_ids is None else tuple(stop_ids)
     return generate(ModelEngine(model, cache, params), prompts, mx, stop_ids=stops, callback=callback,
-                    max_batch=max_batch, loop_abort=loop_abort)
+                    max_batch=max_batch, loop_abort=loop_abort, completions=completions)

@@ -16,7 +16,7 @@ class Attention(Mixer):
     over the causal range (optionally the last ``window`` keys); output projection.
     Order and formulas: src/transformer/cpu.c:859-939, src/transformer/gqa_scalar.c:61-121."""
 
-    kernels = ("linear", "linear_mma", "linear_tc", "gemm_tc", "attention", "attention_decode", "attention_decode_tc", "attention_prefill",
+    kernels = ("linear", "linear_mma", "linear_tc", "gemm_tc", "attention", "attention_decode", "attention_decode_tc", "attention_shared", "attention_prefill",
                "attention_prefill_tc", "rope", "norm")
     graph_safe = True
     accepts_sink = True
@@ -57,10 +57,26 @@ class Attention(Mixer):
             return 0  # the one-launch decode kernel is not used
         return s.n_kv_heads * ((s.n_heads // s.n_kv_heads + 15) // 16)
 
+    def shared_heads(self):
+        """(query heads, key/value heads, head size) if this part can read pages that sequences share once for all of them."""
+        s = self.spec
+        fits = s.window == 0 and s.head_dim <= 128 and s.n_heads // s.n_kv_heads <= ops.SHARED_ROWS and s.softmax_scale > 0
+        return (s.n_heads, s.n_kv_heads, s.head_dim) if fits and self.decode_blocks_per_sequence() and s.q_dim % 8 == 0 and s.kv_dim % 8 == 0 else None
+
     def forward(self, h, ctx, kv, state, sink=None):
         s = self.spec
         n = h.shape[0]
         fusable = getattr(self.position, "rotary_params", None)
+        if kv.owner and ctx.shared is not None and self.shared_heads() == ctx.shared.heads:
+            # sequences forked from one prompt: the pages they share are read once for all of them
+            qkv = ops.linear(h, self.w_qkv, out_dtype=self.build.dtype)
+            self._tap_raw(ctx, qkv)
+            self.position.rotate(qkv, s.n_heads + s.n_kv_heads, s.head_dim, ctx)
+            out = torch.empty((n, s.q_dim), dtype=self.build.dtype, device=h.device)
+            ops.attention_decode_shared(qkv, s.q_dim, s.q_dim + s.kv_dim, out, n, s.n_heads, s.n_kv_heads, s.head_dim, s.softmax_scale, ctx.tok_pos,
+                                        ctx.slots, kv.page_table, kv.k, kv.v, ctx.shared)
+            ctx.tap("attn_out", out)
+            return ops.linear(out, self.w_o, out_dtype=self.build.dtype, sink=sink)
         if kv.owner and ctx.decode and self.build.dtype == torch.bfloat16 and fusable is not None:
             # one token per sequence: position encoding, cache write, attention over the splits of
             # the keys and their combination are one kernel

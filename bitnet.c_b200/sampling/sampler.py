@@ -21,7 +21,9 @@ from ..csrc import build, ops
 @dataclass(frozen=True)
 class SamplingParams:
     """temperature 0 is greedy (src/sampler.c:159-161); ``top_p`` outside (0, 1) turns the nucleus
-    off (src/sampler.c:169); ``repeat_penalty`` 1 is off.  Library defaults are those of
+    off (src/sampler.c:169); ``repeat_penalty`` 1 is off.  ``top_k`` keeps the k most probable tokens (0: all) and ``min_p`` those of at
+    least that share of the most probable one's probability (0: all): neither is in the reference; with either, top-k applies first, then the nucleus
+    of what it leaves, then min-p (``ops.sample_filtered``).  Library defaults are those of
     ``bn_sampler_init`` (src/sampler.c:17-30); the command line sets the reference's CLI defaults."""
 
     temperature: float = 0.0
@@ -29,6 +31,8 @@ class SamplingParams:
     seed: int = 42
     repeat_penalty: float = 1.0
     repeat_window: int = 64
+    top_k: int = 0
+    min_p: float = 0.0
 
     def validate(self) -> None:
         if self.temperature < 0:
@@ -37,6 +41,10 @@ class SamplingParams:
             raise ValueError(f"repeat_penalty={self.repeat_penalty} must be positive")
         if self.repeat_window <= 0:
             raise ValueError(f"repeat_window={self.repeat_window} must be positive")
+        if self.top_k < 0:
+            raise ValueError(f"top_k={self.top_k} must not be negative")
+        if not 0.0 <= self.min_p <= 1.0:
+            raise ValueError(f"min_p={self.min_p} must lie in [0, 1]")
 
     @property
     def greedy(self) -> bool:
@@ -45,6 +53,10 @@ class SamplingParams:
     @property
     def nucleus(self) -> bool:
         return 0.0 < self.top_p < 1.0
+
+    @property
+    def filtered(self) -> bool:
+        return not self.greedy and (self.top_k > 0 or self.min_p > 0.0)
 
 
 def seed_state(seed: int) -> int:
@@ -60,13 +72,14 @@ class Sampler:
                  prompts: Optional[Sequence[Sequence[int]]] = None):
         params.validate()
         if torch.device(device).type == "cuda":
-            build.ensure_built(["sampling"])  # compiled when a sampler is first made, not with the model
+            # compiled when a sampler is first made, not with the model
+            build.ensure_built(["sampling", "sampling_filtered"] if params.filtered else ["sampling"])
         self.params, self.n_rows, self.vocab, self.device = params, n_rows, vocab, device
         self.rng = torch.zeros(n_rows, dtype=torch.int64, device=device)
         self.penalised = params.repeat_penalty != 1.0
         # scratch of the nucleus kernel, allocated once: recorded graphs keep its address
         self.probs: Optional[torch.Tensor] = None
-        if not params.greedy and params.nucleus:
+        if not params.greedy and params.nucleus and not params.filtered:
             self.probs = torch.empty((n_rows, vocab), dtype=torch.float32, device=device)
         if self.penalised:
             w = params.repeat_window
@@ -106,6 +119,8 @@ class Sampler:
             ops.repeat_penalty(logits, self.recent, self.recent_len, p.repeat_penalty, index=index)
         if p.greedy:
             out = ops.argmax(logits)
+        elif p.filtered:
+            out = ops.sample_filtered(logits, p.temperature, p.top_k, p.top_p, p.min_p, rng_state=self.rng, index=index)
         elif p.nucleus:
             if self.probs is None or self.probs.shape[0] < logits.shape[0]:
                 raise ValueError(f"sampler holds {self.n_rows} rows, got logits of {logits.shape[0]}")

@@ -25,7 +25,9 @@ def pieces_of(plan):
     most = ops.SHARED_ROWS // (plan.n_heads // plan.n_kv_heads)
     for i in range(plan.n_items):
         first, count, page, n = items[4 * i:4 * i + 4]
-        assert 1 <= count <= most and n >= 1 and first + count <= plan.n_members
+        if not count:  # what a list of fixed size is padded with
+            continue
+        assert 1 <= count <= most and n >= 1 and first + count <= plan.n_parts
         for m in range(first, first + count):
             b, place = members[2 * m:2 * m + 2]
             assert place not in got[b]
@@ -45,6 +47,18 @@ def test_every_shared_page_is_read_once_for_every_sequence(heads, kv, seed):
         pages.append(p)
     pages = [p + [10 ** 6 + i] for i, p in enumerate(pages)]
     plan = ops.SharedPlan(pages, heads, kv, 64, "cpu", sms=148)
+    look_over(plan, pages)
+    # a list of fixed size for a recorded step
+    padded = ops.SharedPlan(pages, heads, kv, 64, "cpu", sms=148, room=(plan.n_items + 5, plan.n_parts + 9))
+    assert padded.fits and len(padded.host) == 4 * (plan.n_items + 5) + 4 * len(pages) + 2 * (plan.n_parts + 9)
+    assert padded.runs == plan.runs and [x for x in padded.host if x] == [x for x in plan.host if x]
+    tight = ops.SharedPlan(pages, heads, kv, 64, "cpu", sms=148, room=(max(1, plan.n_items // 2), max(1, plan.n_parts // 2)))
+    if tight.fits and plan.runs:
+        look_over(tight, pages)
+    assert not plan.runs or not ops.SharedPlan(pages, heads, kv, 64, "cpu", sms=148, room=(4096, 1)).fits
+
+
+def look_over(plan, pages):
     got, sequences = pieces_of(plan)
     for b in range(len(pages)):
         first_own, place, n, _ = sequences[b]

@@ -157,3 +157,55 @@ def test_the_loop_detector_is_the_references_and_is_off_unless_asked_for():
     assert got[0].tokens == [5, 6, 7, 8, 5, 6, 7] and got[0].finish_reason == "loop"
     assert got[1].tokens == scripts[1] and got[1].finish_reason == "length"
     assert sorted(e.free) == [0, 1, 2, 3] and not e.seq  # both slots came back
+
+
+class Forking(Scripted):
+    """The same with sequences that are forked."""
+
+    def prefill(self, seqs):
+        self.log.append([(s.slot, -len(s.tokens)) for s in seqs])
+        for s in seqs:
+            assert list(s.want) == []
+            self.seq[s.slot].extend(s.tokens)
+
+    def fork(self, slot, n):
+        new = [self.open() for _ in range(n)]
+        for s in new:
+            self.seq[s] = list(self.seq[slot])
+        return new
+
+
+def test_several_completions_run_their_prompt_once():
+    e = Forking(n_slots=8)
+    prompts = [[1, 2, 3], [4], [5, 6, 7, 8, 9]]
+    res = generate(e, prompts, [4, 2, 0], completions=3)
+    assert len(res) == 9
+    for i, r in enumerate(res):
+        p, n = prompts[i // 3], [4, 2, 0][i // 3]
+        assert (r.tokens, r.finish_reason) == (expected(p, n) if n else ([], "length"))
+    # all of the first prompt but its last token; a prompt of one token has nothing to run
+    assert e.log[0] == [(0, -2)] and e.log[1] == [(0, 1), (2, 1), (3, 1), (1, 1), (4, 1), (5, 1)]
+    assert not e.seq and len(e.free) == 8
+
+
+def test_completions_in_batches_that_cut_through_a_prompt():
+    for slots in (1, 2, 4, 7):
+        e = Forking(n_slots=slots)
+        prompts = [[1, 2, 3], [9, 4]]
+        res = generate(e, prompts, 3, completions=3)
+        for i, r in enumerate(res):
+            assert (r.tokens, r.finish_reason) == expected(prompts[i // 3], 3)
+        assert not e.seq
+    with pytest.raises(ValueError, match="completions"):
+        generate(Forking(), [[1]], 1, completions=0)
+
+
+def test_a_prompts_full_pages_count_once_in_a_batch():
+    # 130 tokens and 10 more: three pages, of which two are shared by all of a prompt's completions
+    prompts = [[1] * 130] * 4
+    assert plan_batch(prompts, [10] * 4, 0, 64 * 6, 8, 4096, 4) == 4
+    assert plan_batch(prompts, [10] * 4, 0, 64 * 5, 8, 4096, 4) == 3
+    assert plan_batch(prompts, [10] * 4, 1, 64 * 5, 8, 4096, 4) == 3  # the first of a batch holds all of it
+    assert plan_batch(prompts, [10] * 4, 0, 64 * 6, 8, 4096) == 2
+    assert plan_batch([[1] * 129] * 2, [10] * 2, 0, 64 * 4, 8, 4096, 2) == 2  # 128 tokens in front of the last one
+    assert plan_batch([[1] * 128] * 2, [10] * 2, 0, 64 * 4, 8, 4096, 2) == 1  # and 127: one full page
