@@ -1112,6 +1112,8 @@ class SharedPlan:
         self.device = torch.device(device)
         self.runs, self.first_own = shared_runs([p[:-1] for p in pages])  # the last page takes the new token: it is nobody else's
         self.own_pages = max((len(p) - f for p, f in zip(pages, self.first_own)), default=0)
+        self.deepest = max(self.first_own, default=0)
+        self._grid = None
         self.fits = self._lay_out(sms if sms is not None else n_sms(self.device), room)
         self.table = None
 
@@ -1124,6 +1126,13 @@ class SharedPlan:
         if to is not None:
             to[:host.numel()].copy_(host, non_blocking=True)
         return self
+
+    def own_grid(self):
+        """``decode_grid`` of the sequences' own pages, at most 8 blocks a sequence: those are one cluster and share no workspace with other launches."""
+        if self._grid is None or self._grid[0] != self.own_pages:
+            splits, each = decode_grid(self.own_pages * PAGE, self.n_seqs, self.n_heads, self.n_kv_heads)
+            self._grid = self.own_pages, ((splits, each) if splits <= 8 else (8, -(-self.own_pages // 8)))
+        return self._grid[1]
 
     def _lay_out(self, sms: int, room) -> bool:
         """The list of work, ``host``: items (first member, members, first page, pages), of every sequence (pages read together, first place of its
@@ -1216,18 +1225,19 @@ def attention_decode_shared(qkv: torch.Tensor, k_off: int, v_off: int, out: torc
     _need(page_table, "page_table", torch.int32, 2)
     _need(k_cache, "k_cache", torch.bfloat16, 4)
     _need(v_cache, "v_cache", torch.bfloat16, 4)
-    device = qkv.device
-    if any(t.device != device for t in (out, tok_pos, slots, page_table, k_cache, v_cache)):
+    device, at = qkv.device, qkv.get_device()
+    rows, row = qkv.shape
+    if not (out.get_device() == at == tok_pos.get_device() == slots.get_device() == page_table.get_device() == k_cache.get_device() == v_cache.get_device()):
         raise KernelError(f"attention_decode_shared: everything must lie on {device}")
-    if tuple(k_cache.shape[1:]) != (n_kv_heads, PAGE, head_dim) or k_cache.shape != v_cache.shape:
+    if k_cache.shape[1:] != (n_kv_heads, PAGE, head_dim) or k_cache.shape != v_cache.shape:
         raise KernelError(f"attention_decode_shared: cache {tuple(k_cache.shape)} is not [pages, {n_kv_heads}, {PAGE}, {head_dim}]")
-    if (plan.n_seqs, plan.n_heads, plan.n_kv_heads, plan.head_dim) != (n_seqs, n_heads, n_kv_heads, head_dim) or plan.table is None or plan.table.device != device:
+    if plan.n_seqs != n_seqs or plan.heads != (n_heads, n_kv_heads, head_dim) or plan.table is None or plan.table.get_device() != at:
         raise KernelError(f"attention_decode_shared: the plan is for {plan.n_seqs} sequences, heads {plan.n_heads}/{plan.n_kv_heads} of {plan.head_dim} on "
                           f"{plan.device}")
-    if min(k_off, v_off) < 0 or max(k_off, v_off) + n_kv_heads * head_dim > qkv.shape[1] or n_heads * head_dim > qkv.shape[1] or (k_off | v_off | qkv.shape[1]) % 8:
+    if min(k_off, v_off) < 0 or max(k_off, v_off) + n_kv_heads * head_dim > row or n_heads * head_dim > row or (k_off | v_off | row) % 8:
         raise KernelError("attention_decode_shared: offsets run past the row, or row and offsets are no multiples of 8")
-    if (out.shape[0] < n_seqs or out.shape[1] != n_heads * head_dim or tok_pos.shape[0] < n_seqs or slots.shape[0] < n_seqs or qkv.shape[0] < n_seqs
-            or max(plan.first_own, default=0) >= page_table.shape[1]):
+    if (out.shape[0] < n_seqs or out.shape[1] != n_heads * head_dim or tok_pos.shape[0] < n_seqs or slots.shape[0] < n_seqs or rows < n_seqs
+            or plan.deepest >= page_table.shape[1]):
         raise KernelError("attention_decode_shared: out, qkv, tok_pos, slots or page_table does not fit")
     if not scale > 0:
         raise KernelError(f"attention_decode_shared: scale={scale} must be positive")
@@ -1235,22 +1245,24 @@ def attention_decode_shared(qkv: torch.Tensor, k_off: int, v_off: int, out: torc
         if not plan.n_items:
             return attention_decode_fused(qkv, k_off, v_off, out, n_seqs, n_heads, n_kv_heads, head_dim, scale, 0, 0, 1.0, tok_pos, slots, page_table,
                                           k_cache, v_cache, plan.own_pages * PAGE)
-        n_splits, pages_per_block = decode_grid(plan.own_pages * PAGE, n_seqs, n_heads, n_kv_heads)
-        _scr, counters = _split_scratch(device)
-        floats = lambda n: torch.empty(n, dtype=torch.float32, device=device)  # noqa: E731
-        shared_o, shared_ml = floats(plan.n_parts * n_heads * head_dim), floats(plan.n_parts * n_heads * 2)
-        part_o, part_ml = floats(n_seqs * n_heads * n_splits * head_dim), floats(n_seqs * n_heads * n_splits * 2)
-        items, members, sequences = (c_void_p(plan.table.data_ptr() + 4 * i) for i in plan.at)
-        status = _ptr(tc_status(device))
+        n_splits, pages_per_block = plan.own_grid()
+        counters = _split_scratch(device)[1]
+        # results of the shared pages, values and then (maximum, sum); a sequence's own splits are one cluster and need no room (nor tickets)
+        results = plan.n_parts * n_heads
+        room = torch.empty(results * (head_dim + 2), dtype=torch.float32, device=device)
+        shared_o, shared_ml = c_void_p(room.data_ptr()), c_void_p(room.data_ptr() + 4 * results * head_dim)
+        table = plan.table.data_ptr()
+        items, members, sequences = (c_void_p(table + 4 * i) for i in plan.at)
+        status, stream, f_scale = _tc_status_arg(device), _stream(), c_float(scale)
+        p_qkv, p_pos, p_slots, p_table, p_k, p_v = _ptr(qkv), _ptr(tok_pos), _ptr(slots), _ptr(page_table), _ptr(k_cache), _ptr(v_cache)
+        pages, width = k_cache.shape[0], page_table.shape[1]
         _check(_fn("attention_shared", "bn_attention_shared")(
-            _ptr(qkv), int(qkv.shape[1]), int(n_seqs), int(n_heads), int(n_kv_heads), int(head_dim), c_float(scale), items, plan.n_items, members,
-            plan.n_parts, _ptr(slots), _ptr(page_table), int(page_table.shape[1]), _ptr(k_cache), _ptr(v_cache), int(k_cache.shape[0]), _ptr(shared_o),
-            _ptr(shared_ml), plan.n_parts, status, _stream()), "attention_decode_shared")
+            p_qkv, row, n_seqs, n_heads, n_kv_heads, head_dim, f_scale, items, plan.n_items, members, plan.n_parts, p_slots, p_table, width, p_k, p_v, pages,
+            shared_o, shared_ml, plan.n_parts, status, stream), "attention_decode_shared")
         _check(_fn("attention_decode_tc", "bn_attention_decode_tc_join")(
-            _ptr(qkv), int(qkv.shape[1]), int(k_off), int(v_off), _ptr(out), int(out.shape[1]), int(n_seqs), int(n_heads), int(n_kv_heads), int(head_dim),
-            c_float(scale), _ptr(tok_pos), _ptr(slots), _ptr(page_table), int(page_table.shape[1]), _ptr(k_cache), _ptr(v_cache),
-            int(k_cache.shape[0]), status, _ptr(part_o), _ptr(part_ml), int(n_splits), int(pages_per_block), _ptr(counters), int(counters.numel()),
-            sequences, _ptr(shared_o), _ptr(shared_ml), plan.n_parts, _stream()), "attention_decode_shared")
+            p_qkv, row, k_off, v_off, _ptr(out), out.shape[1], n_seqs, n_heads, n_kv_heads, head_dim, f_scale, p_pos, p_slots, p_table, width, p_k, p_v, pages,
+            status, shared_o, shared_ml, n_splits, pages_per_block, _ptr(counters), counters.numel(), sequences, shared_o, shared_ml, plan.n_parts, stream),
+            "attention_decode_shared")
     return out
 
 

@@ -6,16 +6,21 @@
 // is sorted: every border is "the first whose running sum (of ones, or of weights) exceeds a number", found by the bits of the logits.
 //
 // A cluster of blocks holds a row in its shared memory as ordered 32-bit keys, so that memory is read once however many passes
-// follow.  A pass over a level of 11, 11 or 10 bits adds the ones or weights of the keys that agree with the bits found
-// so far into a histogram per block; the blocks then add up a share of the bins each, over the cluster, and the one
-// whose bins hold the border tells the others.
-// Weights are numbers of 64 bits in fixed point: sums do not depend on the order of additions, and a running sum that lies next to a
-// border falls on the same side as in a sum of doubles (rounding to 2^-45 a token at a vocabulary of 2^17; a float sum would move a token in
-// a thousand).
+// follow.  One pass counts the keys by their weight in steps of 2^(1/64): from the counts the first block knows lower and upper bounds of
+// every running sum, and so the few steps among which each border lies.  A second pass hands the keys of those steps to the first block and adds
+// up the weights of the keys above each; the first block sorts what it got (some tens of keys, of a flat row some hundreds) and decides.  Where
+// too many keys lie together (ties by the thousand, a huge temperature), borders are found by the bits of the keys instead, 11, 11 and 10 at a time, the
+// weights of the keys that agree with the bits found so far added into a histogram.
+// Weights are whole numbers of 64 bits: sums do not depend on the order of additions, and a running sum that lies next to a border falls on the
+// same side as in a sum of doubles (a float sum would move a token in a thousand).  2^-y is taken apart into 2^-(j/64) from a table, a shift, and
+// 1 - e of a remainder below 1/64, whose e is small enough for a float: y = (max - l) / T * log2(e) is carried in two floats.
 #include "common.cuh"
 
 #define SF_THREADS 512
-#define SF_BINS 2048
+#define SF_BINS 2048     // of a histogram of bits
+#define SF_STEPS 4096    // of the counts by weight: 64 octaves of 64 steps
+#define SF_LIST 4096     // keys that the first block may be handed
+#define SF_POINT 56      // a weight of 1 is 2^56 while a thread adds up its own (at most 2^7 of them)
 #define SF_MAX_CLUSTER 8
 
 struct SfArgs {
@@ -71,12 +76,42 @@ __device__ __forceinline__ void sf_store(unsigned long long* p, unsigned rank, u
   asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(sf_remote(p, rank)), "l"(v) : "memory");
 }
 
+struct SfRange {  // steps first .. last
+  int first, last;
+};
+struct alignas(8) SfPlan {
+  SfRange range[4];    // where the borders of top-k, top-p, min-p and the draw lie; none: last < first
+  unsigned least;      // min-p: the smallest key that stays
+  unsigned rest;       // top-k: so many keys of its step stay
+  int by_bits;         // borders are found by the bits of the keys
+  int pad;
+};
+#define SF_TOP_K 0
+#define SF_TOP_P 1
+#define SF_MIN_P 2
+#define SF_DRAW 3
+
 struct SfShared {
-  unsigned long long hist[SF_BINS];
+  union {
+    unsigned long long hist[SF_BINS];
+    unsigned count[SF_STEPS];
+    unsigned long long list[SF_LIST];  // keys falling, equal ones by index: (~key, index)
+  };
   unsigned long long warp[SF_THREADS / 32];
   // one entry per block of the cluster, written by that block; two sets in turn, so that one barrier per exchange is enough
   unsigned long long part[2][SF_MAX_CLUSTER];
   unsigned long long found[2];  // what the block that found a border tells the others
+  unsigned long long mass[SF_MAX_CLUSTER];      // first block: the weights of each block's keys
+  unsigned long long over[SF_MAX_CLUSTER][4];   // first block: of those above each range
+  SfPlan plan;
+  unsigned listed;                              // first block: keys in the list
+  unsigned long long table[64];                 // 2^-(j/64), 1 = 2^SF_POINT
+  int small_table[64];                          // the same, 1 = 2^30
+  float warp_lower[SF_THREADS / 32], warp_upper[SF_THREADS / 32];
+  float got[8];
+  int steps[8];
+  unsigned long long base[4], sum[2];
+  int at[4];
 };
 
 template <typename T, bool RESIDENT>
@@ -90,6 +125,7 @@ struct SfRow {
   int turn = 0;
   double top, per_t;     // the largest logit, 1 / temperature
   bool infinite;         // the largest logit is +inf: those share everything
+  float topf, c_hi, c_lo;  // the largest logit, log2(e) / temperature in two floats
 
   __device__ __forceinline__ unsigned key(int i) const { return RESIDENT ? keys[i] : sf_key(to_f32<T>(row[i])); }
   __device__ __forceinline__ double weight(unsigned k) const {
@@ -205,6 +241,355 @@ struct SfRow {
     return prefix;
   }
 
+  // ---- by steps of weight ----
+  // The step of a key (falling keys, rising steps) and what is behind it: y = step / 64 + rest.
+  __device__ __forceinline__ int step_of(unsigned k, float* rest) const {
+    const float v = sf_value(k), d = topf - v, bb = d - topf, dl = (topf - (d - bb)) - (v + bb);
+    const float y = d * c_hi, yl = fmaf(d, c_hi, -y) + fmaf(d, c_lo, dl * c_hi);
+    const int n = min(__float2int_rd(y * 64.f), SF_STEPS - 1);
+    *rest = fmaf((float)n, -1.f / 64.f, y) + yl;
+    return n;
+  }
+  __device__ __forceinline__ int step_of(unsigned k) const { return min(__float2int_rd((topf - sf_value(k)) * c_hi * 64.f), SF_STEPS - 1); }
+  // 2^-y, 1 = 2^SF_POINT, to 2^-31 of itself
+  __device__ __forceinline__ unsigned long long weight_at(int n, float rest) const {
+    const float g = rest * 0.69314718f, e = g * (1.f - g * (0.5f - g * (0.16666667f - g * 0.041666668f)));  // 1 - exp(-g)
+    const int whole = __float2int_rn(e * 4294967296.f);
+    const unsigned long long w = s.table[n & 63] - (((long long)s.small_table[n & 63] * whole) >> (62 - SF_POINT));
+    return n == SF_STEPS - 1 ? 0ull : w >> (n >> 6);
+  }
+  __device__ __forceinline__ unsigned long long to_scale(unsigned long long w) const {  // from 2^SF_POINT to 2^scale_bits
+    const int down = SF_POINT - a.scale_bits;
+    return down ? (w + (1ull << (down - 1))) >> down : w;
+  }
+  // A thread adds up its weights with SF_POINT bits behind the point while it has few of them (a row that is held), else with as many as the sums have.
+  __device__ __forceinline__ void add(unsigned long long& sum, unsigned long long w) const { sum += RESIDENT ? w : to_scale(w); }
+  __device__ __forceinline__ unsigned long long added(unsigned long long sum) const { return RESIDENT ? to_scale(sum) : sum; }
+  // f(key, index) for the keys above -inf of this block
+  template <class F>
+  __device__ __forceinline__ void each_key(F f) const {
+    if (RESIDENT) {  // (the keys behind the last are 0)
+      for (int i = threadIdx.x * 4; i < n; i += SF_THREADS * 4) {
+        const uint4 k = *reinterpret_cast<const uint4*>(keys + i);
+        if (k.x) f(k.x, i);
+        if (k.y) f(k.y, i + 1);
+        if (k.z) f(k.z, i + 2);
+        if (k.w) f(k.w, i + 3);
+      }
+    } else {
+      for (int i = threadIdx.x; i < n; i += SF_THREADS) {
+        const unsigned k = key(i);
+        if (k) f(k, i);
+      }
+    }
+  }
+  // Of the steps' weights, bounds that hold for every key of a step whatever its float rounding.
+  static __device__ __forceinline__ float upper(int n) { return n == 0 ? 1.0001f : exp2f(-(n - 0.02f) / 64.f); }
+  static __device__ __forceinline__ float lower(int n) { return n == SF_STEPS - 1 ? 0.f : exp2f(-(n + 1.02f) / 64.f); }
+
+  // First block: where the borders lie, from the counts of all blocks.  k, p, m: which filters there are.
+  __device__ void make_plan(bool k_on, unsigned top_k, bool p_on, float top_p, bool m_on, float min_p, float temperature, float u, unsigned long long all_mass) {
+    constexpr int EACH = SF_STEPS / SF_THREADS, NW = SF_THREADS / 32;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n0 = tid * EACH;
+    unsigned c[EACH];
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) c[e] = 0;
+    for (unsigned r = 0; r < blocks; ++r) {
+#pragma unroll
+      for (int e = 0; e < EACH; e += 4) {
+        uint4 v;
+        asm volatile("ld.shared::cluster.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(sf_remote(&s.count[n0 + e], r)) : "memory");
+        c[e] += v.x; c[e + 1] += v.y; c[e + 2] += v.z; c[e + 3] += v.w;
+      }
+    }
+    // in front of this thread's steps: keys, and bounds of their weights
+    unsigned before = 0;
+    float low = 0.f, up = 0.f;
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+      before += c[e];
+      low += c[e] * lower(n0 + e);
+      up += c[e] * upper(n0 + e);
+    }
+    unsigned cs = before;
+    float ls = low, us = up;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const unsigned x = __shfl_up_sync(0xffffffffu, cs, o);
+      const float y = __shfl_up_sync(0xffffffffu, ls, o), z = __shfl_up_sync(0xffffffffu, us, o);
+      if (lane >= o) { cs += x; ls += y; us += z; }
+    }
+    if (lane == 31) { s.warp[warp] = cs; s.warp_lower[warp] = ls; s.warp_upper[warp] = us; }
+    if (tid < 8) s.steps[tid] = -1;
+    if (tid == 0 && m_on) {
+      // the smallest key whose weight is at least min_p: near max + T log(min_p), found by trying its neighbours
+      unsigned k = sf_key((float)(top + (double)temperature * log((double)min_p)));
+      k = min(max(k, 1u), sf_key(topf));
+      for (int i = 0; i < 8 && k > 1u && weight(k - 1) >= (double)min_p; ++i) --k;
+      for (int i = 0; i < 8 && k < sf_key(topf) && !(weight(k) >= (double)min_p); ++i) ++k;
+      s.plan.least = k;
+    }
+    __syncthreads();
+    cs -= before; ls -= low; us -= up;
+    unsigned total = 0;
+    for (int w = 0; w < NW; ++w) {
+      if (w < warp) { cs += (unsigned)s.warp[w]; ls += s.warp_lower[w]; us += s.warp_upper[w]; }
+      total += (unsigned)s.warp[w];
+    }
+    // the first step whose running sum exceeds thr by the upper or lower bound goes to steps[slot] (-1: none does)
+    auto find = [&](int slot, float thr, bool by_upper) {
+      float run = by_upper ? us : ls;
+      unsigned mine = ~0u;
+#pragma unroll
+      for (int e = 0; e < EACH; ++e) {
+        run += c[e] * (by_upper ? upper(n0 + e) : lower(n0 + e));
+        if (mine == ~0u && c[e] && run > thr) mine = (unsigned)(n0 + e);
+      }
+      mine = __reduce_min_sync(0xffffffffu, mine);
+      if (lane == 0 && mine != ~0u) atomicMin((unsigned*)&s.steps[slot], mine);
+    };
+    const unsigned kth = min(top_k, total);
+    {
+      unsigned run = cs;
+      float l = ls, h = us;
+#pragma unroll
+      for (int e = 0; e < EACH; ++e) {
+        if (c[e] && run + c[e] == total) s.steps[7] = n0 + e;
+        if (k_on && run < kth && run + c[e] >= kth) {
+          s.steps[0] = n0 + e;
+          s.plan.rest = kth - run;
+          s.got[0] = l + (kth - run) * lower(n0 + e);
+          s.got[1] = h + (kth - run) * upper(n0 + e);
+        }
+        if (m_on && step_of(s.plan.least) == n0 + e) {
+          s.got[2] = l;
+          s.got[3] = h + c[e] * upper(n0 + e);
+        }
+        run += c[e];
+        l += c[e] * lower(n0 + e);
+        h += c[e] * upper(n0 + e);
+      }
+    }
+    __syncthreads();
+    const float slack = 1e-4f;  // far more than the float sums of bounds are off
+    const int last = s.steps[7], k_step = k_on ? s.steps[0] : last, m_step = m_on ? step_of(s.plan.least) : SF_STEPS;
+    const float exact = (float)ldexp((double)all_mass, -a.scale_bits);
+    const float all_low = k_on ? s.got[0] : exact, all_up = k_on ? s.got[1] : exact;  // (without a use for it, exact is 0 and not looked at)
+    if (p_on) {
+      find(1, top_p * all_low * (1.f - slack), true);
+      find(2, top_p * all_up * (1.f + slack), false);
+    }
+    __syncthreads();
+    SfRange range[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) range[r] = SfRange{1, 0};
+    int cut = last;
+    float kept_low = all_low, kept_up = all_up;
+    if (k_on) { range[SF_TOP_K] = SfRange{k_step, k_step}; cut = k_step; }
+    if (p_on) {
+      const int p1 = s.steps[2] < 0 ? cut : min(cut, s.steps[2]), p0 = s.steps[1] < 0 ? p1 : min(p1, s.steps[1]);
+      range[SF_TOP_P] = SfRange{p0, p1};
+      cut = p1;
+      kept_low = top_p * all_low;
+      kept_up = top_p * all_up + upper(p0);
+    }
+    if (m_on && m_step <= cut) {
+      if (!(k_on || p_on) || m_step < (p_on ? range[SF_TOP_P].first : k_step)) {  // what lies behind does not matter
+        range[SF_TOP_K] = range[SF_TOP_P] = SfRange{1, 0};
+        kept_low = s.got[2];
+        kept_up = s.got[3];
+      } else {
+        kept_low = fminf(kept_low, s.got[2]);
+        kept_up = fminf(kept_up, s.got[3]);
+      }
+      range[SF_MIN_P] = SfRange{m_step, m_step};
+      cut = min(cut, m_step);
+    } else if (m_on && !(k_on || p_on)) {  // everything stays
+      range[SF_MIN_P] = SfRange{last, last};
+      kept_low = s.got[2];
+      kept_up = s.got[3];
+    }
+    find(3, u * kept_low * (1.f - slack), true);
+    find(4, u * kept_up * (1.f + slack), false);
+    __syncthreads();
+    const int d1 = s.steps[4] < 0 ? cut : min(cut, s.steps[4]), d0 = s.steps[3] < 0 ? d1 : min(d1, s.steps[3]);
+    range[SF_DRAW] = SfRange{d0, d1};
+    unsigned wanted = 0;
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+      bool in = false;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) in |= n0 + e >= range[r].first && n0 + e <= range[r].last;
+      wanted += in ? c[e] : 0u;
+    }
+    wanted = (unsigned)block_sum64(wanted);
+    if (tid == 0) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) s.plan.range[r] = range[r];
+      s.plan.by_bits = wanted > SF_LIST;
+      s.listed = 0;
+    }
+  }
+
+  // All blocks: the keys of the ranges to the first block, and the weights above each range.
+  __device__ void hand_over(const SfPlan& plan) {
+    unsigned long long over[4] = {0, 0, 0, 0};
+    int first[4], end = 0;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      first[r] = plan.range[r].last < plan.range[r].first ? 0 : plan.range[r].first;
+      end = max(end, plan.range[r].last);
+    }
+    const int offset = (int)rank * a.per;
+    each_key([&](unsigned k, int i) {
+      float rest;
+      const int n = step_of(k, &rest);
+      if (n > end) return;
+      const unsigned long long w = weight_at(n, rest);
+      bool in = false;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        if (n < first[r]) add(over[r], w);
+        in |= n >= plan.range[r].first && n <= plan.range[r].last;
+      }
+      if (in) {
+        unsigned at;
+        asm volatile("atom.relaxed.cluster.shared::cluster.add.u32 %0, [%1], 1;" : "=r"(at) : "r"(sf_remote(&s.listed, 0)) : "memory");
+        if (at < SF_LIST) sf_store(&s.list[at], 0, ((unsigned long long)~k << 32) | (unsigned)(offset + i));
+      }
+    });
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const unsigned long long sum = block_sum64(added(over[r]));
+      if (threadIdx.x == 0) sf_store(&s.over[rank][r], 0, sum);
+    }
+  }
+
+  // First block: sort what was handed over and walk the borders; the token.
+  __device__ void decide(bool k_on, bool p_on, float top_p, bool m_on, float u, unsigned long long all_mass, int* out) {
+    const int m = min((int)s.listed, SF_LIST), tid = threadIdx.x;
+    int size = 2;
+    while (size < m) size *= 2;
+    for (int i = m + tid; i < size; i += SF_THREADS) s.list[i] = ~0ull;
+    __syncthreads();
+    for (int k = 2; k <= size; k *= 2) {
+      for (int j = k / 2; j > 0; j /= 2) {
+        for (int i = tid; i < size / 2; i += SF_THREADS) {
+          const int x = 2 * i - (i & (j - 1)), y = x + j;
+          const unsigned long long p = s.list[x], q = s.list[y];
+          if ((p > q) == ((x & k) == 0)) { s.list[x] = q; s.list[y] = p; }
+        }
+        __syncthreads();
+      }
+    }
+    // running sums: thread t has entries t * each and on
+    constexpr int MOST = SF_LIST / SF_THREADS;
+    const int each = (m + SF_THREADS - 1) / SF_THREADS, i0 = tid * each;
+    unsigned long long w[MOST], sum = 0;
+    int step[MOST];
+#pragma unroll
+    for (int e = 0; e < MOST; ++e) {
+      w[e] = 0;
+      step[e] = SF_STEPS;
+      if (e < each && i0 + e < m) {
+        float rest;
+        step[e] = step_of(~(unsigned)(s.list[i0 + e] >> 32), &rest);
+        w[e] = to_scale(weight_at(step[e], rest));
+      }
+      sum += w[e];
+    }
+    const int lane = tid & 31, warp = tid >> 5;
+    unsigned long long run0 = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const unsigned long long t = __shfl_up_sync(0xffffffffu, run0, o);
+      if (lane >= o) run0 += t;
+    }
+    if (lane == 31) s.warp[warp] = run0;
+    __syncthreads();
+    run0 -= sum;
+    unsigned long long total = 0;
+    for (int x = 0; x < SF_THREADS / 32; ++x) {
+      if (x < warp) run0 += s.warp[x];
+      total += s.warp[x];
+    }
+    unsigned long long over[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      over[r] = 0;
+      for (unsigned b = 0; b < blocks; ++b) over[r] += s.over[b][r];
+    }
+    if (tid < 4) { s.base[tid] = total; s.at[tid] = m; }
+    __syncthreads();
+    // where each range begins, and the running sum in front of it
+    {
+      unsigned long long run = run0;
+      int prev = i0 > 0 && i0 <= m ? step_of(~(unsigned)(s.list[i0 - 1] >> 32)) : -1;
+#pragma unroll
+      for (int e = 0; e < MOST; ++e) {
+        if (e < each && i0 + e < m) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (step[e] >= s.plan.range[r].first && prev < s.plan.range[r].first) { s.base[r] = run; s.at[r] = i0 + e; }
+          prev = step[e];
+        }
+        run += w[e];
+      }
+    }
+    __syncthreads();
+    const bool k_in = k_on && s.plan.range[SF_TOP_K].last >= s.plan.range[SF_TOP_K].first;
+    const bool p_in = p_on && s.plan.range[SF_TOP_P].last >= s.plan.range[SF_TOP_P].first;
+    const bool m_in = m_on && s.plan.range[SF_MIN_P].last >= s.plan.range[SF_MIN_P].first;
+    // f(entry, running sum in front of it, with it)
+    auto walk = [&](auto f) {
+      unsigned long long run = run0;
+#pragma unroll
+      for (int e = 0; e < MOST; ++e) {
+        if (e < each && i0 + e < m) f(i0 + e, run, run + w[e]);
+        run += w[e];
+      }
+    };
+    if (tid == 0) { s.sum[0] = all_mass; s.sum[1] = ~0ull; }
+    __syncthreads();
+    if (k_in) {
+      const int at = s.at[SF_TOP_K] + (int)s.plan.rest - 1;
+      walk([&](int i, unsigned long long, unsigned long long run) {
+        if (i == at) s.sum[0] = over[SF_TOP_K] + run - s.base[SF_TOP_K];
+      });
+    }
+    if (m_in) {
+      // the last entry that stays; without one nothing of the range does
+      if (tid == 0) s.sum[1] = over[SF_MIN_P];
+      __syncthreads();
+      const int at0 = s.at[SF_MIN_P];
+      walk([&](int i, unsigned long long, unsigned long long run) {
+        if (i >= at0 && ~(unsigned)(s.list[i] >> 32) >= s.plan.least && (i + 1 >= m || ~(unsigned)(s.list[i + 1] >> 32) < s.plan.least))
+          s.sum[1] = over[SF_MIN_P] + run - s.base[SF_MIN_P];
+      });
+    }
+    __syncthreads();
+    const unsigned long long by_k = s.sum[0], by_m = s.sum[1];
+    __syncthreads();
+    if (p_in) {
+      const unsigned long long thr = min((unsigned long long)((double)top_p * (double)by_k), by_k - 1);
+      const int at0 = s.at[SF_TOP_P];
+      walk([&](int i, unsigned long long before, unsigned long long run) {
+        const unsigned long long off = over[SF_TOP_P] - s.base[SF_TOP_P];
+        if (i >= at0 && before + off <= thr && run + off > thr) s.sum[0] = run + off;
+      });
+    }
+    __syncthreads();
+    const unsigned long long kept = min((k_in || p_in || !m_in) ? s.sum[0] : ~0ull, by_m);
+    const unsigned long long thr = min((unsigned long long)((double)u * (double)kept), kept - 1);
+    const int at0 = s.at[SF_DRAW];
+    if (tid == 0) *out = (int)(unsigned)s.list[min(at0, m - 1)];
+    __syncthreads();
+    walk([&](int i, unsigned long long before, unsigned long long run) {
+      const unsigned long long off = over[SF_DRAW] - s.base[SF_DRAW];
+      if (i >= at0 && before + off <= thr && run + off > thr) *out = (int)(unsigned)s.list[i];
+    });
+  }
+
   // The index of the j-th (from 0) of the row's numbers with key k, in the block that has it; -1 elsewhere.
   __device__ int nth(unsigned k, unsigned long long j) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = SF_THREADS / 32;
@@ -234,29 +619,62 @@ struct SfRow {
   }
 };
 
+// Keys of one block's part of a row into shared memory (RESIDENT); the largest.
 template <typename T, bool RESIDENT>
-__global__ void __launch_bounds__(SF_THREADS) sample_filtered_kernel(SfArgs a) {
+__device__ __forceinline__ unsigned sf_read(const T* row, int n, int per, unsigned* keys) {
+  unsigned high = 0;
+  constexpr int V = 16 / (int)sizeof(T);
+  int done = 0;
+  if ((((uintptr_t)row) & 15) == 0) {
+    const int nv = n / V;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < nv; i += SF_THREADS) {
+      const uint4 raw = reinterpret_cast<const uint4*>(row)[i];
+      const T* x = reinterpret_cast<const T*>(&raw);
+      unsigned k[V];
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        k[e] = sf_key(to_f32<T>(x[e]));
+        high = max(high, k[e]);
+      }
+      if (RESIDENT) {
+#pragma unroll
+        for (int e = 0; e < V; e += 4) *reinterpret_cast<uint4*>(keys + i * V + e) = make_uint4(k[e], k[e + 1], k[e + 2], k[e + 3]);
+      }
+    }
+    done = nv * V;
+  }
+#pragma unroll 4
+  for (int i = done + threadIdx.x; i < (RESIDENT ? per : n); i += SF_THREADS) {
+    const unsigned k = i < n ? sf_key(to_f32<T>(row[i])) : 0u;
+    high = max(high, k);
+    if (RESIDENT) keys[i] = k;
+  }
+  return high;
+}
+
+template <typename T, bool RESIDENT>
+__global__ void __launch_bounds__(SF_THREADS, 2) sample_filtered_kernel(const __grid_constant__ SfArgs a) {
   pdl_launch_dependents();
   extern __shared__ __align__(16) unsigned char smem_raw[];
   SfShared& s = *reinterpret_cast<SfShared*>(smem_raw);
-  unsigned* keys = reinterpret_cast<unsigned*>(smem_raw + sizeof(SfShared));
+  unsigned* keys = reinterpret_cast<unsigned*>(smem_raw + ((sizeof(SfShared) + 15) & ~(size_t)15));
   const unsigned rank = sf_rank(), blocks = sf_size();
   const int r = blockIdx.x / blocks;
   const int first = min(a.vocab, (int)rank * a.per);
   SfRow<T, RESIDENT> row{a, s, keys, (const T*)a.logits + (size_t)r * a.ld + first, min(a.vocab, first + a.per) - first, rank, blocks};
+  for (int b = threadIdx.x; b < SF_STEPS; b += SF_THREADS) s.count[b] = 0;
+  if (threadIdx.x < 64) {
+    const double x = exp2(-(double)threadIdx.x / 64.0);
+    s.table[threadIdx.x] = (unsigned long long)__double2ll_rn(ldexp(x, SF_POINT));
+    s.small_table[threadIdx.x] = __double2int_rn(ldexp(x, 30));
+  }
   pdl_wait();
   const float temperature = a.temperatures ? a.temperatures[r] : a.temperature;
   const float top_p = a.top_ps ? a.top_ps[r] : a.top_p, asked = a.min_ps ? a.min_ps[r] : a.min_p;
   const float min_p = asked > 0.f ? fminf(asked, 1.f) : 0.f;  // the most probable token always stays
   const int top_k = a.top_ks ? a.top_ks[r] : a.top_k;
-  unsigned high = 0;
-  unsigned long long valid = 0;
-  for (int i = threadIdx.x; i < row.n; i += SF_THREADS) {
-    const unsigned k = sf_key(to_f32<T>(row.row[i]));
-    if (RESIDENT) keys[i] = k;
-    high = max(high, k);
-    valid += k != 0u;
-  }
+  unsigned high = sf_read<T, RESIDENT>(row.row, row.n, a.per, keys);
   sf_sync();  // every block of the cluster runs: its shared memory may be written
   // the random number, drawn once for the whole cluster
   if (rank == 0 && threadIdx.x == 0) {
@@ -278,15 +696,61 @@ __global__ void __launch_bounds__(SF_THREADS) sample_filtered_kernel(SfArgs a) {
   __syncthreads();
   for (int w = 0; w < SF_THREADS / 32; ++w) high = max(high, (unsigned)s.warp[w]);
   high = row.exchange_max(high);
-  const float u = __uint_as_float((unsigned)s.found[0]);
+  const float asked_u = __uint_as_float((unsigned)s.found[0]), u = asked_u > 0.f ? asked_u : 0.f;
   unsigned chosen = high;
   unsigned long long tie = 0;
   if (high != 0u && temperature > 0.f) {
-    unsigned long long before;
-    valid = row.exchange_sum(row.block_sum64(valid), &before);
-    row.top = (double)sf_value(high);
-    row.infinite = row.top == INFINITY;
+    row.topf = sf_value(high);
+    row.top = (double)row.topf;
+    row.infinite = row.topf == INFINITY;
     row.per_t = 1.0 / (double)temperature;
+    const double c = 1.4426950408889634 * row.per_t;
+    row.c_hi = (float)c;
+    row.c_lo = (float)(c - (double)row.c_hi);
+    const bool k_on = top_k > 0 && top_k < a.vocab, p_on = top_p > 0.f && top_p < 1.f, m_on = min_p > 0.f;
+    bool by_bits = row.infinite || !(c > 1e-30 && c < 1e30);  // (a temperature near the ends of float's range)
+    if (!by_bits) {
+      // counts by weight; the sum of all weights where a border asks for it
+      const bool need = !k_on && (p_on || !m_on);
+      unsigned long long mine = 0;
+      if (need) {
+        row.each_key([&](unsigned k, int) {
+          float rest;
+          const int n = row.step_of(k, &rest);
+          atomicAdd(&s.count[n], 1u);
+          row.add(mine, row.weight_at(n, rest));
+        });
+      } else {
+        row.each_key([&](unsigned k, int) { atomicAdd(&s.count[row.step_of(k)], 1u); });
+      }
+      const unsigned long long sum = row.block_sum64(row.added(mine));
+      if (threadIdx.x == 0) sf_store(&s.mass[rank], 0, sum);
+      sf_sync();
+      unsigned long long all_mass = 0;
+      if (rank == 0) {
+        for (unsigned b = 0; b < blocks; ++b) all_mass += s.mass[b];
+        row.make_plan(k_on, (unsigned)top_k, p_on, top_p, m_on, min_p, temperature, u, all_mass);
+      }
+      sf_sync();
+      SfPlan plan;
+      {
+        constexpr int WORDS = sizeof(SfPlan) / 8;
+        unsigned long long* to = reinterpret_cast<unsigned long long*>(&plan);
+#pragma unroll
+        for (int i = 0; i < WORDS; ++i) to[i] = sf_load(reinterpret_cast<const unsigned long long*>(&s.plan) + i, 0);
+      }
+      by_bits = plan.by_bits;
+      if (!by_bits) {
+        row.hand_over(plan);
+        sf_sync();  // the last time that another block is needed
+        if (rank == 0) row.decide(k_on, p_on, top_p, m_on, u, all_mass, a.out + r);
+        return;
+      }
+      sf_sync();  // the plan has been read: shared memory is used anew
+    }
+    unsigned long long valid = 0, before;
+    row.each_key([&](unsigned, int) { ++valid; });
+    valid = row.exchange_sum(row.block_sum64(valid), &before);
     // kept: all larger than `cut`, and `ties` of those equal to it
     unsigned cut = 1u;
     unsigned long long ties = 0;
@@ -297,13 +761,12 @@ __global__ void __launch_bounds__(SF_THREADS) sample_filtered_kernel(SfArgs a) {
     }
     auto kept_mass = [&](float least) {
       unsigned long long m = 0;
-      for (int i = threadIdx.x; i < row.n; i += SF_THREADS) {
-        const unsigned k = row.key(i);
+      row.each_key([&](unsigned k, int) {
         if (k > cut) {
           const double w = row.weight(k);
           if (w >= (double)least) m += row.fixed(w);
         }
-      }
+      });
       m = row.block_sum64(m);
       unsigned long long low, all = row.exchange_sum(m, &low);
       if (ties) {
@@ -312,7 +775,7 @@ __global__ void __launch_bounds__(SF_THREADS) sample_filtered_kernel(SfArgs a) {
       }
       return all;
     };
-    if (top_p > 0.f && top_p < 1.f) {
+    if (p_on) {
       const unsigned long long all = kept_mass(0.f);
       const unsigned long long thr = min((unsigned long long)((double)top_p * (double)all), all - 1);
       unsigned long long above;
@@ -322,8 +785,7 @@ __global__ void __launch_bounds__(SF_THREADS) sample_filtered_kernel(SfArgs a) {
       cut = k;
     }
     const unsigned long long all = kept_mass(min_p);
-    const float share = u > 0.f ? u : 0.f;
-    const unsigned long long thr = min((unsigned long long)((double)share * (double)all), all - 1);
+    const unsigned long long thr = min((unsigned long long)((double)u * (double)all), all - 1);
     unsigned long long above;
     chosen = row.template first_exceeding<false>(thr, &above);
     tie = (thr - above) / row.fixed(row.weight(chosen));
@@ -347,7 +809,7 @@ static int sf_launch(const SfArgs& a, int n_rows, int blocks, size_t smem, cudaS
   return e == cudaSuccess ? BN_OK : BN_ERR_LAUNCH + (int)e;
 }
 
-#define SF_KEYS_MAX 51200  // keys that a block holds beside its histogram
+#define SF_KEYS_MAX 48000  // keys that a block holds beside its counts and its list (and fewer than 2^7 per thread)
 
 // logits [n_rows, vocab] of `dtype`, rows ld numbers apart.  The four parameters hold for all rows where their array is null.  u: a number in
 // [0, 1) per row, or null: drawn from the generator rng[index ? index[r] : r], which is advanced.  out: the tokens, -1 for a row
@@ -365,12 +827,12 @@ extern "C" int bn_sample_filtered(const void* logits, int dtype, long long ld, i
   a.u = u; a.rng = rng; a.index = index; a.out = out;
   int bits = 0;
   while ((1ll << bits) < vocab) ++bits;
-  a.scale_bits = 62 - bits;  // the sum of all weights stays below 2^62
+  a.scale_bits = 62 - bits < SF_POINT ? 62 - bits : SF_POINT;  // the sum of all weights stays below 2^62
   int blocks = SF_MAX_CLUSTER;
   while (blocks > 1 && vocab <= (blocks / 2) * 2048) blocks /= 2;
   a.per = (((vocab + blocks - 1) / blocks) + 7) & ~7;
   const bool resident = a.per <= SF_KEYS_MAX;
-  const size_t smem = sizeof(SfShared) + (resident ? (size_t)a.per * 4 : 0);
+  const size_t smem = ((sizeof(SfShared) + 15) & ~(size_t)15) + (resident ? (size_t)a.per * 4 : 0);
   if (dtype == BN_F32) return resident ? sf_launch<float, true>(a, n_rows, blocks, smem, stream) : sf_launch<float, false>(a, n_rows, blocks, smem, stream);
   return resident ? sf_launch<__nv_bfloat16, true>(a, n_rows, blocks, smem, stream) : sf_launch<__nv_bfloat16, false>(a, n_rows, blocks, smem, stream);
 }
