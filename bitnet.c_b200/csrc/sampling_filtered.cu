@@ -6,20 +6,23 @@
 // is sorted: every border is "the first whose running sum (of ones, or of weights) exceeds a number", found by the bits of the logits.
 //
 // A cluster of blocks holds a row in its shared memory as ordered 32-bit keys, so that memory is read once however many passes
-// follow.  One pass counts the keys by their weight in steps of 2^(1/64): from the counts the first block knows lower and upper bounds of
-// every running sum, and so the few steps among which each border lies.  A second pass hands the keys of those steps to the first block and adds
+// follow.  One pass counts the keys by their weight in steps of 2^(1/32), and sums what the keys of a step fall short of its largest weight: from
+// these the first block knows every running sum closely enough to name the step or two in which each border lies.  A second pass hands the keys of those steps to the first block and adds
 // up the weights of the keys above each; the first block sorts what it got (some tens of keys, of a flat row some hundreds) and decides.  Where
 // too many keys lie together (ties by the thousand, a huge temperature), borders are found by the bits of the keys instead, 11, 11 and 10 at a time, the
 // weights of the keys that agree with the bits found so far added into a histogram.
 // Weights are whole numbers of 64 bits: sums do not depend on the order of additions, and a running sum that lies next to a border falls on the
-// same side as in a sum of doubles (a float sum would move a token in a thousand).  2^-y is taken apart into 2^-(j/64) from a table, a shift, and
-// 1 - e of a remainder below 1/64, whose e is small enough for a float: y = (max - l) / T * log2(e) is carried in two floats.
+// same side as in a sum of doubles (a float sum would move a token in a thousand).  2^-y is taken apart into 2^-(j/32) from a table, a shift, and
+// 1 - e of a remainder below 1/32, whose e is small enough for a float: y = (max - l) / T * log2(e) is carried in two floats.
 #include "common.cuh"
 
 #define SF_THREADS 512
 #define SF_BINS 2048     // of a histogram of bits
-#define SF_STEPS 4096    // of the counts by weight: 64 octaves of 64 steps
-#define SF_LIST 4096     // keys that the first block may be handed
+#define SF_STEPS 2048    // of the counts by weight: 64 octaves of 32 steps; the last one's keys weigh nothing
+#define SF_LIST 2048     // keys that the first block may be handed
+#define SF_FEW 256       // so many of them are one warp's work
+#define SF_REST_BITS 21  // a step's sum of what its keys fall short of its largest weight, 1 = 2^21
+#define SF_COUNTED 90000 // keys of a block whose shortfalls fit 32 bits whatever their steps
 #define SF_POINT 56      // a weight of 1 is 2^56 while a thread adds up its own (at most 2^7 of them)
 #define SF_MAX_CLUSTER 8
 
@@ -57,10 +60,17 @@ __device__ __forceinline__ unsigned sf_size() {
   asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
   return r;
 }
-__device__ __forceinline__ void sf_sync() {  // all threads of the cluster; what they wrote to shared memory is seen by all
+__device__ __forceinline__ void sf_arrive() {
   __syncwarp();
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void sf_wait() {
+  __syncwarp();
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void sf_sync() {  // all threads of the cluster; what they wrote to shared memory is seen by all
+  sf_arrive();
+  sf_wait();
 }
 __device__ __forceinline__ unsigned sf_remote(const void* p, unsigned rank) {
   unsigned r;
@@ -70,6 +80,11 @@ __device__ __forceinline__ unsigned sf_remote(const void* p, unsigned rank) {
 __device__ __forceinline__ unsigned long long sf_load(const unsigned long long* p, unsigned rank) {
   unsigned long long v;
   asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(sf_remote(p, rank)) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint4 sf_load4(const unsigned* p, unsigned rank) {  // 16-byte aligned
+  uint4 v;
+  asm volatile("ld.shared::cluster.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(sf_remote(p, rank)));
   return v;
 }
 __device__ __forceinline__ void sf_store(unsigned long long* p, unsigned rank, unsigned long long v) {
@@ -94,7 +109,9 @@ struct alignas(8) SfPlan {
 struct SfShared {
   union {
     unsigned long long hist[SF_BINS];
-    unsigned count[SF_STEPS];
+    struct {
+      unsigned count[SF_STEPS], shy[SF_STEPS];  // keys of a step, and by how much they fall short of its largest weight, in parts of that
+    };
     unsigned long long list[SF_LIST];  // keys falling, equal ones by index: (~key, index)
   };
   unsigned long long warp[SF_THREADS / 32];
@@ -105,10 +122,11 @@ struct SfShared {
   unsigned long long over[SF_MAX_CLUSTER][4];   // first block: of those above each range
   SfPlan plan;
   unsigned listed;                              // first block: keys in the list
-  unsigned long long table[64];                 // 2^-(j/64), 1 = 2^SF_POINT
-  int small_table[64];                          // the same, 1 = 2^30
+  unsigned long long table[32];                 // 2^-(j/32), 1 = 2^SF_POINT
+  int small_table[32];                          // the same, 1 = 2^30
+  unsigned long long warp4[SF_THREADS / 32][4];
   float warp_lower[SF_THREADS / 32], warp_upper[SF_THREADS / 32];
-  float got[8];
+  float got[4];
   int steps[8];
   unsigned long long base[4], sum[2];
   int at[4];
@@ -242,21 +260,25 @@ struct SfRow {
   }
 
   // ---- by steps of weight ----
-  // The step of a key (falling keys, rising steps) and what is behind it: y = step / 64 + rest.
+  // The step of a key (falling keys, rising steps) and what is behind it: y = step / 32 + rest.
   __device__ __forceinline__ int step_of(unsigned k, float* rest) const {
     const float v = sf_value(k), d = topf - v, bb = d - topf, dl = (topf - (d - bb)) - (v + bb);
     const float y = d * c_hi, yl = fmaf(d, c_hi, -y) + fmaf(d, c_lo, dl * c_hi);
-    const int n = min(__float2int_rd(y * 64.f), SF_STEPS - 1);
-    *rest = fmaf((float)n, -1.f / 64.f, y) + yl;
+    const int n = min(__float2int_rd(y * 32.f), SF_STEPS - 1);
+    *rest = fmaf((float)n, -1.f / 32.f, y) + yl;
     return n;
   }
-  __device__ __forceinline__ int step_of(unsigned k) const { return min(__float2int_rd((topf - sf_value(k)) * c_hi * 64.f), SF_STEPS - 1); }
-  // 2^-y, 1 = 2^SF_POINT, to 2^-31 of itself
-  __device__ __forceinline__ unsigned long long weight_at(int n, float rest) const {
-    const float g = rest * 0.69314718f, e = g * (1.f - g * (0.5f - g * (0.16666667f - g * 0.041666668f)));  // 1 - exp(-g)
+  __device__ __forceinline__ int step_of(unsigned k) const { return min(__float2int_rd((topf - sf_value(k)) * c_hi * 32.f), SF_STEPS - 1); }
+  // 1 - 2^-rest
+  static __device__ __forceinline__ float short_of(float rest) {
+    const float g = rest * 0.69314718f;
+    return g * (1.f - g * (0.5f - g * (0.16666667f - g * 0.041666668f)));
+  }
+  // 2^-y, 1 = 2^SF_POINT, to 2^-30 of itself
+  __device__ __forceinline__ unsigned long long weight_at(int n, float e) const {
     const int whole = __float2int_rn(e * 4294967296.f);
-    const unsigned long long w = s.table[n & 63] - (((long long)s.small_table[n & 63] * whole) >> (62 - SF_POINT));
-    return n == SF_STEPS - 1 ? 0ull : w >> (n >> 6);
+    const unsigned long long w = s.table[n & 31] - (((long long)s.small_table[n & 31] * whole) >> (62 - SF_POINT));
+    return n == SF_STEPS - 1 ? 0ull : w >> (n >> 5);
   }
   __device__ __forceinline__ unsigned long long to_scale(unsigned long long w) const {  // from 2^SF_POINT to 2^scale_bits
     const int down = SF_POINT - a.scale_bits;
@@ -283,45 +305,43 @@ struct SfRow {
       }
     }
   }
-  // Of the steps' weights, bounds that hold for every key of a step whatever its float rounding.
-  static __device__ __forceinline__ float upper(int n) { return n == 0 ? 1.0001f : exp2f(-(n - 0.02f) / 64.f); }
-  static __device__ __forceinline__ float lower(int n) { return n == SF_STEPS - 1 ? 0.f : exp2f(-(n + 1.02f) / 64.f); }
 
-  // First block: where the borders lie, from the counts of all blocks.  k, p, m: which filters there are.
-  __device__ void make_plan(bool k_on, unsigned top_k, bool p_on, float top_p, bool m_on, float min_p, float temperature, float u, unsigned long long all_mass) {
+  // All blocks: counts by weight.  SUMS: also what the steps fall short of, and the sum of this block's weights.
+  template <bool SUMS>
+  __device__ __forceinline__ unsigned long long count_steps() const {
+    unsigned long long mine = 0;
+    each_key([&](unsigned k, int) {
+      if (SUMS) {
+        float rest;
+        const int n = step_of(k, &rest);
+        const float e = short_of(rest);
+        atomicAdd(&s.count[n], 1u);
+        atomicAdd(&s.shy[n], (unsigned)max(0, __float2int_rn(e * (float)(1 << SF_REST_BITS))));
+        add(mine, weight_at(n, e));
+      } else {
+        atomicAdd(&s.count[step_of(k)], 1u);
+      }
+    });
+    return added(mine);
+  }
+
+  // First block: where the borders lie, from the counts of all blocks.  sums: count_steps had them.
+  __device__ void make_plan(bool sums, bool k_on, unsigned top_k, bool p_on, float top_p, bool m_on, float min_p, float temperature, float u,
+                            unsigned long long all_mass) {
     constexpr int EACH = SF_STEPS / SF_THREADS, NW = SF_THREADS / 32;
+    static_assert(EACH == 4, "a thread's steps are read 16 bytes at a time");
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n0 = tid * EACH;
-    unsigned c[EACH];
+    uint4 cv[SF_MAX_CLUSTER], ev[SF_MAX_CLUSTER];  // all of them asked for before the first is used
 #pragma unroll
-    for (int e = 0; e < EACH; ++e) c[e] = 0;
-    for (unsigned r = 0; r < blocks; ++r) {
-#pragma unroll
-      for (int e = 0; e < EACH; e += 4) {
-        uint4 v;
-        asm volatile("ld.shared::cluster.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(sf_remote(&s.count[n0 + e], r)) : "memory");
-        c[e] += v.x; c[e + 1] += v.y; c[e + 2] += v.z; c[e + 3] += v.w;
+    for (unsigned r = 0; r < SF_MAX_CLUSTER; ++r) {
+      cv[r] = ev[r] = make_uint4(0u, 0u, 0u, 0u);
+      if (r < blocks) {
+        cv[r] = sf_load4(&s.count[n0], r);
+        if (sums) ev[r] = sf_load4(&s.shy[n0], r);
       }
     }
-    // in front of this thread's steps: keys, and bounds of their weights
-    unsigned before = 0;
-    float low = 0.f, up = 0.f;
-#pragma unroll
-    for (int e = 0; e < EACH; ++e) {
-      before += c[e];
-      low += c[e] * lower(n0 + e);
-      up += c[e] * upper(n0 + e);
-    }
-    unsigned cs = before;
-    float ls = low, us = up;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const unsigned x = __shfl_up_sync(0xffffffffu, cs, o);
-      const float y = __shfl_up_sync(0xffffffffu, ls, o), z = __shfl_up_sync(0xffffffffu, us, o);
-      if (lane >= o) { cs += x; ls += y; us += z; }
-    }
-    if (lane == 31) { s.warp[warp] = cs; s.warp_lower[warp] = ls; s.warp_upper[warp] = us; }
     if (tid < 8) s.steps[tid] = -1;
-    if (tid == 0 && m_on) {
+    if (tid == SF_THREADS - 1 && m_on) {
       // the smallest key whose weight is at least min_p: near max + T log(min_p), found by trying its neighbours
       unsigned k = sf_key((float)(top + (double)temperature * log((double)min_p)));
       k = min(max(k, 1u), sf_key(topf));
@@ -329,52 +349,93 @@ struct SfRow {
       for (int i = 0; i < 8 && k < sf_key(topf) && !(weight(k) >= (double)min_p); ++i) ++k;
       s.plan.least = k;
     }
+    // keys of this thread's steps, and bounds of their weights' sums: with the sums a part in 10^5 apart, without them the step's own width
+    unsigned c[EACH];
+    float lo[EACH], up[EACH];
+    unsigned before = 0;
+    float low = 0.f, high = 0.f;
+    const float most = exp2f(-(float)n0 / 32.f);
+    constexpr float DOWN[EACH + 1] = {1.f, 0.97857206f, 0.95760328f, 0.93708382f, 0.91700404f};  // 2^(-e / 32)
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+      c[e] = 0;
+      float shy = 0.f;
+#pragma unroll
+      for (int r = 0; r < SF_MAX_CLUSTER; ++r) {
+        const unsigned cc = e == 0 ? cv[r].x : e == 1 ? cv[r].y : e == 2 ? cv[r].z : cv[r].w;
+        const unsigned ee = e == 0 ? ev[r].x : e == 1 ? ev[r].y : e == 2 ? ev[r].z : ev[r].w;
+        c[e] += cc;
+        shy += (float)ee;
+      }
+      const float n = (float)c[e], w = most * DOWN[e];
+      const float mid = w * (n - shy * (1.f / (1 << SF_REST_BITS)));
+      up[e] = sums ? mid * 1.00001f : w * n * 1.001f;
+      lo[e] = sums ? mid * 0.99999f : most * DOWN[e + 1] * n * 0.999f;
+      if (n0 + e == SF_STEPS - 1) up[e] = lo[e] = 0.f;
+      before += c[e];
+      low += lo[e];
+      high += up[e];
+    }
+    unsigned cs = before;
+    float ls = low, us = high;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const unsigned x = __shfl_up_sync(0xffffffffu, cs, o);
+      const float y = __shfl_up_sync(0xffffffffu, ls, o), z = __shfl_up_sync(0xffffffffu, us, o);
+      if (lane >= o) { cs += x; ls += y; us += z; }
+    }
+    if (lane == 31) { s.warp[warp] = cs; s.warp_lower[warp] = ls; s.warp_upper[warp] = us; }
     __syncthreads();
-    cs -= before; ls -= low; us -= up;
+    cs -= before; ls -= low; us -= high;
     unsigned total = 0;
+#pragma unroll
     for (int w = 0; w < NW; ++w) {
-      if (w < warp) { cs += (unsigned)s.warp[w]; ls += s.warp_lower[w]; us += s.warp_upper[w]; }
-      total += (unsigned)s.warp[w];
+      const unsigned x = (unsigned)s.warp[w];
+      if (w < warp) { cs += x; ls += s.warp_lower[w]; us += s.warp_upper[w]; }
+      total += x;
     }
     // the first step whose running sum exceeds thr by the upper or lower bound goes to steps[slot] (-1: none does)
     auto find = [&](int slot, float thr, bool by_upper) {
       float run = by_upper ? us : ls;
       unsigned mine = ~0u;
 #pragma unroll
-      for (int e = 0; e < EACH; ++e) {
-        run += c[e] * (by_upper ? upper(n0 + e) : lower(n0 + e));
-        if (mine == ~0u && c[e] && run > thr) mine = (unsigned)(n0 + e);
+      for (int e = EACH - 1; e >= 0; --e) {
+        float at = run;
+#pragma unroll
+        for (int x = 0; x <= e; ++x) at += by_upper ? up[x] : lo[x];
+        if (c[e] && at > thr) mine = (unsigned)(n0 + e);
       }
       mine = __reduce_min_sync(0xffffffffu, mine);
       if (lane == 0 && mine != ~0u) atomicMin((unsigned*)&s.steps[slot], mine);
     };
     const unsigned kth = min(top_k, total);
+    const int m_step = m_on ? step_of(s.plan.least) : SF_STEPS;
     {
       unsigned run = cs;
       float l = ls, h = us;
 #pragma unroll
       for (int e = 0; e < EACH; ++e) {
-        if (c[e] && run + c[e] == total) s.steps[7] = n0 + e;
         if (k_on && run < kth && run + c[e] >= kth) {
+          const float part = (float)(kth - run) / (float)c[e], w = most * DOWN[e] * (float)(kth - run);
           s.steps[0] = n0 + e;
           s.plan.rest = kth - run;
-          s.got[0] = l + (kth - run) * lower(n0 + e);
-          s.got[1] = h + (kth - run) * upper(n0 + e);
+          s.got[0] = part == 1.f ? l + lo[e] : n0 + e == SF_STEPS - 1 ? l : l + w * 0.978f;
+          s.got[1] = part == 1.f ? h + up[e] : n0 + e == SF_STEPS - 1 ? h : h + w * 1.001f;
         }
-        if (m_on && step_of(s.plan.least) == n0 + e) {
+        if (m_step == n0 + e) {
           s.got[2] = l;
-          s.got[3] = h + c[e] * upper(n0 + e);
+          s.got[3] = h + up[e];
         }
         run += c[e];
-        l += c[e] * lower(n0 + e);
-        h += c[e] * upper(n0 + e);
+        l += lo[e];
+        h += up[e];
       }
     }
     __syncthreads();
-    const float slack = 1e-4f;  // far more than the float sums of bounds are off
-    const int last = s.steps[7], k_step = k_on ? s.steps[0] : last, m_step = m_on ? step_of(s.plan.least) : SF_STEPS;
+    const float slack = 1e-5f;  // more than the float sums of bounds are off
+    const int k_step = k_on ? s.steps[0] : SF_STEPS - 1;
     const float exact = (float)ldexp((double)all_mass, -a.scale_bits);
-    const float all_low = k_on ? s.got[0] : exact, all_up = k_on ? s.got[1] : exact;  // (without a use for it, exact is 0 and not looked at)
+    const float all_low = k_on ? s.got[0] : exact, all_up = k_on ? s.got[1] : exact;
     if (p_on) {
       find(1, top_p * all_low * (1.f - slack), true);
       find(2, top_p * all_up * (1.f + slack), false);
@@ -383,18 +444,19 @@ struct SfRow {
     SfRange range[4];
 #pragma unroll
     for (int r = 0; r < 4; ++r) range[r] = SfRange{1, 0};
-    int cut = last;
+    // (no border that matters lies in the last step, whose keys weigh nothing: its keys are not asked for)
+    int cut = SF_STEPS - 2;
     float kept_low = all_low, kept_up = all_up;
-    if (k_on) { range[SF_TOP_K] = SfRange{k_step, k_step}; cut = k_step; }
+    if (k_on) { range[SF_TOP_K] = SfRange{k_step, k_step}; cut = min(cut, k_step); }
     if (p_on) {
       const int p1 = s.steps[2] < 0 ? cut : min(cut, s.steps[2]), p0 = s.steps[1] < 0 ? p1 : min(p1, s.steps[1]);
       range[SF_TOP_P] = SfRange{p0, p1};
       cut = p1;
       kept_low = top_p * all_low;
-      kept_up = top_p * all_up + upper(p0);
+      kept_up = top_p * all_up + exp2f(-(float)p0 / 32.f);
     }
-    if (m_on && m_step <= cut) {
-      if (!(k_on || p_on) || m_step < (p_on ? range[SF_TOP_P].first : k_step)) {  // what lies behind does not matter
+    if (m_on && (m_step <= cut || !(k_on || p_on))) {
+      if (m_step < (p_on ? range[SF_TOP_P].first : k_step) || !(k_on || p_on)) {  // what lies behind does not matter
         range[SF_TOP_K] = range[SF_TOP_P] = SfRange{1, 0};
         kept_low = s.got[2];
         kept_up = s.got[3];
@@ -404,10 +466,6 @@ struct SfRow {
       }
       range[SF_MIN_P] = SfRange{m_step, m_step};
       cut = min(cut, m_step);
-    } else if (m_on && !(k_on || p_on)) {  // everything stays
-      range[SF_MIN_P] = SfRange{last, last};
-      kept_low = s.got[2];
-      kept_up = s.got[3];
     }
     find(3, u * kept_low * (1.f - slack), true);
     find(4, u * kept_up * (1.f + slack), false);
@@ -420,37 +478,51 @@ struct SfRow {
       bool in = false;
 #pragma unroll
       for (int r = 0; r < 4; ++r) in |= n0 + e >= range[r].first && n0 + e <= range[r].last;
-      wanted += in ? c[e] : 0u;
+      wanted += in && n0 + e != SF_STEPS - 1 ? c[e] : 0u;
     }
-    wanted = (unsigned)block_sum64(wanted);
+    wanted = __reduce_add_sync(0xffffffffu, wanted);
+    if (lane == 0) s.warp[warp] = wanted;
+    __syncthreads();
     if (tid == 0) {
+      wanted = 0;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) wanted += (unsigned)s.warp[w];
 #pragma unroll
       for (int r = 0; r < 4; ++r) s.plan.range[r] = range[r];
       s.plan.by_bits = wanted > SF_LIST;
       s.listed = 0;
     }
+    __syncthreads();
+    constexpr int WORDS = sizeof(SfPlan) / 8;
+    if (tid < WORDS * (int)blocks && tid >= WORDS) sf_store(reinterpret_cast<unsigned long long*>(&s.plan) + tid % WORDS, tid / WORDS,
+                                                            reinterpret_cast<const unsigned long long*>(&s.plan)[tid % WORDS]);
   }
 
   // All blocks: the keys of the ranges to the first block, and the weights above each range.
-  __device__ void hand_over(const SfPlan& plan) {
+  __device__ void hand_over() {
     unsigned long long over[4] = {0, 0, 0, 0};
-    int first[4], end = 0;
+    int first[4], last[4], end = 0;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      first[r] = plan.range[r].last < plan.range[r].first ? 0 : plan.range[r].first;
-      end = max(end, plan.range[r].last);
+      first[r] = s.plan.range[r].first;
+      last[r] = s.plan.range[r].last;
+      if (last[r] < first[r]) first[r] = last[r] = -1;
+      end = max(end, last[r]);
+      last[r] = min(last[r], SF_STEPS - 2);
     }
     const int offset = (int)rank * a.per;
     each_key([&](unsigned k, int i) {
       float rest;
       const int n = step_of(k, &rest);
       if (n > end) return;
-      const unsigned long long w = weight_at(n, rest);
       bool in = false;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        if (n < first[r]) add(over[r], w);
-        in |= n >= plan.range[r].first && n <= plan.range[r].last;
+      for (int r = 0; r < 4; ++r) in |= n >= first[r] && n <= last[r];
+      if (n < max(max(first[0], first[1]), max(first[2], first[3]))) {
+        const unsigned long long w = weight_at(n, short_of(rest));
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (n < first[r]) add(over[r], w);
       }
       if (in) {
         unsigned at;
@@ -460,31 +532,46 @@ struct SfRow {
     });
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const unsigned long long sum = block_sum64(added(over[r]));
-      if (threadIdx.x == 0) sf_store(&s.over[rank][r], 0, sum);
+      over[r] = added(over[r]);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) over[r] += __shfl_xor_sync(0xffffffffu, over[r], o);
+    }
+    const int lane = threadIdx.x & 31;
+    if (lane < 4) s.warp4[threadIdx.x >> 5][lane] = lane == 0 ? over[0] : lane == 1 ? over[1] : lane == 2 ? over[2] : over[3];
+    __syncthreads();
+    if (threadIdx.x < 4) {
+      unsigned long long sum = 0;
+#pragma unroll
+      for (int w = 0; w < SF_THREADS / 32; ++w) sum += s.warp4[w][threadIdx.x];
+      sf_store(&s.over[rank][threadIdx.x], 0, sum);
     }
   }
 
-  // First block: sort what was handed over and walk the borders; the token.
+  // First block: sort what was handed over and walk the borders; the token.  GROUP: the threads that do it, one warp or all of the block.
+  template <int GROUP>
   __device__ void decide(bool k_on, bool p_on, float top_p, bool m_on, float u, unsigned long long all_mass, int* out) {
+    const auto sync = [] {
+      if (GROUP == 32) __syncwarp();
+      else __syncthreads();
+    };
     const int m = min((int)s.listed, SF_LIST), tid = threadIdx.x;
     int size = 2;
     while (size < m) size *= 2;
-    for (int i = m + tid; i < size; i += SF_THREADS) s.list[i] = ~0ull;
-    __syncthreads();
+    for (int i = m + tid; i < size; i += GROUP) s.list[i] = ~0ull;
+    sync();
     for (int k = 2; k <= size; k *= 2) {
       for (int j = k / 2; j > 0; j /= 2) {
-        for (int i = tid; i < size / 2; i += SF_THREADS) {
+        for (int i = tid; i < size / 2; i += GROUP) {
           const int x = 2 * i - (i & (j - 1)), y = x + j;
           const unsigned long long p = s.list[x], q = s.list[y];
           if ((p > q) == ((x & k) == 0)) { s.list[x] = q; s.list[y] = p; }
         }
-        __syncthreads();
+        sync();
       }
     }
     // running sums: thread t has entries t * each and on
-    constexpr int MOST = SF_LIST / SF_THREADS;
-    const int each = (m + SF_THREADS - 1) / SF_THREADS, i0 = tid * each;
+    constexpr int MOST = (GROUP == 32 ? SF_FEW : SF_LIST) / GROUP;
+    const int each = (m + GROUP - 1) / GROUP, i0 = tid * each;
     unsigned long long w[MOST], sum = 0;
     int step[MOST];
 #pragma unroll
@@ -494,7 +581,7 @@ struct SfRow {
       if (e < each && i0 + e < m) {
         float rest;
         step[e] = step_of(~(unsigned)(s.list[i0 + e] >> 32), &rest);
-        w[e] = to_scale(weight_at(step[e], rest));
+        w[e] = to_scale(weight_at(step[e], short_of(rest)));
       }
       sum += w[e];
     }
@@ -505,22 +592,31 @@ struct SfRow {
       const unsigned long long t = __shfl_up_sync(0xffffffffu, run0, o);
       if (lane >= o) run0 += t;
     }
-    if (lane == 31) s.warp[warp] = run0;
-    __syncthreads();
-    run0 -= sum;
-    unsigned long long total = 0;
-    for (int x = 0; x < SF_THREADS / 32; ++x) {
-      if (x < warp) run0 += s.warp[x];
-      total += s.warp[x];
+    unsigned long long total = __shfl_sync(0xffffffffu, run0, 31);
+    if (GROUP > 32) {
+      if (lane == 31) s.warp[warp] = run0;
+      __syncthreads();
+      total = 0;
+      for (int x = 0; x < GROUP / 32; ++x) {
+        if (x < warp) run0 += s.warp[x];
+        total += s.warp[x];
+      }
     }
+    run0 -= sum;
     unsigned long long over[4];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       over[r] = 0;
-      for (unsigned b = 0; b < blocks; ++b) over[r] += s.over[b][r];
+#pragma unroll
+      for (unsigned b = 0; b < SF_MAX_CLUSTER; ++b) over[r] += b < blocks ? s.over[b][r] : 0ull;
     }
+    SfRange range[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) range[r] = s.plan.range[r];
+    const auto is_in = [&](int r) { return range[r].last >= range[r].first; };
     if (tid < 4) { s.base[tid] = total; s.at[tid] = m; }
-    __syncthreads();
+    if (tid == 0) { s.sum[0] = k_on && is_in(SF_TOP_K) ? over[SF_TOP_K] : all_mass; s.sum[1] = is_in(SF_MIN_P) ? over[SF_MIN_P] : ~0ull; }
+    sync();
     // where each range begins, and the running sum in front of it
     {
       unsigned long long run = run0;
@@ -530,16 +626,13 @@ struct SfRow {
         if (e < each && i0 + e < m) {
 #pragma unroll
           for (int r = 0; r < 4; ++r)
-            if (step[e] >= s.plan.range[r].first && prev < s.plan.range[r].first) { s.base[r] = run; s.at[r] = i0 + e; }
+            if (step[e] >= range[r].first && prev < range[r].first) { s.base[r] = run; s.at[r] = i0 + e; }
           prev = step[e];
         }
         run += w[e];
       }
     }
-    __syncthreads();
-    const bool k_in = k_on && s.plan.range[SF_TOP_K].last >= s.plan.range[SF_TOP_K].first;
-    const bool p_in = p_on && s.plan.range[SF_TOP_P].last >= s.plan.range[SF_TOP_P].first;
-    const bool m_in = m_on && s.plan.range[SF_MIN_P].last >= s.plan.range[SF_MIN_P].first;
+    sync();
     // f(entry, running sum in front of it, with it)
     auto walk = [&](auto f) {
       unsigned long long run = run0;
@@ -549,43 +642,41 @@ struct SfRow {
         run += w[e];
       }
     };
-    if (tid == 0) { s.sum[0] = all_mass; s.sum[1] = ~0ull; }
-    __syncthreads();
-    if (k_in) {
+    if (is_in(SF_TOP_K)) {  // (in the last step, whose keys are not here, all that weighs lies above)
       const int at = s.at[SF_TOP_K] + (int)s.plan.rest - 1;
-      walk([&](int i, unsigned long long, unsigned long long run) {
+      if (range[SF_TOP_K].first != SF_STEPS - 1) walk([&](int i, unsigned long long, unsigned long long run) {
         if (i == at) s.sum[0] = over[SF_TOP_K] + run - s.base[SF_TOP_K];
       });
     }
-    if (m_in) {
-      // the last entry that stays; without one nothing of the range does
-      if (tid == 0) s.sum[1] = over[SF_MIN_P];
-      __syncthreads();
+    if (is_in(SF_MIN_P)) {  // the last entry that stays; without one nothing of the range does
       const int at0 = s.at[SF_MIN_P];
+      const unsigned least = s.plan.least;
       walk([&](int i, unsigned long long, unsigned long long run) {
-        if (i >= at0 && ~(unsigned)(s.list[i] >> 32) >= s.plan.least && (i + 1 >= m || ~(unsigned)(s.list[i + 1] >> 32) < s.plan.least))
+        if (i >= at0 && ~(unsigned)(s.list[i] >> 32) >= least && (i + 1 >= m || ~(unsigned)(s.list[i + 1] >> 32) < least))
           s.sum[1] = over[SF_MIN_P] + run - s.base[SF_MIN_P];
       });
     }
-    __syncthreads();
-    const unsigned long long by_k = s.sum[0], by_m = s.sum[1];
-    __syncthreads();
-    if (p_in) {
-      const unsigned long long thr = min((unsigned long long)((double)top_p * (double)by_k), by_k - 1);
+    sync();
+    unsigned long long kept = s.sum[0];
+    if (is_in(SF_TOP_P)) {
+      const unsigned long long thr = min((unsigned long long)((double)top_p * (double)kept), kept - 1);
       const int at0 = s.at[SF_TOP_P];
+      const unsigned long long off = over[SF_TOP_P] - s.base[SF_TOP_P];
+      sync();
       walk([&](int i, unsigned long long before, unsigned long long run) {
-        const unsigned long long off = over[SF_TOP_P] - s.base[SF_TOP_P];
         if (i >= at0 && before + off <= thr && run + off > thr) s.sum[0] = run + off;
       });
+      sync();
+      kept = s.sum[0];
     }
-    __syncthreads();
-    const unsigned long long kept = min((k_in || p_in || !m_in) ? s.sum[0] : ~0ull, by_m);
+    // (where min-p alone decides, the plan has no other range, and its sum is the smaller one)
+    if (is_in(SF_MIN_P)) kept = is_in(SF_TOP_K) || is_in(SF_TOP_P) ? min(kept, s.sum[1]) : s.sum[1];
     const unsigned long long thr = min((unsigned long long)((double)u * (double)kept), kept - 1);
     const int at0 = s.at[SF_DRAW];
+    const unsigned long long off = over[SF_DRAW] - s.base[SF_DRAW];
     if (tid == 0) *out = (int)(unsigned)s.list[min(at0, m - 1)];
-    __syncthreads();
+    sync();
     walk([&](int i, unsigned long long before, unsigned long long run) {
-      const unsigned long long off = over[SF_DRAW] - s.base[SF_DRAW];
       if (i >= at0 && before + off <= thr && run + off > thr) *out = (int)(unsigned)s.list[i];
     });
   }
@@ -663,9 +754,10 @@ __global__ void __launch_bounds__(SF_THREADS, 2) sample_filtered_kernel(const __
   const int r = blockIdx.x / blocks;
   const int first = min(a.vocab, (int)rank * a.per);
   SfRow<T, RESIDENT> row{a, s, keys, (const T*)a.logits + (size_t)r * a.ld + first, min(a.vocab, first + a.per) - first, rank, blocks};
-  for (int b = threadIdx.x; b < SF_STEPS; b += SF_THREADS) s.count[b] = 0;
-  if (threadIdx.x < 64) {
-    const double x = exp2(-(double)threadIdx.x / 64.0);
+  sf_arrive();
+  for (int b = threadIdx.x; b < SF_STEPS; b += SF_THREADS) s.count[b] = s.shy[b] = 0;
+  if (threadIdx.x < 32) {
+    const double x = exp2(-(double)threadIdx.x / 32.0);
     s.table[threadIdx.x] = (unsigned long long)__double2ll_rn(ldexp(x, SF_POINT));
     s.small_table[threadIdx.x] = __double2int_rn(ldexp(x, 30));
   }
@@ -675,7 +767,7 @@ __global__ void __launch_bounds__(SF_THREADS, 2) sample_filtered_kernel(const __
   const float min_p = asked > 0.f ? fminf(asked, 1.f) : 0.f;  // the most probable token always stays
   const int top_k = a.top_ks ? a.top_ks[r] : a.top_k;
   unsigned high = sf_read<T, RESIDENT>(row.row, row.n, a.per, keys);
-  sf_sync();  // every block of the cluster runs: its shared memory may be written
+  sf_wait();  // every block of the cluster runs: its shared memory may be written
   // the random number, drawn once for the whole cluster
   if (rank == 0 && threadIdx.x == 0) {
     float u;
@@ -708,45 +800,31 @@ __global__ void __launch_bounds__(SF_THREADS, 2) sample_filtered_kernel(const __
     row.c_hi = (float)c;
     row.c_lo = (float)(c - (double)row.c_hi);
     const bool k_on = top_k > 0 && top_k < a.vocab, p_on = top_p > 0.f && top_p < 1.f, m_on = min_p > 0.f;
-    bool by_bits = row.infinite || !(c > 1e-30 && c < 1e30);  // (a temperature near the ends of float's range)
+    // (a temperature near the ends of float's range; so many keys that a step's sums could overflow)
+    bool by_bits = row.infinite || !(c > 1e-30 && c < 1e30) || a.per > SF_COUNTED;
     if (!by_bits) {
-      // counts by weight; the sum of all weights where a border asks for it
-      const bool need = !k_on && (p_on || !m_on);
-      unsigned long long mine = 0;
-      if (need) {
-        row.each_key([&](unsigned k, int) {
-          float rest;
-          const int n = row.step_of(k, &rest);
-          atomicAdd(&s.count[n], 1u);
-          row.add(mine, row.weight_at(n, rest));
-        });
-      } else {
-        row.each_key([&](unsigned k, int) { atomicAdd(&s.count[row.step_of(k)], 1u); });
-      }
-      const unsigned long long sum = row.block_sum64(row.added(mine));
+      // Sums as well, unless top-k leaves few tokens: then the bounds that counts alone give are close enough to find borders among those, and the sum of
+      // all weights is not asked for (one row of 32,000 and k = 50: 1.3 us for the counts, 2.0 with sums).
+      const bool sums = !k_on || top_k > SF_LIST / 2;
+      const unsigned long long sum = row.block_sum64(sums ? row.template count_steps<true>() : row.template count_steps<false>());
       if (threadIdx.x == 0) sf_store(&s.mass[rank], 0, sum);
       sf_sync();
       unsigned long long all_mass = 0;
       if (rank == 0) {
         for (unsigned b = 0; b < blocks; ++b) all_mass += s.mass[b];
-        row.make_plan(k_on, (unsigned)top_k, p_on, top_p, m_on, min_p, temperature, u, all_mass);
+        row.make_plan(sums, k_on, (unsigned)top_k, p_on, top_p, m_on, min_p, temperature, u, all_mass);
       }
       sf_sync();
-      SfPlan plan;
-      {
-        constexpr int WORDS = sizeof(SfPlan) / 8;
-        unsigned long long* to = reinterpret_cast<unsigned long long*>(&plan);
-#pragma unroll
-        for (int i = 0; i < WORDS; ++i) to[i] = sf_load(reinterpret_cast<const unsigned long long*>(&s.plan) + i, 0);
-      }
-      by_bits = plan.by_bits;
+      by_bits = s.plan.by_bits;
       if (!by_bits) {
-        row.hand_over(plan);
+        row.hand_over();
         sf_sync();  // the last time that another block is needed
-        if (rank == 0) row.decide(k_on, p_on, top_p, m_on, u, all_mass, a.out + r);
+        if (rank == 0) {
+          if (s.listed > SF_FEW) row.template decide<SF_THREADS>(k_on, p_on, top_p, m_on, u, all_mass, a.out + r);
+          else if (threadIdx.x < 32) row.template decide<32>(k_on, p_on, top_p, m_on, u, all_mass, a.out + r);
+        }
         return;
       }
-      sf_sync();  // the plan has been read: shared memory is used anew
     }
     unsigned long long valid = 0, before;
     row.each_key([&](unsigned, int) { ++valid; });
