@@ -6,23 +6,22 @@
 // is sorted: every border is "the first whose running sum (of ones, or of weights) exceeds a number", found by the bits of the logits.
 //
 // A cluster of blocks holds a row in its shared memory as ordered 32-bit keys, so that memory is read once however many passes
-// follow.  One pass counts the keys by their weight in steps of 2^(1/32), and sums what the keys of a step fall short of its largest weight: from
-// these the first block knows every running sum closely enough to name the step or two in which each border lies.  A second pass hands the keys of those steps to the first block and adds
-// up the weights of the keys above each; the first block sorts what it got (some tens of keys, of a flat row some hundreds) and decides.  Where
-// too many keys lie together (ties by the thousand, a huge temperature), borders are found by the bits of the keys instead, 11, 11 and 10 at a time, the
-// weights of the keys that agree with the bits found so far added into a histogram.
+// follow.  One pass adds up the keys' weights (with top-k: counts the keys) in steps of 2^(1/32) of the weight; from these sums the first block of the
+// cluster knows in which step each border lies.  A second pass hands the keys of those steps to it; it sorts them (some tens of keys, of a flat row
+// hundreds) and decides.  Where too many keys lie together (ties by the thousand, a huge temperature), borders are found by the bits of the keys
+// instead, 11, 11 and 10 at a time, the weights of the keys that agree with the bits found so far added into a histogram.
 // Weights are whole numbers of 64 bits: sums do not depend on the order of additions, and a running sum that lies next to a border falls on the
 // same side as in a sum of doubles (a float sum would move a token in a thousand).  2^-y is taken apart into 2^-(j/32) from a table, a shift, and
 // 1 - e of a remainder below 1/32, whose e is small enough for a float: y = (max - l) / T * log2(e) is carried in two floats.
 #include "common.cuh"
+#include <math.h>
 
 #define SF_THREADS 512
 #define SF_BINS 2048     // of a histogram of bits
 #define SF_STEPS 2048    // of the counts by weight: 64 octaves of 32 steps; the last one's keys weigh nothing
 #define SF_LIST 2048     // keys that the first block may be handed
-#define SF_FEW 256       // so many of them are one warp's work
-#define SF_REST_BITS 21  // a step's sum of what its keys fall short of its largest weight, 1 = 2^21
-#define SF_COUNTED 90000 // keys of a block whose shortfalls fit 32 bits whatever their steps
+#define SF_FEW 128       // so many of them are one warp's work
+#define SF_COUNTED 65536 // keys of a block whose weights' halves add up in 32 bits whatever their steps
 #define SF_POINT 56      // a weight of 1 is 2^56 while a thread adds up its own (at most 2^7 of them)
 #define SF_MAX_CLUSTER 8
 
@@ -41,6 +40,7 @@ struct SfArgs {
   const int* index;           // row -> its generator, or null
   int* out;
   int scale_bits;             // weights are multiples of 2^-scale_bits
+  unsigned long long table[32];  // 2^-(j/32), 1 = 2^SF_POINT
 };
 
 __device__ __forceinline__ unsigned sf_key(float v) {
@@ -49,6 +49,22 @@ __device__ __forceinline__ unsigned sf_key(float v) {
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ float sf_value(unsigned key) { return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key); }
+
+// What a block holds of a row: of a bfloat16 the upper half of its key (the lower half follows from the sign).
+template <typename T>
+struct SfHeld;
+template <>
+struct SfHeld<float> {
+  typedef unsigned Key;
+  static __device__ __forceinline__ Key pack(unsigned k) { return k; }
+  static __device__ __forceinline__ unsigned key(Key h) { return h; }
+};
+template <>
+struct SfHeld<__nv_bfloat16> {
+  typedef unsigned short Key;
+  static __device__ __forceinline__ Key pack(unsigned k) { return (Key)(k >> 16); }
+  static __device__ __forceinline__ unsigned key(Key h) { return h == 0 ? 0u : ((unsigned)h << 16) | (h & 0x8000u ? 0u : 0xffffu); }
+};
 
 __device__ __forceinline__ unsigned sf_rank() {
   unsigned r;
@@ -68,9 +84,13 @@ __device__ __forceinline__ void sf_wait() {
   __syncwarp();
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ void sf_sync() {  // all threads of the cluster; what they wrote to shared memory is seen by all
-  sf_arrive();
-  sf_wait();
+__device__ __forceinline__ void sf_sync(unsigned blocks) {  // all threads of the cluster; what they wrote to shared memory is seen by all
+  if (blocks == 1) {
+    __syncthreads();
+  } else {
+    sf_arrive();
+    sf_wait();
+  }
 }
 __device__ __forceinline__ unsigned sf_remote(const void* p, unsigned rank) {
   unsigned r;
@@ -107,10 +127,12 @@ struct alignas(8) SfPlan {
 #define SF_DRAW 3
 
 struct SfShared {
+  ulonglong2 warp_sums[SF_THREADS / 32];  // first block: bounds of the weights of a warp's steps
   union {
     unsigned long long hist[SF_BINS];
     struct {
-      unsigned count[SF_STEPS], shy[SF_STEPS];  // keys of a step, and by how much they fall short of its largest weight, in parts of that
+      // of a step's keys their number, in two parts; or the sum of their weights in parts of 2^-31 of its largest, upper and lower 16 bits apart
+      unsigned one[SF_STEPS], two[SF_STEPS];
     };
     unsigned long long list[SF_LIST];  // keys falling, equal ones by index: (~key, index)
   };
@@ -118,15 +140,15 @@ struct SfShared {
   // one entry per block of the cluster, written by that block; two sets in turn, so that one barrier per exchange is enough
   unsigned long long part[2][SF_MAX_CLUSTER];
   unsigned long long found[2];  // what the block that found a border tells the others
-  unsigned long long mass[SF_MAX_CLUSTER];      // first block: the weights of each block's keys
-  unsigned long long over[SF_MAX_CLUSTER][4];   // first block: of those above each range
+  unsigned long long over[SF_MAX_CLUSTER][4];   // first block: the weights of each block's keys above each range
+  unsigned long long all_mass;                  // first block: of all keys (not with top-k)
   SfPlan plan;
   unsigned listed;                              // first block: keys in the list
+  unsigned high;                                // the largest key of this block
   unsigned long long table[32];                 // 2^-(j/32), 1 = 2^SF_POINT
   int small_table[32];                          // the same, 1 = 2^30
   unsigned long long warp4[SF_THREADS / 32][4];
-  float warp_lower[SF_THREADS / 32], warp_upper[SF_THREADS / 32];
-  float got[4];
+  unsigned long long got[4];
   int steps[8];
   unsigned long long base[4], sum[2];
   int at[4];
@@ -136,7 +158,8 @@ template <typename T, bool RESIDENT>
 struct SfRow {
   SfArgs a;
   SfShared& s;
-  const unsigned* keys;  // shared memory, RESIDENT
+  typedef SfHeld<T> Held;
+  const typename Held::Key* keys;  // shared memory, RESIDENT
   const T* row;          // this block's part of the row
   int n;                 // numbers of it
   unsigned rank, blocks;
@@ -145,7 +168,7 @@ struct SfRow {
   bool infinite;         // the largest logit is +inf: those share everything
   float topf, c_hi, c_lo;  // the largest logit, log2(e) / temperature in two floats
 
-  __device__ __forceinline__ unsigned key(int i) const { return RESIDENT ? keys[i] : sf_key(to_f32<T>(row[i])); }
+  __device__ __forceinline__ unsigned key(int i) const { return RESIDENT ? Held::key(keys[i]) : sf_key(to_f32<T>(row[i])); }
   __device__ __forceinline__ double weight(unsigned k) const {
     const double v = (double)sf_value(k);
     return infinite ? (v == top ? 1.0 : 0.0) : exp((v - top) * per_t);
@@ -158,16 +181,16 @@ struct SfRow {
     __syncthreads();
     if ((threadIdx.x & 31) == 0) s.warp[threadIdx.x >> 5] = v;
     __syncthreads();
-    unsigned long long all = 0;
+    v = (threadIdx.x & 31) < SF_THREADS / 32 ? s.warp[threadIdx.x & 31] : 0;
 #pragma unroll
-    for (int w = 0; w < SF_THREADS / 32; ++w) all += s.warp[w];
-    return all;
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
   }
   // Every block's number to every block; *before: the sum over the blocks with a lower rank.
   __device__ unsigned long long exchange_sum(unsigned long long v, unsigned long long* before) {
     const int t = turn++ & 1;
     if (threadIdx.x < blocks) sf_store(&s.part[t][rank], threadIdx.x, v);
-    sf_sync();
+    sf_sync(blocks);
     unsigned long long all = 0, low = 0;
     for (unsigned r = 0; r < blocks; ++r) {
       if (r < rank) low += s.part[t][r];
@@ -179,7 +202,7 @@ struct SfRow {
   __device__ unsigned exchange_max(unsigned v) {
     const int t = turn++ & 1;
     if (threadIdx.x < blocks) sf_store(&s.part[t][rank], threadIdx.x, v);
-    sf_sync();
+    sf_sync(blocks);
     unsigned m = 0;
     for (unsigned r = 0; r < blocks; ++r) m = max(m, (unsigned)s.part[t][r]);
     return m;
@@ -205,7 +228,7 @@ struct SfRow {
           if (w) atomicAdd(&s.hist[(k >> shift) & low_bits], w);
         }
       }
-      sf_sync();
+      sf_sync(blocks);
       // this block's share of the bins, higher ranks the higher bins; thread t the t-th of them
       const int share = SF_BINS / (int)blocks, b0 = (int)rank * share;
       constexpr int MOST = SF_BINS / SF_THREADS;  // bins of a thread when one block has them all
@@ -250,7 +273,7 @@ struct SfRow {
         }
         if (e < each) run += mine[e];
       }
-      sf_sync();
+      sf_sync(blocks);
       prefix |= (unsigned)s.found[0] << shift;
       mask |= low_bits << shift;
       over = s.found[1];
@@ -287,173 +310,200 @@ struct SfRow {
   // A thread adds up its weights with SF_POINT bits behind the point while it has few of them (a row that is held), else with as many as the sums have.
   __device__ __forceinline__ void add(unsigned long long& sum, unsigned long long w) const { sum += RESIDENT ? w : to_scale(w); }
   __device__ __forceinline__ unsigned long long added(unsigned long long sum) const { return RESIDENT ? to_scale(sum) : sum; }
-  // f(key, index) for the keys above -inf of this block
+  // f(key, index) for this block's keys from `least` (above 0) on
   template <class F>
-  __device__ __forceinline__ void each_key(F f) const {
+  __device__ __forceinline__ void each_key(unsigned least, F f) const {
     if (RESIDENT) {  // (the keys behind the last are 0)
-      for (int i = threadIdx.x * 4; i < n; i += SF_THREADS * 4) {
-        const uint4 k = *reinterpret_cast<const uint4*>(keys + i);
-        if (k.x) f(k.x, i);
-        if (k.y) f(k.y, i + 1);
-        if (k.z) f(k.z, i + 2);
-        if (k.w) f(k.w, i + 3);
+      constexpr int V = 16 / (int)sizeof(typename Held::Key);
+#pragma unroll 1
+      for (int i = threadIdx.x * V; i < n; i += SF_THREADS * V) {
+        const uint4 raw = *reinterpret_cast<const uint4*>(keys + i);
+        const typename Held::Key* h = reinterpret_cast<const typename Held::Key*>(&raw);
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          const unsigned k = Held::key(h[e]);
+          if (k >= least) f(k, i + e);
+        }
       }
-    } else {
-      for (int i = threadIdx.x; i < n; i += SF_THREADS) {
-        const unsigned k = key(i);
-        if (k) f(k, i);
+      return;
+    }
+    constexpr int V = 16 / (int)sizeof(T);
+    int done = 0;
+    if ((((uintptr_t)row) & 15) == 0) {
+      const int nv = n / V;
+      done = nv * V;
+#pragma unroll 1
+      for (int i = threadIdx.x; i < nv; i += 2 * SF_THREADS) {  // two loads in flight
+        const uint4 raw[2] = {__ldg(reinterpret_cast<const uint4*>(row) + i), __ldg(reinterpret_cast<const uint4*>(row) + min(i + SF_THREADS, nv - 1))};
+        const T* x = reinterpret_cast<const T*>(raw);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          if (half && i + SF_THREADS >= nv) break;
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            const unsigned k = sf_key(to_f32<T>(x[half * V + e]));
+            if (k >= least) f(k, (i + half * SF_THREADS) * V + e);
+          }
+        }
       }
+    }
+#pragma unroll 1
+    for (int i = done + threadIdx.x; i < n; i += SF_THREADS) {
+      const unsigned k = key(i);
+      if (k >= least) f(k, i);
     }
   }
 
-  // All blocks: counts by weight.  SUMS: also what the steps fall short of, and the sum of this block's weights.
-  template <bool SUMS>
-  __device__ __forceinline__ unsigned long long count_steps() const {
-    unsigned long long mine = 0;
-    each_key([&](unsigned k, int) {
-      if (SUMS) {
+  // All blocks: the keys by their steps.  With top-k their numbers (in two histograms, for even and odd lanes, so that fewer lanes of a warp meet); without it
+  // their weights, to 2^-31 of themselves.
+  __device__ __forceinline__ void count_steps(bool numbers) const {
+    if (numbers) {
+      unsigned* mine = threadIdx.x & 1 ? s.two : s.one;
+      each_key(1u, [&](unsigned k, int) { atomicAdd(mine + step_of(k), 1u); });
+    } else {
+      each_key(1u, [&](unsigned k, int) {
         float rest;
         const int n = step_of(k, &rest);
-        const float e = short_of(rest);
-        atomicAdd(&s.count[n], 1u);
-        atomicAdd(&s.shy[n], (unsigned)max(0, __float2int_rn(e * (float)(1 << SF_REST_BITS))));
-        add(mine, weight_at(n, e));
-      } else {
-        atomicAdd(&s.count[step_of(k)], 1u);
-      }
-    });
-    return added(mine);
+        const unsigned w = 0x80000000u - (unsigned)__float2int_rn(short_of(rest) * 2147483648.f);
+        atomicAdd(&s.one[n], w >> 16);
+        atomicAdd(&s.two[n], w & 0xffffu);
+      });
+    }
   }
 
-  // First block: where the borders lie, from the counts of all blocks.  sums: count_steps had them.
-  __device__ void make_plan(bool sums, bool k_on, unsigned top_k, bool p_on, float top_p, bool m_on, float min_p, float temperature, float u,
-                            unsigned long long all_mass) {
+  // First block: the steps in which the borders lie, from what all blocks have counted.
+  __device__ void make_plan(bool k_on, unsigned top_k, bool p_on, float top_p, bool m_on, float min_p, float temperature, float u) {
     constexpr int EACH = SF_STEPS / SF_THREADS, NW = SF_THREADS / 32;
     static_assert(EACH == 4, "a thread's steps are read 16 bytes at a time");
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n0 = tid * EACH;
-    uint4 cv[SF_MAX_CLUSTER], ev[SF_MAX_CLUSTER];  // all of them asked for before the first is used
+    unsigned long long one[EACH] = {}, two[EACH] = {};
+#pragma unroll 1
+    for (unsigned r0 = 0; r0 < blocks; r0 += 4) {
+      uint4 ones[4], twos[4];  // all of them asked for before the first is used
 #pragma unroll
-    for (unsigned r = 0; r < SF_MAX_CLUSTER; ++r) {
-      cv[r] = ev[r] = make_uint4(0u, 0u, 0u, 0u);
-      if (r < blocks) {
-        cv[r] = sf_load4(&s.count[n0], r);
-        if (sums) ev[r] = sf_load4(&s.shy[n0], r);
+      for (unsigned r = 0; r < 4; ++r) {
+        ones[r] = r0 + r < blocks ? sf_load4(&s.one[n0], r0 + r) : make_uint4(0u, 0u, 0u, 0u);
+        twos[r] = r0 + r < blocks ? sf_load4(&s.two[n0], r0 + r) : make_uint4(0u, 0u, 0u, 0u);
+      }
+#pragma unroll
+      for (unsigned r = 0; r < 4; ++r) {
+        one[0] += ones[r].x; one[1] += ones[r].y; one[2] += ones[r].z; one[3] += ones[r].w;
+        two[0] += twos[r].x; two[1] += twos[r].y; two[2] += twos[r].z; two[3] += twos[r].w;
       }
     }
     if (tid < 8) s.steps[tid] = -1;
-    if (tid == SF_THREADS - 1 && m_on) {
-      // the smallest key whose weight is at least min_p: near max + T log(min_p), found by trying its neighbours
-      unsigned k = sf_key((float)(top + (double)temperature * log((double)min_p)));
-      k = min(max(k, 1u), sf_key(topf));
-      for (int i = 0; i < 8 && k > 1u && weight(k - 1) >= (double)min_p; ++i) --k;
-      for (int i = 0; i < 8 && k < sf_key(topf) && !(weight(k) >= (double)min_p); ++i) ++k;
-      s.plan.least = k;
-    }
-    // keys of this thread's steps, and bounds of their weights' sums: with the sums a part in 10^5 apart, without them the step's own width
+    // the smallest key whose weight is at least min_p: exp((v - max) / T) >= min_p where v >= max + T log(min_p)
+    if (tid == SF_THREADS - 1 && m_on) s.plan.least = min(max(sf_key(__double2float_ru(top + (double)temperature * log((double)min_p))), 1u), sf_key(topf));
+    // of each step its keys (without top-k: at least so many) and bounds of their weights' sum, which are the sum itself without top-k; the last step's keys
+    // weigh nothing
     unsigned c[EACH];
-    float lo[EACH], up[EACH];
+    unsigned long long lo[EACH], up[EACH];
     unsigned before = 0;
-    float low = 0.f, high = 0.f;
-    const float most = exp2f(-(float)n0 / 32.f);
-    constexpr float DOWN[EACH + 1] = {1.f, 0.97857206f, 0.95760328f, 0.93708382f, 0.91700404f};  // 2^(-e / 32)
+    unsigned long long low = 0, high = 0;
 #pragma unroll
     for (int e = 0; e < EACH; ++e) {
-      c[e] = 0;
-      float shy = 0.f;
-#pragma unroll
-      for (int r = 0; r < SF_MAX_CLUSTER; ++r) {
-        const unsigned cc = e == 0 ? cv[r].x : e == 1 ? cv[r].y : e == 2 ? cv[r].z : cv[r].w;
-        const unsigned ee = e == 0 ? ev[r].x : e == 1 ? ev[r].y : e == 2 ? ev[r].z : ev[r].w;
-        c[e] += cc;
-        shy += (float)ee;
+      const int n = n0 + e;
+      const unsigned long long t = s.table[n & 31] >> (n >> 5);  // the step's largest weight
+      if (k_on) {
+        c[e] = (unsigned)(one[e] + two[e]);
+        const unsigned long long t1 = s.table[(n + 1) & 31] >> ((n + 1) >> 5);
+        up[e] = c[e] * (to_scale(t + (t >> 10)) + 1);
+        lo[e] = c[e] * to_scale(t1 - (t1 >> 10));
+      } else {
+        const unsigned long long w = (one[e] << 16) + two[e];  // 1 = 2^31, below 2^51
+        c[e] = (unsigned)((w + (w >> 5)) >> 31) + (w ? 1u : 0u);
+        // w * t / 2^31, t of SF_POINT bits, to 2^scale_bits
+        const int down = 31 + SF_POINT - a.scale_bits;
+        const unsigned long long h = __umul64hi(w, t), l = w * t;
+        const unsigned long long half = 1ull << (down - 1), l2 = l + half;
+        up[e] = lo[e] = ((h + (l2 < l)) << (64 - down)) | (l2 >> down);
       }
-      const float n = (float)c[e], w = most * DOWN[e];
-      const float mid = w * (n - shy * (1.f / (1 << SF_REST_BITS)));
-      up[e] = sums ? mid * 1.00001f : w * n * 1.001f;
-      lo[e] = sums ? mid * 0.99999f : most * DOWN[e + 1] * n * 0.999f;
-      if (n0 + e == SF_STEPS - 1) up[e] = lo[e] = 0.f;
+      if (n == SF_STEPS - 1) up[e] = lo[e] = 0;
       before += c[e];
       low += lo[e];
       high += up[e];
     }
     unsigned cs = before;
-    float ls = low, us = high;
+    unsigned long long ls = low, us = high;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const unsigned x = __shfl_up_sync(0xffffffffu, cs, o);
-      const float y = __shfl_up_sync(0xffffffffu, ls, o), z = __shfl_up_sync(0xffffffffu, us, o);
+      const unsigned long long y = __shfl_up_sync(0xffffffffu, ls, o), z = __shfl_up_sync(0xffffffffu, us, o);
       if (lane >= o) { cs += x; ls += y; us += z; }
     }
-    if (lane == 31) { s.warp[warp] = cs; s.warp_lower[warp] = ls; s.warp_upper[warp] = us; }
+    if (lane == 31) {
+      s.warp_sums[warp] = make_ulonglong2(ls, us);
+      s.warp[warp] = cs;
+    }
     __syncthreads();
     cs -= before; ls -= low; us -= high;
     unsigned total = 0;
-#pragma unroll
+    unsigned long long all_low = 0;
+#pragma unroll 4
     for (int w = 0; w < NW; ++w) {
-      const unsigned x = (unsigned)s.warp[w];
-      if (w < warp) { cs += x; ls += s.warp_lower[w]; us += s.warp_upper[w]; }
-      total += x;
+      const ulonglong2 x = s.warp_sums[w];
+      const unsigned y = (unsigned)s.warp[w];
+      if (w < warp) { cs += y; ls += x.x; us += x.y; }
+      total += y;
+      all_low += x.x;
     }
-    // the first step whose running sum exceeds thr by the upper or lower bound goes to steps[slot] (-1: none does)
-    auto find = [&](int slot, float thr, bool by_upper) {
-      float run = by_upper ? us : ls;
-      unsigned mine = ~0u;
+    unsigned long long all_up = all_low;
+    const unsigned long long ls_before = ls;
+    // from here on running sums, each with its step
+    unsigned ci[EACH];
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+      cs += c[e]; ls += lo[e]; us += up[e];
+      ci[e] = cs; lo[e] = ls; up[e] = us;
+    }
+    // the first step whose running sum exceeds thr, by the upper and the lower bound, goes to steps[slot] and steps[slot + 1] (-1: none does)
+    auto find = [&](int slot, unsigned long long thr_up, unsigned long long thr_lo) {
+      unsigned by_up = ~0u, by_lo = ~0u;
 #pragma unroll
       for (int e = EACH - 1; e >= 0; --e) {
-        float at = run;
-#pragma unroll
-        for (int x = 0; x <= e; ++x) at += by_upper ? up[x] : lo[x];
-        if (c[e] && at > thr) mine = (unsigned)(n0 + e);
+        if (up[e] > thr_up) by_up = (unsigned)(n0 + e);
+        if (lo[e] > thr_lo) by_lo = (unsigned)(n0 + e);
       }
-      mine = __reduce_min_sync(0xffffffffu, mine);
-      if (lane == 0 && mine != ~0u) atomicMin((unsigned*)&s.steps[slot], mine);
+      by_up = __reduce_min_sync(0xffffffffu, by_up);
+      by_lo = __reduce_min_sync(0xffffffffu, by_lo);
+      if (lane == 0 && by_up != ~0u) atomicMin((unsigned*)&s.steps[slot], by_up);
+      if (lane == 0 && by_lo != ~0u) atomicMin((unsigned*)&s.steps[slot + 1], by_lo);
     };
     const unsigned kth = min(top_k, total);
     const int m_step = m_on ? step_of(s.plan.least) : SF_STEPS;
-    {
-      unsigned run = cs;
-      float l = ls, h = us;
 #pragma unroll
-      for (int e = 0; e < EACH; ++e) {
-        if (k_on && run < kth && run + c[e] >= kth) {
-          const float part = (float)(kth - run) / (float)c[e], w = most * DOWN[e] * (float)(kth - run);
-          s.steps[0] = n0 + e;
-          s.plan.rest = kth - run;
-          s.got[0] = part == 1.f ? l + lo[e] : n0 + e == SF_STEPS - 1 ? l : l + w * 0.978f;
-          s.got[1] = part == 1.f ? h + up[e] : n0 + e == SF_STEPS - 1 ? h : h + w * 1.001f;
-        }
-        if (m_step == n0 + e) {
-          s.got[2] = l;
-          s.got[3] = h + up[e];
-        }
-        run += c[e];
-        l += lo[e];
-        h += up[e];
+    for (int e = 0; e < EACH; ++e) {
+      if (k_on && ci[e] - c[e] < kth && ci[e] >= kth) {
+        s.steps[0] = n0 + e;
+        s.plan.rest = kth - (ci[e] - c[e]);
+        s.got[0] = e ? lo[e - 1] : ls_before;  // (some of the step's weights stay)
+        s.got[1] = up[e];
+      }
+      if (m_step == n0 + e) {
+        s.got[2] = e ? lo[e - 1] : ls_before;
+        s.got[3] = up[e];
       }
     }
     __syncthreads();
-    const float slack = 1e-5f;  // more than the float sums of bounds are off
     const int k_step = k_on ? s.steps[0] : SF_STEPS - 1;
-    const float exact = (float)ldexp((double)all_mass, -a.scale_bits);
-    const float all_low = k_on ? s.got[0] : exact, all_up = k_on ? s.got[1] : exact;
-    if (p_on) {
-      find(1, top_p * all_low * (1.f - slack), true);
-      find(2, top_p * all_up * (1.f + slack), false);
-    }
+    if (k_on) { all_low = s.got[0]; all_up = s.got[1]; }
+    const auto part = [](float share, unsigned long long of) { return (unsigned long long)((double)share * (double)of); };
+    if (p_on) find(1, min(part(top_p, all_low), all_low ? all_low - 1 : 0ull), min(part(top_p, all_up), all_up - 1));
     __syncthreads();
     SfRange range[4];
 #pragma unroll
     for (int r = 0; r < 4; ++r) range[r] = SfRange{1, 0};
-    // (no border that matters lies in the last step, whose keys weigh nothing: its keys are not asked for)
+    // (no border that matters lies in the last step: its keys are not asked for)
     int cut = SF_STEPS - 2;
-    float kept_low = all_low, kept_up = all_up;
+    unsigned long long kept_low = all_low, kept_up = all_up;
     if (k_on) { range[SF_TOP_K] = SfRange{k_step, k_step}; cut = min(cut, k_step); }
     if (p_on) {
       const int p1 = s.steps[2] < 0 ? cut : min(cut, s.steps[2]), p0 = s.steps[1] < 0 ? p1 : min(p1, s.steps[1]);
       range[SF_TOP_P] = SfRange{p0, p1};
       cut = p1;
-      kept_low = top_p * all_low;
-      kept_up = top_p * all_up + exp2f(-(float)p0 / 32.f);
+      kept_low = part(top_p, all_low);
+      const unsigned long long t = s.table[p0 & 31] >> (p0 >> 5);  // the token that crosses stays
+      kept_up = part(top_p, all_up) + to_scale(t + (t >> 10)) + 1;
     }
     if (m_on && (m_step <= cut || !(k_on || p_on))) {
       if (m_step < (p_on ? range[SF_TOP_P].first : k_step) || !(k_on || p_on)) {  // what lies behind does not matter
@@ -461,75 +511,96 @@ struct SfRow {
         kept_low = s.got[2];
         kept_up = s.got[3];
       } else {
-        kept_low = fminf(kept_low, s.got[2]);
-        kept_up = fminf(kept_up, s.got[3]);
+        kept_low = min(kept_low, s.got[2]);
+        kept_up = min(kept_up, s.got[3]);
       }
       range[SF_MIN_P] = SfRange{m_step, m_step};
       cut = min(cut, m_step);
     }
-    find(3, u * kept_low * (1.f - slack), true);
-    find(4, u * kept_up * (1.f + slack), false);
+    // (the weights of single keys are rounded once more than those of steps: a draw that lies next to a border of steps is looked for on both sides)
+    const unsigned long long r0 = part(u, kept_low), r1 = part(u, kept_up);
+    find(3, r0 - (r0 >> 30), r1 + (r1 >> 30));
     __syncthreads();
     const int d1 = s.steps[4] < 0 ? cut : min(cut, s.steps[4]), d0 = s.steps[3] < 0 ? d1 : min(d1, s.steps[3]);
     range[SF_DRAW] = SfRange{d0, d1};
     unsigned wanted = 0;
 #pragma unroll
     for (int e = 0; e < EACH; ++e) {
+      const int n = n0 + e;
       bool in = false;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) in |= n0 + e >= range[r].first && n0 + e <= range[r].last;
-      wanted += in && n0 + e != SF_STEPS - 1 ? c[e] : 0u;
+      for (int r = 0; r < 4; ++r) {
+        in |= n >= range[r].first && n <= range[r].last;
+        if (n == range[r].first) s.over[0][r] = e ? lo[e - 1] : ls_before;  // (with top-k the blocks write what they find)
+      }
+      wanted += in && n != SF_STEPS - 1 ? c[e] : 0u;
     }
     wanted = __reduce_add_sync(0xffffffffu, wanted);
-    if (lane == 0) s.warp[warp] = wanted;
-    __syncthreads();
+    if (lane == 0 && wanted) atomicAdd((unsigned*)&s.steps[7], wanted);  // (from -1 on)
     if (tid == 0) {
-      wanted = 0;
-#pragma unroll
-      for (int w = 0; w < NW; ++w) wanted += (unsigned)s.warp[w];
 #pragma unroll
       for (int r = 0; r < 4; ++r) s.plan.range[r] = range[r];
-      s.plan.by_bits = wanted > SF_LIST;
       s.listed = 0;
+      s.all_mass = all_low;
     }
+    if (tid >= 4 && tid < 4 * (int)blocks) s.over[tid >> 2][tid & 3] = 0;
+    __syncthreads();
+    if (tid == 0) s.plan.by_bits = s.steps[7] + 1 > SF_LIST;
     __syncthreads();
     constexpr int WORDS = sizeof(SfPlan) / 8;
     if (tid < WORDS * (int)blocks && tid >= WORDS) sf_store(reinterpret_cast<unsigned long long*>(&s.plan) + tid % WORDS, tid / WORDS,
                                                             reinterpret_cast<const unsigned long long*>(&s.plan)[tid % WORDS]);
   }
 
-  // All blocks: the keys of the ranges to the first block, and the weights above each range.
-  __device__ void hand_over() {
-    unsigned long long over[4] = {0, 0, 0, 0};
-    int first[4], last[4], end = 0;
+  // All blocks: the keys of the ranges to the first block; with top-k also the weights above each range (few keys lie there).
+  __device__ void hand_over(bool numbers) {
+    int first[4], last[4], begin = SF_STEPS, end = 0;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       first[r] = s.plan.range[r].first;
       last[r] = s.plan.range[r].last;
-      if (last[r] < first[r]) first[r] = last[r] = -1;
-      end = max(end, last[r]);
-      last[r] = min(last[r], SF_STEPS - 2);
+      if (last[r] < first[r]) {
+        first[r] = last[r] = -1;
+      } else {
+        begin = min(begin, first[r]);
+        end = max(end, last[r]);
+        last[r] = min(last[r], SF_STEPS - 2);
+      }
     }
+    unsigned long long over[4] = {0, 0, 0, 0};
     const int offset = (int)rank * a.per;
-    each_key([&](unsigned k, int i) {
-      float rest;
-      const int n = step_of(k, &rest);
-      if (n > end) return;
-      bool in = false;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) in |= n >= first[r] && n <= last[r];
-      if (n < max(max(first[0], first[1]), max(first[2], first[3]))) {
+    const auto give = [&](unsigned k, int i) {
+      unsigned at;
+      asm volatile("atom.relaxed.cluster.shared::cluster.add.u32 %0, [%1], 1;" : "=r"(at) : "r"(sf_remote(&s.listed, 0)) : "memory");
+      if (at < SF_LIST) sf_store(&s.list[at], 0, ((unsigned long long)~k << 32) | (unsigned)(offset + i));
+    };
+    // the keys of steps begin .. end lie between about these (the steps are looked at again)
+    const float y0 = topf - (float)(end + 2) / (32.f * c_hi), y1 = topf - (float)(begin - 1) / (32.f * c_hi);
+    const unsigned least = max(sf_key(y0 - fminf(fabsf(y0), 1e38f) * 1e-6f), 1u), most = sf_key(y1 + fminf(fabsf(y1), 1e38f) * 1e-6f);
+    if (numbers) {
+      each_key(least, [&](unsigned k, int i) {
+        float rest;
+        const int n = step_of(k, &rest);
+        bool in = false;
         const unsigned long long w = weight_at(n, short_of(rest));
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
+        for (int r = 0; r < 4; ++r) {
+          in |= n >= first[r] && n <= last[r];
           if (n < first[r]) add(over[r], w);
-      }
-      if (in) {
-        unsigned at;
-        asm volatile("atom.relaxed.cluster.shared::cluster.add.u32 %0, [%1], 1;" : "=r"(at) : "r"(sf_remote(&s.listed, 0)) : "memory");
-        if (at < SF_LIST) sf_store(&s.list[at], 0, ((unsigned long long)~k << 32) | (unsigned)(offset + i));
-      }
-    });
+        }
+        if (in) give(k, i);
+      });
+    } else {
+      each_key(least, [&](unsigned k, int i) {
+        if (k > most) return;
+        const int n = step_of(k);
+        bool in = false;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) in |= n >= first[r] && n <= last[r];
+        if (in) give(k, i);
+      });
+      return;
+    }
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       over[r] = added(over[r]);
@@ -541,7 +612,7 @@ struct SfRow {
     __syncthreads();
     if (threadIdx.x < 4) {
       unsigned long long sum = 0;
-#pragma unroll
+#pragma unroll 4
       for (int w = 0; w < SF_THREADS / 32; ++w) sum += s.warp4[w][threadIdx.x];
       sf_store(&s.over[rank][threadIdx.x], 0, sum);
     }
@@ -549,7 +620,7 @@ struct SfRow {
 
   // First block: sort what was handed over and walk the borders; the token.  GROUP: the threads that do it, one warp or all of the block.
   template <int GROUP>
-  __device__ void decide(bool k_on, bool p_on, float top_p, bool m_on, float u, unsigned long long all_mass, int* out) {
+  __device__ void decide(float top_p, float u, int* out) {
     const auto sync = [] {
       if (GROUP == 32) __syncwarp();
       else __syncthreads();
@@ -569,22 +640,20 @@ struct SfRow {
         sync();
       }
     }
-    // running sums: thread t has entries t * each and on
-    constexpr int MOST = (GROUP == 32 ? SF_FEW : SF_LIST) / GROUP;
-    const int each = (m + GROUP - 1) / GROUP, i0 = tid * each;
-    unsigned long long w[MOST], sum = 0;
-    int step[MOST];
-#pragma unroll
-    for (int e = 0; e < MOST; ++e) {
-      w[e] = 0;
-      step[e] = SF_STEPS;
-      if (e < each && i0 + e < m) {
+    // running sums: thread t has entries t * each and on; f(entry, its step, the running sum in front of it, with it)
+    const int each = (m + GROUP - 1) / GROUP, i0 = min(tid * each, m), i1 = min(i0 + each, m);
+    auto walk = [&](unsigned long long run, auto f) {
+#pragma unroll 1
+      for (int i = i0; i < i1; ++i) {
         float rest;
-        step[e] = step_of(~(unsigned)(s.list[i0 + e] >> 32), &rest);
-        w[e] = to_scale(weight_at(step[e], short_of(rest)));
+        const int n = step_of(~(unsigned)(s.list[i] >> 32), &rest);
+        const unsigned long long next = run + to_scale(weight_at(n, short_of(rest)));
+        f(i, n, run, next);
+        run = next;
       }
-      sum += w[e];
-    }
+      return run;
+    };
+    const unsigned long long sum = walk(0ull, [](int, int, unsigned long long, unsigned long long) {});
     const int lane = tid & 31, warp = tid >> 5;
     unsigned long long run0 = sum;
 #pragma unroll
@@ -603,55 +672,38 @@ struct SfRow {
       }
     }
     run0 -= sum;
-    unsigned long long over[4];
+    unsigned long long over[4], part4 = 0;  // lane: block lane / 4 and 8 more, range lane % 4
+    for (unsigned b = lane >> 2; b < blocks; b += 8) part4 += s.over[b][lane & 3];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      over[r] = 0;
+    for (int o = 4; o < 32; o <<= 1) part4 += __shfl_xor_sync(0xffffffffu, part4, o);
 #pragma unroll
-      for (unsigned b = 0; b < SF_MAX_CLUSTER; ++b) over[r] += b < blocks ? s.over[b][r] : 0ull;
-    }
+    for (int r = 0; r < 4; ++r) over[r] = __shfl_sync(0xffffffffu, part4, r);
     SfRange range[4];
 #pragma unroll
     for (int r = 0; r < 4; ++r) range[r] = s.plan.range[r];
     const auto is_in = [&](int r) { return range[r].last >= range[r].first; };
     if (tid < 4) { s.base[tid] = total; s.at[tid] = m; }
-    if (tid == 0) { s.sum[0] = k_on && is_in(SF_TOP_K) ? over[SF_TOP_K] : all_mass; s.sum[1] = is_in(SF_MIN_P) ? over[SF_MIN_P] : ~0ull; }
+    if (tid == 0) { s.sum[0] = is_in(SF_TOP_K) ? over[SF_TOP_K] : s.all_mass; s.sum[1] = is_in(SF_MIN_P) ? over[SF_MIN_P] : ~0ull; }
     sync();
     // where each range begins, and the running sum in front of it
-    {
-      unsigned long long run = run0;
-      int prev = i0 > 0 && i0 <= m ? step_of(~(unsigned)(s.list[i0 - 1] >> 32)) : -1;
+    int prev = i0 > 0 ? step_of(~(unsigned)(s.list[i0 - 1] >> 32)) : -1;
+    walk(run0, [&](int i, int n, unsigned long long before, unsigned long long) {
 #pragma unroll
-      for (int e = 0; e < MOST; ++e) {
-        if (e < each && i0 + e < m) {
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (step[e] >= range[r].first && prev < range[r].first) { s.base[r] = run; s.at[r] = i0 + e; }
-          prev = step[e];
-        }
-        run += w[e];
-      }
-    }
+      for (int r = 0; r < 4; ++r)
+        if (n >= range[r].first && prev < range[r].first) { s.base[r] = before; s.at[r] = i; }
+      prev = n;
+    });
     sync();
-    // f(entry, running sum in front of it, with it)
-    auto walk = [&](auto f) {
-      unsigned long long run = run0;
-#pragma unroll
-      for (int e = 0; e < MOST; ++e) {
-        if (e < each && i0 + e < m) f(i0 + e, run, run + w[e]);
-        run += w[e];
-      }
-    };
     if (is_in(SF_TOP_K)) {  // (in the last step, whose keys are not here, all that weighs lies above)
       const int at = s.at[SF_TOP_K] + (int)s.plan.rest - 1;
-      if (range[SF_TOP_K].first != SF_STEPS - 1) walk([&](int i, unsigned long long, unsigned long long run) {
+      if (range[SF_TOP_K].first != SF_STEPS - 1) walk(run0, [&](int i, int, unsigned long long, unsigned long long run) {
         if (i == at) s.sum[0] = over[SF_TOP_K] + run - s.base[SF_TOP_K];
       });
     }
     if (is_in(SF_MIN_P)) {  // the last entry that stays; without one nothing of the range does
       const int at0 = s.at[SF_MIN_P];
       const unsigned least = s.plan.least;
-      walk([&](int i, unsigned long long, unsigned long long run) {
+      walk(run0, [&](int i, int, unsigned long long, unsigned long long run) {
         if (i >= at0 && ~(unsigned)(s.list[i] >> 32) >= least && (i + 1 >= m || ~(unsigned)(s.list[i + 1] >> 32) < least))
           s.sum[1] = over[SF_MIN_P] + run - s.base[SF_MIN_P];
       });
@@ -663,8 +715,11 @@ struct SfRow {
       const int at0 = s.at[SF_TOP_P];
       const unsigned long long off = over[SF_TOP_P] - s.base[SF_TOP_P];
       sync();
-      walk([&](int i, unsigned long long before, unsigned long long run) {
-        if (i >= at0 && before + off <= thr && run + off > thr) s.sum[0] = run + off;
+      if (tid == 0) s.sum[0] = over[SF_TOP_P];
+      sync();
+      // the last whose predecessors do not exceed it
+      walk(run0, [&](int i, int n, unsigned long long before, unsigned long long run) {
+        if (i >= at0 && n <= range[SF_TOP_P].last && before + off <= thr) atomicMax(&s.sum[0], run + off);
       });
       sync();
       kept = s.sum[0];
@@ -674,11 +729,13 @@ struct SfRow {
     const unsigned long long thr = min((unsigned long long)((double)u * (double)kept), kept - 1);
     const int at0 = s.at[SF_DRAW];
     const unsigned long long off = over[SF_DRAW] - s.base[SF_DRAW];
-    if (tid == 0) *out = (int)(unsigned)s.list[min(at0, m - 1)];
+    if (tid == 0) s.at[0] = max(min(at0, m - 1), 0);
     sync();
-    walk([&](int i, unsigned long long before, unsigned long long run) {
-      if (i >= at0 && before + off <= thr && run + off > thr) *out = (int)(unsigned)s.list[i];
+    walk(run0, [&](int i, int n, unsigned long long before, unsigned long long) {
+      if (i >= at0 && n <= range[SF_DRAW].last && before + off <= thr) atomicMax(&s.at[0], i);
     });
+    sync();
+    if (tid == 0) *out = (int)(unsigned)s.list[s.at[0]];
   }
 
   // The index of the j-th (from 0) of the row's numbers with key k, in the block that has it; -1 elsewhere.
@@ -712,34 +769,34 @@ struct SfRow {
 
 // Keys of one block's part of a row into shared memory (RESIDENT); the largest.
 template <typename T, bool RESIDENT>
-__device__ __forceinline__ unsigned sf_read(const T* row, int n, int per, unsigned* keys) {
+__device__ __forceinline__ unsigned sf_read(const T* row, int n, int per, typename SfHeld<T>::Key* keys) {
+  typedef SfHeld<T> Held;
   unsigned high = 0;
   constexpr int V = 16 / (int)sizeof(T);
   int done = 0;
   if ((((uintptr_t)row) & 15) == 0) {
     const int nv = n / V;
-#pragma unroll 4
+#pragma unroll 8
     for (int i = threadIdx.x; i < nv; i += SF_THREADS) {
-      const uint4 raw = reinterpret_cast<const uint4*>(row)[i];
+      const uint4 raw = __ldcs(reinterpret_cast<const uint4*>(row) + i);
       const T* x = reinterpret_cast<const T*>(&raw);
-      unsigned k[V];
+      uint4 packed;
+      typename Held::Key* h = reinterpret_cast<typename Held::Key*>(&packed);
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        k[e] = sf_key(to_f32<T>(x[e]));
-        high = max(high, k[e]);
+        const unsigned k = sf_key(to_f32<T>(x[e]));
+        high = max(high, k);
+        h[e] = Held::pack(k);
       }
-      if (RESIDENT) {
-#pragma unroll
-        for (int e = 0; e < V; e += 4) *reinterpret_cast<uint4*>(keys + i * V + e) = make_uint4(k[e], k[e + 1], k[e + 2], k[e + 3]);
-      }
+      if (RESIDENT) reinterpret_cast<uint4*>(keys)[i] = packed;
     }
     done = nv * V;
   }
-#pragma unroll 4
+#pragma unroll 8
   for (int i = done + threadIdx.x; i < (RESIDENT ? per : n); i += SF_THREADS) {
     const unsigned k = i < n ? sf_key(to_f32<T>(row[i])) : 0u;
     high = max(high, k);
-    if (RESIDENT) keys[i] = k;
+    if (RESIDENT) keys[i] = Held::pack(k);
   }
   return high;
 }
@@ -749,25 +806,27 @@ __global__ void __launch_bounds__(SF_THREADS, 2) sample_filtered_kernel(const __
   pdl_launch_dependents();
   extern __shared__ __align__(16) unsigned char smem_raw[];
   SfShared& s = *reinterpret_cast<SfShared*>(smem_raw);
-  unsigned* keys = reinterpret_cast<unsigned*>(smem_raw + ((sizeof(SfShared) + 15) & ~(size_t)15));
+  typename SfHeld<T>::Key* keys = reinterpret_cast<typename SfHeld<T>::Key*>(smem_raw + ((sizeof(SfShared) + 15) & ~(size_t)15));
   const unsigned rank = sf_rank(), blocks = sf_size();
   const int r = blockIdx.x / blocks;
   const int first = min(a.vocab, (int)rank * a.per);
   SfRow<T, RESIDENT> row{a, s, keys, (const T*)a.logits + (size_t)r * a.ld + first, min(a.vocab, first + a.per) - first, rank, blocks};
-  sf_arrive();
-  for (int b = threadIdx.x; b < SF_STEPS; b += SF_THREADS) s.count[b] = s.shy[b] = 0;
+  if (blocks > 1) sf_arrive();
+  for (int b = threadIdx.x; b < SF_STEPS; b += SF_THREADS) s.one[b] = s.two[b] = 0;
   if (threadIdx.x < 32) {
-    const double x = exp2(-(double)threadIdx.x / 32.0);
-    s.table[threadIdx.x] = (unsigned long long)__double2ll_rn(ldexp(x, SF_POINT));
-    s.small_table[threadIdx.x] = __double2int_rn(ldexp(x, 30));
+    const unsigned long long x = a.table[threadIdx.x];
+    s.table[threadIdx.x] = x;
+    s.small_table[threadIdx.x] = (int)((x + (1ull << (SF_POINT - 31))) >> (SF_POINT - 30));
   }
+  if (threadIdx.x == 0) s.high = 0;
   pdl_wait();
   const float temperature = a.temperatures ? a.temperatures[r] : a.temperature;
   const float top_p = a.top_ps ? a.top_ps[r] : a.top_p, asked = a.min_ps ? a.min_ps[r] : a.min_p;
   const float min_p = asked > 0.f ? fminf(asked, 1.f) : 0.f;  // the most probable token always stays
   const int top_k = a.top_ks ? a.top_ks[r] : a.top_k;
   unsigned high = sf_read<T, RESIDENT>(row.row, row.n, a.per, keys);
-  sf_wait();  // every block of the cluster runs: its shared memory may be written
+  if (blocks > 1) sf_wait();
+  else __syncthreads();  // every block of the cluster runs: its shared memory may be written
   // the random number, drawn once for the whole cluster
   if (rank == 0 && threadIdx.x == 0) {
     float u;
@@ -782,11 +841,10 @@ __global__ void __launch_bounds__(SF_THREADS, 2) sample_filtered_kernel(const __
     }
     for (unsigned b = 0; b < blocks; ++b) sf_store(&s.found[0], b, __float_as_uint(u));
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) high = max(high, __shfl_xor_sync(0xffffffffu, high, o));
-  if ((threadIdx.x & 31) == 0) s.warp[threadIdx.x >> 5] = high;
+  high = __reduce_max_sync(0xffffffffu, high);
+  if ((threadIdx.x & 31) == 0) atomicMax(&s.high, high);
   __syncthreads();
-  for (int w = 0; w < SF_THREADS / 32; ++w) high = max(high, (unsigned)s.warp[w]);
+  high = s.high;
   high = row.exchange_max(high);
   const float asked_u = __uint_as_float((unsigned)s.found[0]), u = asked_u > 0.f ? asked_u : 0.f;
   unsigned chosen = high;
@@ -800,34 +858,25 @@ __global__ void __launch_bounds__(SF_THREADS, 2) sample_filtered_kernel(const __
     row.c_hi = (float)c;
     row.c_lo = (float)(c - (double)row.c_hi);
     const bool k_on = top_k > 0 && top_k < a.vocab, p_on = top_p > 0.f && top_p < 1.f, m_on = min_p > 0.f;
-    // (a temperature near the ends of float's range; so many keys that a step's sums could overflow)
-    bool by_bits = row.infinite || !(c > 1e-30 && c < 1e30) || a.per > SF_COUNTED;
+      bool by_bits = row.infinite || !(c > 1e-30 && c < 1e30) || a.per > SF_COUNTED;
     if (!by_bits) {
-      // Sums as well, unless top-k leaves few tokens: then the bounds that counts alone give are close enough to find borders among those, and the sum of
-      // all weights is not asked for (one row of 32,000 and k = 50: 1.3 us for the counts, 2.0 with sums).
-      const bool sums = !k_on || top_k > SF_LIST / 2;
-      const unsigned long long sum = row.block_sum64(sums ? row.template count_steps<true>() : row.template count_steps<false>());
-      if (threadIdx.x == 0) sf_store(&s.mass[rank], 0, sum);
-      sf_sync();
-      unsigned long long all_mass = 0;
-      if (rank == 0) {
-        for (unsigned b = 0; b < blocks; ++b) all_mass += s.mass[b];
-        row.make_plan(sums, k_on, (unsigned)top_k, p_on, top_p, m_on, min_p, temperature, u, all_mass);
-      }
-      sf_sync();
+      row.count_steps(k_on);
+      sf_sync(blocks);
+      if (rank == 0) row.make_plan(k_on, (unsigned)top_k, p_on, top_p, m_on, min_p, temperature, u);
+      sf_sync(blocks);
       by_bits = s.plan.by_bits;
       if (!by_bits) {
-        row.hand_over();
-        sf_sync();  // the last time that another block is needed
+        row.hand_over(k_on);
+        sf_sync(blocks);  // the last time that another block is needed
         if (rank == 0) {
-          if (s.listed > SF_FEW) row.template decide<SF_THREADS>(k_on, p_on, top_p, m_on, u, all_mass, a.out + r);
-          else if (threadIdx.x < 32) row.template decide<32>(k_on, p_on, top_p, m_on, u, all_mass, a.out + r);
+          if (s.listed > SF_FEW) row.template decide<SF_THREADS>(top_p, u, a.out + r);
+          else if (threadIdx.x < 32) row.template decide<32>(top_p, u, a.out + r);
         }
         return;
       }
     }
     unsigned long long valid = 0, before;
-    row.each_key([&](unsigned, int) { ++valid; });
+    row.each_key(1u, [&](unsigned, int) { ++valid; });
     valid = row.exchange_sum(row.block_sum64(valid), &before);
     // kept: all larger than `cut`, and `ties` of those equal to it
     unsigned cut = 1u;
@@ -839,7 +888,7 @@ __global__ void __launch_bounds__(SF_THREADS, 2) sample_filtered_kernel(const __
     }
     auto kept_mass = [&](float least) {
       unsigned long long m = 0;
-      row.each_key([&](unsigned k, int) {
+      row.each_key(1u, [&](unsigned k, int) {
         if (k > cut) {
           const double w = row.weight(k);
           if (w >= (double)least) m += row.fixed(w);
@@ -874,20 +923,38 @@ __global__ void __launch_bounds__(SF_THREADS, 2) sample_filtered_kernel(const __
     const int at = row.nth(chosen, tie);
     if (at >= 0) a.out[r] = first + at;
   }
-  sf_sync();  // no block leaves while another may still read from it or write to it
+  sf_sync(blocks);  // no block leaves while another may still read from it or write to it
 }
 
+static int SF_FORCE = 0, SF_RES = -1;
+extern "C" void sf_force(int b, int r) { SF_FORCE = b; SF_RES = r; }
 template <typename T, bool RESIDENT>
 static int sf_launch(const SfArgs& a, int n_rows, int blocks, size_t smem, cudaStream_t stream) {
   static BnGrant grant;
-  const cudaError_t g = grant.ask((const void*)sample_filtered_kernel<T, RESIDENT>, smem, 0);
-  if (g != cudaSuccess) return BN_ERR_LAUNCH + (int)g;
-  const cudaError_t e = bn_launch_cluster(sample_filtered_kernel<T, RESIDENT>, dim3((unsigned)(n_rows * blocks)), dim3(SF_THREADS), smem, stream,
-                                          dim3((unsigned)blocks, 1, 1), a);
+  cudaError_t e = grant.ask((const void*)sample_filtered_kernel<T, RESIDENT>, smem, 0);
+  if (e != cudaSuccess) return BN_ERR_LAUNCH + (int)e;
+  e = bn_launch_cluster(sample_filtered_kernel<T, RESIDENT>, dim3((unsigned)(n_rows * blocks)), dim3(SF_THREADS), smem, stream,
+                        dim3((unsigned)blocks, 1, 1), a);
   return e == cudaSuccess ? BN_OK : BN_ERR_LAUNCH + (int)e;
 }
-
-#define SF_KEYS_MAX 48000  // keys that a block holds beside its counts and its list (and fewer than 2^7 per thread)
+template <typename T>
+static int sf_run(SfArgs& a, int n_rows, cudaStream_t stream) {
+  typedef typename SfHeld<T>::Key Key;
+  int device = 0, sms = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
+  if (e != cudaSuccess) return BN_ERR_LAUNCH + (int)e;
+  int blocks = SF_MAX_CLUSTER;
+  while (blocks > 1 && a.vocab <= blocks / 2 * 4096) blocks /= 2;
+  while (blocks > 1 && (long long)n_rows * blocks > 2 * sms && (a.vocab + blocks / 2 - 1) / (blocks / 2) <= SF_COUNTED - 8) blocks /= 2;
+  if (SF_FORCE) blocks = SF_FORCE;
+  a.per = (((a.vocab + blocks - 1) / blocks) + 7) & ~7;
+  const size_t base = (sizeof(SfShared) + 15) & ~(size_t)15, held = (((size_t)a.per * sizeof(Key)) + 15) & ~(size_t)15;
+  const size_t room = (long long)n_rows * blocks <= sms ? 220 * 1024 : 112 * 1024;
+  bool resident = base + held <= room && a.per <= 128 * SF_THREADS;
+  if (SF_RES >= 0) resident = SF_RES && base + held <= 220 * 1024 && a.per <= 128 * SF_THREADS;
+  return resident ? sf_launch<T, true>(a, n_rows, blocks, base + held, stream) : sf_launch<T, false>(a, n_rows, blocks, base, stream);
+}
 
 // logits [n_rows, vocab] of `dtype`, rows ld numbers apart.  The four parameters hold for all rows where their array is null.  u: a number in
 // [0, 1) per row, or null: drawn from the generator rng[index ? index[r] : r], which is advanced.  out: the tokens, -1 for a row
@@ -906,11 +973,6 @@ extern "C" int bn_sample_filtered(const void* logits, int dtype, long long ld, i
   int bits = 0;
   while ((1ll << bits) < vocab) ++bits;
   a.scale_bits = 62 - bits < SF_POINT ? 62 - bits : SF_POINT;  // the sum of all weights stays below 2^62
-  int blocks = SF_MAX_CLUSTER;
-  while (blocks > 1 && vocab <= (blocks / 2) * 2048) blocks /= 2;
-  a.per = (((vocab + blocks - 1) / blocks) + 7) & ~7;
-  const bool resident = a.per <= SF_KEYS_MAX;
-  const size_t smem = ((sizeof(SfShared) + 15) & ~(size_t)15) + (resident ? (size_t)a.per * 4 : 0);
-  if (dtype == BN_F32) return resident ? sf_launch<float, true>(a, n_rows, blocks, smem, stream) : sf_launch<float, false>(a, n_rows, blocks, smem, stream);
-  return resident ? sf_launch<__nv_bfloat16, true>(a, n_rows, blocks, smem, stream) : sf_launch<__nv_bfloat16, false>(a, n_rows, blocks, smem, stream);
+  for (int j = 0; j < 32; ++j) a.table[j] = (unsigned long long)llround(ldexp(exp2(-j / 32.0), SF_POINT));
+  return dtype == BN_F32 ? sf_run<float>(a, n_rows, stream) : sf_run<__nv_bfloat16>(a, n_rows, stream);
 }
