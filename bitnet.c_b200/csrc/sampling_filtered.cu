@@ -6,7 +6,8 @@
 // is sorted: every border is "the first whose running sum (of ones, or of weights) exceeds a number", found by the bits of the logits.
 //
 // A cluster of blocks holds a row in its shared memory as ordered 32-bit keys, so that memory is read once however many passes
-// follow.  One pass adds up the keys' weights (with top-k: counts the keys) in steps of 2^(1/32) of the weight; from these sums the first block of the
+// follow.  One pass adds up the keys' weights (with top-k: counts the keys) in steps of 2^(1/32) of the weight (finer ones
+// where the row's weights lie closer together: fewer keys meet in a step); from these sums the first block of the
 // cluster knows in which step each border lies.  A second pass hands the keys of those steps to it; it sorts them (some tens of keys, of a flat row
 // hundreds) and decides.  Where too many keys lie together (ties by the thousand, a huge temperature), borders are found by the bits of the keys
 // instead, 11, 11 and 10 at a time, the weights of the keys that agree with the bits found so far added into a histogram.
@@ -144,7 +145,7 @@ struct SfShared {
   unsigned long long all_mass;                  // first block: of all keys (not with top-k)
   SfPlan plan;
   unsigned listed;                              // first block: keys in the list
-  unsigned high;                                // the largest key of this block
+  unsigned high, low;                           // the largest key of this block, the largest of 0 - key
   unsigned long long table[32];                 // 2^-(j/32), 1 = 2^SF_POINT
   int small_table[32];                          // the same, 1 = 2^30
   unsigned long long warp4[SF_THREADS / 32][4];
@@ -167,6 +168,8 @@ struct SfRow {
   double top, per_t;     // the largest logit, 1 / temperature
   bool infinite;         // the largest logit is +inf: those share everything
   float topf, c_hi, c_lo;  // the largest logit, log2(e) / temperature in two floats
+  int fine;                // steps are 2^-fine of a 32nd of an octave: as fine as lets the smallest weight have a step in front of the last
+  float steps;             // to an octave
 
   __device__ __forceinline__ unsigned key(int i) const { return RESIDENT ? Held::key(keys[i]) : sf_key(to_f32<T>(row[i])); }
   __device__ __forceinline__ double weight(unsigned k) const {
@@ -199,13 +202,16 @@ struct SfRow {
     *before = low;
     return all;
   }
-  __device__ unsigned exchange_max(unsigned v) {
+  // The largest of every block's `high` and `low`.
+  __device__ void exchange_max(unsigned* high, unsigned* low) {
     const int t = turn++ & 1;
-    if (threadIdx.x < blocks) sf_store(&s.part[t][rank], threadIdx.x, v);
+    if (threadIdx.x < blocks) sf_store(&s.part[t][rank], threadIdx.x, ((unsigned long long)*high << 32) | *low);
     sf_sync(blocks);
-    unsigned m = 0;
-    for (unsigned r = 0; r < blocks; ++r) m = max(m, (unsigned)s.part[t][r]);
-    return m;
+    for (unsigned r = 0; r < blocks; ++r) {
+      const unsigned long long x = s.part[t][r];
+      *high = max(*high, (unsigned)(x >> 32));
+      *low = max(*low, (unsigned)x);
+    }
   }
 
   // The first key, from the largest on, where the running sum of the weights (ones, if ONES) exceeds thr; *above: the sum over larger keys.
@@ -283,26 +289,30 @@ struct SfRow {
   }
 
   // ---- by steps of weight ----
-  // The step of a key (falling keys, rising steps) and what is behind it: y = step / 32 + rest.
+  // The step of a key (falling keys, rising steps), and what its y is behind the 32nd of an octave that the step lies in.
   __device__ __forceinline__ int step_of(unsigned k, float* rest) const {
     const float v = sf_value(k), d = topf - v, bb = d - topf, dl = (topf - (d - bb)) - (v + bb);
     const float y = d * c_hi, yl = fmaf(d, c_hi, -y) + fmaf(d, c_lo, dl * c_hi);
-    const int n = min(__float2int_rd(y * 32.f), SF_STEPS - 1);
-    *rest = fmaf((float)n, -1.f / 32.f, y) + yl;
+    const int n = min(__float2int_rd(y * steps), SF_STEPS - 1);
+    *rest = fmaf((float)(n >> fine), -1.f / 32.f, y) + yl;
     return n;
   }
-  __device__ __forceinline__ int step_of(unsigned k) const { return min(__float2int_rd((topf - sf_value(k)) * c_hi * 32.f), SF_STEPS - 1); }
+  __device__ __forceinline__ int step_of(unsigned k) const { return min(__float2int_rd((topf - sf_value(k)) * c_hi * steps), SF_STEPS - 1); }
   // 1 - 2^-rest
   static __device__ __forceinline__ float short_of(float rest) {
     const float g = rest * 0.69314718f;
     return g * (1.f - g * (0.5f - g * (0.16666667f - g * 0.041666668f)));
   }
+  // The largest weight in a step's 32nd of an octave.
+  __device__ __forceinline__ unsigned long long most_at(int n) const { return s.table[(n >> fine) & 31] >> (n >> fine >> 5); }
   // 2^-y, 1 = 2^SF_POINT, to 2^-30 of itself
   __device__ __forceinline__ unsigned long long weight_at(int n, float e) const {
-    const int whole = __float2int_rn(e * 4294967296.f);
-    const unsigned long long w = s.table[n & 31] - (((long long)s.small_table[n & 31] * whole) >> (62 - SF_POINT));
-    return n == SF_STEPS - 1 ? 0ull : w >> (n >> 5);
+    const int whole = __float2int_rn(e * 4294967296.f), at = n >> fine;
+    const unsigned long long w = s.table[at & 31] - (((long long)s.small_table[at & 31] * whole) >> (62 - SF_POINT));
+    return nothing(n) ? 0ull : w >> (at >> 5);
   }
+  // Whether a step's keys weigh nothing: the last one's, where steps are as wide as they get (else no key lies there).
+  __device__ __forceinline__ bool nothing(int n) const { return n == SF_STEPS - 1; }
   __device__ __forceinline__ unsigned long long to_scale(unsigned long long w) const {  // from 2^SF_POINT to 2^scale_bits
     const int down = SF_POINT - a.scale_bits;
     return down ? (w + (1ull << (down - 1))) >> down : w;
@@ -403,10 +413,10 @@ struct SfRow {
 #pragma unroll
     for (int e = 0; e < EACH; ++e) {
       const int n = n0 + e;
-      const unsigned long long t = s.table[n & 31] >> (n >> 5);  // the step's largest weight
+      const unsigned long long t = most_at(n);
       if (k_on) {
         c[e] = (unsigned)(one[e] + two[e]);
-        const unsigned long long t1 = s.table[(n + 1) & 31] >> ((n + 1) >> 5);
+        const unsigned long long t1 = most_at(n + (1 << fine));
         up[e] = c[e] * (to_scale(t + (t >> 10)) + 1);
         lo[e] = c[e] * to_scale(t1 - (t1 >> 10));
       } else {
@@ -502,7 +512,7 @@ struct SfRow {
       range[SF_TOP_P] = SfRange{p0, p1};
       cut = p1;
       kept_low = part(top_p, all_low);
-      const unsigned long long t = s.table[p0 & 31] >> (p0 >> 5);  // the token that crosses stays
+      const unsigned long long t = most_at(p0);  // the token that crosses stays
       kept_up = part(top_p, all_up) + to_scale(t + (t >> 10)) + 1;
     }
     if (m_on && (m_step <= cut || !(k_on || p_on))) {
@@ -569,13 +579,15 @@ struct SfRow {
     }
     unsigned long long over[4] = {0, 0, 0, 0};
     const int offset = (int)rank * a.per;
-    const auto give = [&](unsigned k, int i) {
-      unsigned at;
-      asm volatile("atom.relaxed.cluster.shared::cluster.add.u32 %0, [%1], 1;" : "=r"(at) : "r"(sf_remote(&s.listed, 0)) : "memory");
+    const auto give = [&](unsigned k, int i) {  // (lanes that come here together take their places with one atomic)
+      const unsigned with = __activemask(), lead = __ffs(with) - 1, lane = threadIdx.x & 31;
+      unsigned at = 0;
+      if (lane == lead) asm volatile("atom.relaxed.cluster.shared::cluster.add.u32 %0, [%1], %2;" : "=r"(at) : "r"(sf_remote(&s.listed, 0)), "r"(__popc(with)) : "memory");
+      at = __shfl_sync(with, at, lead) + __popc(with & ((1u << lane) - 1));
       if (at < SF_LIST) sf_store(&s.list[at], 0, ((unsigned long long)~k << 32) | (unsigned)(offset + i));
     };
     // the keys of steps begin .. end lie between about these (the steps are looked at again)
-    const float y0 = topf - (float)(end + 2) / (32.f * c_hi), y1 = topf - (float)(begin - 1) / (32.f * c_hi);
+    const float y0 = topf - (float)(end + 2) / (steps * c_hi), y1 = topf - (float)(begin - 1) / (steps * c_hi);
     const unsigned least = max(sf_key(y0 - fminf(fabsf(y0), 1e38f) * 1e-6f), 1u), most = sf_key(y1 + fminf(fabsf(y1), 1e38f) * 1e-6f);
     if (numbers) {
       each_key(least, [&](unsigned k, int i) {
@@ -767,11 +779,11 @@ struct SfRow {
   }
 };
 
-// Keys of one block's part of a row into shared memory (RESIDENT); the largest.
+// Keys of one block's part of a row into shared memory (RESIDENT); the largest, and the smallest above -inf.
 template <typename T, bool RESIDENT>
-__device__ __forceinline__ unsigned sf_read(const T* row, int n, int per, typename SfHeld<T>::Key* keys) {
+__device__ __forceinline__ unsigned sf_read(const T* row, int n, int per, typename SfHeld<T>::Key* keys, unsigned* smallest) {
   typedef SfHeld<T> Held;
-  unsigned high = 0;
+  unsigned high = 0, low = 0;  // (low: of 0 - key, which is 0 for -inf)
   constexpr int V = 16 / (int)sizeof(T);
   int done = 0;
   if ((((uintptr_t)row) & 15) == 0) {
@@ -786,6 +798,7 @@ __device__ __forceinline__ unsigned sf_read(const T* row, int n, int per, typena
       for (int e = 0; e < V; ++e) {
         const unsigned k = sf_key(to_f32<T>(x[e]));
         high = max(high, k);
+        low = max(low, 0u - k);
         h[e] = Held::pack(k);
       }
       if (RESIDENT) reinterpret_cast<uint4*>(keys)[i] = packed;
@@ -796,8 +809,10 @@ __device__ __forceinline__ unsigned sf_read(const T* row, int n, int per, typena
   for (int i = done + threadIdx.x; i < (RESIDENT ? per : n); i += SF_THREADS) {
     const unsigned k = i < n ? sf_key(to_f32<T>(row[i])) : 0u;
     high = max(high, k);
+    low = max(low, 0u - k);
     if (RESIDENT) keys[i] = Held::pack(k);
   }
+  *smallest = low;
   return high;
 }
 
@@ -818,13 +833,13 @@ __global__ void __launch_bounds__(SF_THREADS, 2) sample_filtered_kernel(const __
     s.table[threadIdx.x] = x;
     s.small_table[threadIdx.x] = (int)((x + (1ull << (SF_POINT - 31))) >> (SF_POINT - 30));
   }
-  if (threadIdx.x == 0) s.high = 0;
+  if (threadIdx.x == 0) s.high = s.low = 0;
   pdl_wait();
   const float temperature = a.temperatures ? a.temperatures[r] : a.temperature;
   const float top_p = a.top_ps ? a.top_ps[r] : a.top_p, asked = a.min_ps ? a.min_ps[r] : a.min_p;
   const float min_p = asked > 0.f ? fminf(asked, 1.f) : 0.f;  // the most probable token always stays
   const int top_k = a.top_ks ? a.top_ks[r] : a.top_k;
-  unsigned high = sf_read<T, RESIDENT>(row.row, row.n, a.per, keys);
+  unsigned low, high = sf_read<T, RESIDENT>(row.row, row.n, a.per, keys, &low);
   if (blocks > 1) sf_wait();
   else __syncthreads();  // every block of the cluster runs: its shared memory may be written
   // the random number, drawn once for the whole cluster
@@ -842,10 +857,12 @@ __global__ void __launch_bounds__(SF_THREADS, 2) sample_filtered_kernel(const __
     for (unsigned b = 0; b < blocks; ++b) sf_store(&s.found[0], b, __float_as_uint(u));
   }
   high = __reduce_max_sync(0xffffffffu, high);
-  if ((threadIdx.x & 31) == 0) atomicMax(&s.high, high);
+  low = __reduce_max_sync(0xffffffffu, low);
+  if ((threadIdx.x & 31) == 0) { atomicMax(&s.high, high); atomicMax(&s.low, low); }
   __syncthreads();
   high = s.high;
-  high = row.exchange_max(high);
+  low = s.low;
+  row.exchange_max(&high, &low);
   const float asked_u = __uint_as_float((unsigned)s.found[0]), u = asked_u > 0.f ? asked_u : 0.f;
   unsigned chosen = high;
   unsigned long long tie = 0;
@@ -857,6 +874,10 @@ __global__ void __launch_bounds__(SF_THREADS, 2) sample_filtered_kernel(const __
     const double c = 1.4426950408889634 * row.per_t;
     row.c_hi = (float)c;
     row.c_lo = (float)(c - (double)row.c_hi);
+    const float octaves = (row.topf - sf_value(0u - low)) * row.c_hi;
+    row.fine = 0;
+    while (row.fine < 5 && octaves * (float)(64 << row.fine) < (float)(SF_STEPS - 2)) ++row.fine;
+    row.steps = (float)(32 << row.fine);
     const bool k_on = top_k > 0 && top_k < a.vocab, p_on = top_p > 0.f && top_p < 1.f, m_on = min_p > 0.f;
       bool by_bits = row.infinite || !(c > 1e-30 && c < 1e30) || a.per > SF_COUNTED;
     if (!by_bits) {
