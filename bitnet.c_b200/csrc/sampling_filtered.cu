@@ -17,7 +17,9 @@
 #include "common.cuh"
 #include <math.h>
 
+#ifndef SF_THREADS
 #define SF_THREADS 512
+#endif
 #define SF_BINS 2048     // of a histogram of bits
 #define SF_STEPS 2048    // of the counts by weight: 64 octaves of 32 steps; the last one's keys weigh nothing
 #define SF_LIST 2048     // keys that the first block may be handed
@@ -133,7 +135,7 @@ struct SfShared {
     unsigned long long hist[SF_BINS];
     struct {
       // of a step's keys their number, in two parts; or the sum of their weights in parts of 2^-31 of its largest, upper and lower 16 bits apart
-      unsigned one[SF_STEPS], two[SF_STEPS];
+      unsigned one[SF_STEPS + 32], two[SF_STEPS + 32];  // (what -inf brings goes behind the last step, for each lane apart)
     };
     unsigned long long list[SF_LIST];  // keys falling, equal ones by index: (~key, index)
   };
@@ -320,20 +322,19 @@ struct SfRow {
   // A thread adds up its weights with SF_POINT bits behind the point while it has few of them (a row that is held), else with as many as the sums have.
   __device__ __forceinline__ void add(unsigned long long& sum, unsigned long long w) const { sum += RESIDENT ? w : to_scale(w); }
   __device__ __forceinline__ unsigned long long added(unsigned long long sum) const { return RESIDENT ? to_scale(sum) : sum; }
-  // f(key, index) for this block's keys from `least` (above 0) on
+  // f(keys, index of the first) for this block's keys, a few at a time, 0 among them for -inf.
   template <class F>
-  __device__ __forceinline__ void each_key(unsigned least, F f) const {
+  __device__ __forceinline__ void each_keys(F f) const {
     if (RESIDENT) {  // (the keys behind the last are 0)
       constexpr int V = 16 / (int)sizeof(typename Held::Key);
 #pragma unroll 1
       for (int i = threadIdx.x * V; i < n; i += SF_THREADS * V) {
         const uint4 raw = *reinterpret_cast<const uint4*>(keys + i);
         const typename Held::Key* h = reinterpret_cast<const typename Held::Key*>(&raw);
+        unsigned k[V];
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-          const unsigned k = Held::key(h[e]);
-          if (k >= least) f(k, i + e);
-        }
+        for (int e = 0; e < V; ++e) k[e] = Held::key(h[e]);
+        f(k, i);
       }
       return;
     }
@@ -343,40 +344,49 @@ struct SfRow {
       const int nv = n / V;
       done = nv * V;
 #pragma unroll 1
-      for (int i = threadIdx.x; i < nv; i += 2 * SF_THREADS) {  // two loads in flight
-        const uint4 raw[2] = {__ldg(reinterpret_cast<const uint4*>(row) + i), __ldg(reinterpret_cast<const uint4*>(row) + min(i + SF_THREADS, nv - 1))};
-        const T* x = reinterpret_cast<const T*>(raw);
+      for (int i = threadIdx.x; i < nv; i += 4 * SF_THREADS) {  // four loads in flight
+        uint4 raw[4];
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          if (half && i + SF_THREADS >= nv) break;
+        for (int q = 0; q < 4; ++q) raw[q] = __ldg(reinterpret_cast<const uint4*>(row) + min(i + q * SF_THREADS, nv - 1));
+#pragma unroll 1
+        for (int q = 0; q < 4; ++q) {
+          if (i + q * SF_THREADS >= nv) break;
+          const T* x = reinterpret_cast<const T*>(&raw[0]);
+          unsigned k[V];
 #pragma unroll
-          for (int e = 0; e < V; ++e) {
-            const unsigned k = sf_key(to_f32<T>(x[half * V + e]));
-            if (k >= least) f(k, (i + half * SF_THREADS) * V + e);
-          }
+          for (int e = 0; e < V; ++e) k[e] = sf_key(to_f32<T>(x[e]));
+          f(k, (i + q * SF_THREADS) * V);
+          raw[0] = raw[1]; raw[1] = raw[2]; raw[2] = raw[3];
         }
       }
     }
 #pragma unroll 1
     for (int i = done + threadIdx.x; i < n; i += SF_THREADS) {
-      const unsigned k = key(i);
-      if (k >= least) f(k, i);
+      unsigned k[1] = {key(i)};
+      f(k, i);
     }
   }
 
   // All blocks: the keys by their steps.  With top-k their numbers (in two histograms, for even and odd lanes, so that fewer lanes of a warp meet); without it
   // their weights, to 2^-31 of themselves.
   __device__ __forceinline__ void count_steps(bool numbers) const {
+    const int none = SF_STEPS + (int)(threadIdx.x & 31);
     if (numbers) {
       unsigned* mine = threadIdx.x & 1 ? s.two : s.one;
-      each_key(1u, [&](unsigned k, int) { atomicAdd(mine + step_of(k), 1u); });
+      each_keys([&](const auto& k, int) {
+#pragma unroll
+        for (const unsigned x : k) atomicAdd(mine + (x ? step_of(x) : none), 1u);
+      });
     } else {
-      each_key(1u, [&](unsigned k, int) {
-        float rest;
-        const int n = step_of(k, &rest);
-        const unsigned w = 0x80000000u - (unsigned)__float2int_rn(short_of(rest) * 2147483648.f);
-        atomicAdd(&s.one[n], w >> 16);
-        atomicAdd(&s.two[n], w & 0xffffu);
+      each_keys([&](const auto& k, int) {
+#pragma unroll
+        for (const unsigned x : k) {
+          float rest;
+          const int n = step_of(x, &rest), at = x ? n : none;
+          const unsigned w = 0x80000000u - (unsigned)__float2int_rn(short_of(rest) * 2147483648.f);
+          atomicAdd(&s.one[at], w >> 16);
+          atomicAdd(&s.two[at], w & 0xffffu);
+        }
       });
     }
   }
@@ -384,22 +394,26 @@ struct SfRow {
   // First block: the steps in which the borders lie, from what all blocks have counted.
   __device__ void make_plan(bool k_on, unsigned top_k, bool p_on, float top_p, bool m_on, float min_p, float temperature, float u) {
     constexpr int EACH = SF_STEPS / SF_THREADS, NW = SF_THREADS / 32;
-    static_assert(EACH == 4, "a thread's steps are read 16 bytes at a time");
+    static_assert(EACH % 4 == 0, "a thread's steps are read 16 bytes at a time");
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n0 = tid * EACH;
     unsigned long long one[EACH] = {}, two[EACH] = {};
 #pragma unroll 1
     for (unsigned r0 = 0; r0 < blocks; r0 += 4) {
-      uint4 ones[4], twos[4];  // all of them asked for before the first is used
+      uint4 ones[4][EACH / 4], twos[4][EACH / 4];  // all of them asked for before the first is used
 #pragma unroll
-      for (unsigned r = 0; r < 4; ++r) {
-        ones[r] = r0 + r < blocks ? sf_load4(&s.one[n0], r0 + r) : make_uint4(0u, 0u, 0u, 0u);
-        twos[r] = r0 + r < blocks ? sf_load4(&s.two[n0], r0 + r) : make_uint4(0u, 0u, 0u, 0u);
-      }
+      for (unsigned r = 0; r < 4; ++r)
 #pragma unroll
-      for (unsigned r = 0; r < 4; ++r) {
-        one[0] += ones[r].x; one[1] += ones[r].y; one[2] += ones[r].z; one[3] += ones[r].w;
-        two[0] += twos[r].x; two[1] += twos[r].y; two[2] += twos[r].z; two[3] += twos[r].w;
-      }
+        for (int q = 0; q < EACH / 4; ++q) {
+          ones[r][q] = r0 + r < blocks ? sf_load4(&s.one[n0 + 4 * q], r0 + r) : make_uint4(0u, 0u, 0u, 0u);
+          twos[r][q] = r0 + r < blocks ? sf_load4(&s.two[n0 + 4 * q], r0 + r) : make_uint4(0u, 0u, 0u, 0u);
+        }
+#pragma unroll
+      for (unsigned r = 0; r < 4; ++r)
+#pragma unroll
+        for (int q = 0; q < EACH / 4; ++q) {
+          one[4 * q] += ones[r][q].x; one[4 * q + 1] += ones[r][q].y; one[4 * q + 2] += ones[r][q].z; one[4 * q + 3] += ones[r][q].w;
+          two[4 * q] += twos[r][q].x; two[4 * q + 1] += twos[r][q].y; two[4 * q + 2] += twos[r][q].z; two[4 * q + 3] += twos[r][q].w;
+        }
     }
     if (tid < 8) s.steps[tid] = -1;
     // the smallest key whose weight is at least min_p: exp((v - max) / T) >= min_p where v >= max + T log(min_p)
@@ -550,7 +564,6 @@ struct SfRow {
     if (tid == 0) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) s.plan.range[r] = range[r];
-      s.listed = 0;
       s.all_mass = all_low;
     }
     if (tid >= 4 && tid < 4 * (int)blocks) s.over[tid >> 2][tid & 3] = 0;
@@ -564,55 +577,80 @@ struct SfRow {
 
   // All blocks: the keys of the ranges to the first block; with top-k also the weights above each range (few keys lie there).
   __device__ void hand_over(bool numbers) {
-    int first[4], last[4], begin = SF_STEPS, end = 0;
+    int first[4], last[4];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       first[r] = s.plan.range[r].first;
       last[r] = s.plan.range[r].last;
       if (last[r] < first[r]) {
         first[r] = last[r] = -1;
-      } else {
-        begin = min(begin, first[r]);
-        end = max(end, last[r]);
-        last[r] = min(last[r], SF_STEPS - 2);
       }
     }
     unsigned long long over[4] = {0, 0, 0, 0};
     const int offset = (int)rank * a.per;
-    const auto give = [&](unsigned k, int i) {  // (lanes that come here together take their places with one atomic)
+    // Each block fills the list of its own first; the first block's is the one that counts.  (Lanes that come here together take their places with one atomic.)
+    const auto give = [&](unsigned k, int i) {
       const unsigned with = __activemask(), lead = __ffs(with) - 1, lane = threadIdx.x & 31;
       unsigned at = 0;
-      if (lane == lead) asm volatile("atom.relaxed.cluster.shared::cluster.add.u32 %0, [%1], %2;" : "=r"(at) : "r"(sf_remote(&s.listed, 0)), "r"(__popc(with)) : "memory");
+      if (lane == lead) at = atomicAdd(&s.listed, (unsigned)__popc(with));
       at = __shfl_sync(with, at, lead) + __popc(with & ((1u << lane) - 1));
-      if (at < SF_LIST) sf_store(&s.list[at], 0, ((unsigned long long)~k << 32) | (unsigned)(offset + i));
+      if (at < SF_LIST) s.list[at] = ((unsigned long long)~k << 32) | (unsigned)(offset + i);
     };
-    // the keys of steps begin .. end lie between about these (the steps are looked at again)
-    const float y0 = topf - (float)(end + 2) / (steps * c_hi), y1 = topf - (float)(begin - 1) / (steps * c_hi);
-    const unsigned least = max(sf_key(y0 - fminf(fabsf(y0), 1e38f) * 1e-6f), 1u), most = sf_key(y1 + fminf(fabsf(y1), 1e38f) * 1e-6f);
-    if (numbers) {
-      each_key(least, [&](unsigned k, int i) {
-        float rest;
-        const int n = step_of(k, &rest);
-        bool in = false;
-        const unsigned long long w = weight_at(n, short_of(rest));
+    // The keys of a range lie between about these (the steps are looked at again); with top-k all keys above the last are needed.
+    unsigned from[4], span[4];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          in |= n >= first[r] && n <= last[r];
-          if (n < first[r]) add(over[r], w);
-        }
-        if (in) give(k, i);
-      });
-    } else {
-      each_key(least, [&](unsigned k, int i) {
-        if (k > most) return;
-        const int n = step_of(k);
-        bool in = false;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) in |= n >= first[r] && n <= last[r];
-        if (in) give(k, i);
-      });
-      return;
+    for (int r = 0; r < 4; ++r) {
+      const float y0 = topf - (float)(last[r] + 2) / (steps * c_hi), y1 = topf - (float)(first[r] - 1) / (steps * c_hi);
+      from[r] = max(sf_key(y0 - fminf(fabsf(y0), 1e38f) * 1e-6f), 1u);
+      span[r] = numbers ? 0xffffffffu - from[r] : sf_key(y1 + fminf(fabsf(y1), 1e38f) * 1e-6f) - from[r];
+      if (first[r] < 0) {
+        from[r] = 0xffffffffu;
+        span[r] = 0;
+      }
     }
+    const auto near = [&](unsigned x) {
+      bool is = false;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) is |= x - from[r] <= span[r];
+      return is;
+    };
+    each_keys([&](const auto& k, int i0) {
+      bool any = false;
+#pragma unroll
+      for (const unsigned x : k) any |= near(x);
+      if (!any) return;
+      int i = i0;
+      for (const unsigned x : k) {
+        if (near(x)) {
+          float rest;
+          const int n = step_of(x, &rest);
+          bool in = false;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) in |= n >= first[r] && n <= last[r] && !nothing(n);
+          if (numbers) {
+            const unsigned long long w = weight_at(n, short_of(rest));
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (n < first[r]) add(over[r], w);
+          }
+          if (in) give(x, i);
+        }
+        ++i;
+      }
+    });
+    __syncthreads();
+    if (rank != 0 && s.listed) {
+      const int mine = min((int)s.listed, SF_LIST);
+      if (threadIdx.x == 0) {
+        unsigned at;
+        asm volatile("atom.relaxed.cluster.shared::cluster.add.u32 %0, [%1], %2;" : "=r"(at) : "r"(sf_remote(&s.listed, 0)), "r"(mine) : "memory");
+        s.base[0] = at;
+      }
+      __syncthreads();
+      const int at = (int)s.base[0];
+      for (int i = threadIdx.x; i < mine && at + i < SF_LIST; i += SF_THREADS) sf_store(&s.list[at + i], 0, s.list[i]);
+    }
+    if (!numbers) return;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       over[r] = added(over[r]);
@@ -817,7 +855,7 @@ __device__ __forceinline__ unsigned sf_read(const T* row, int n, int per, typena
 }
 
 template <typename T, bool RESIDENT>
-__global__ void __launch_bounds__(SF_THREADS, 2) sample_filtered_kernel(const __grid_constant__ SfArgs a) {
+__global__ void __launch_bounds__(SF_THREADS, 1024 / SF_THREADS) sample_filtered_kernel(const __grid_constant__ SfArgs a) {
   pdl_launch_dependents();
   extern __shared__ __align__(16) unsigned char smem_raw[];
   SfShared& s = *reinterpret_cast<SfShared*>(smem_raw);
@@ -827,13 +865,13 @@ __global__ void __launch_bounds__(SF_THREADS, 2) sample_filtered_kernel(const __
   const int first = min(a.vocab, (int)rank * a.per);
   SfRow<T, RESIDENT> row{a, s, keys, (const T*)a.logits + (size_t)r * a.ld + first, min(a.vocab, first + a.per) - first, rank, blocks};
   if (blocks > 1) sf_arrive();
-  for (int b = threadIdx.x; b < SF_STEPS; b += SF_THREADS) s.one[b] = s.two[b] = 0;
+  for (int b = threadIdx.x; b < SF_STEPS; b += SF_THREADS) s.one[b] = s.two[b] = 0;  // (nothing reads what lies behind)
   if (threadIdx.x < 32) {
     const unsigned long long x = a.table[threadIdx.x];
     s.table[threadIdx.x] = x;
     s.small_table[threadIdx.x] = (int)((x + (1ull << (SF_POINT - 31))) >> (SF_POINT - 30));
   }
-  if (threadIdx.x == 0) s.high = s.low = 0;
+  if (threadIdx.x == 0) s.high = s.low = s.listed = 0;
   pdl_wait();
   const float temperature = a.temperatures ? a.temperatures[r] : a.temperature;
   const float top_p = a.top_ps ? a.top_ps[r] : a.top_p, asked = a.min_ps ? a.min_ps[r] : a.min_p;
@@ -897,7 +935,7 @@ __global__ void __launch_bounds__(SF_THREADS, 2) sample_filtered_kernel(const __
       }
     }
     unsigned long long valid = 0, before;
-    row.each_key(1u, [&](unsigned, int) { ++valid; });
+    for (int i = threadIdx.x; i < row.n; i += SF_THREADS) valid += row.key(i) != 0u;
     valid = row.exchange_sum(row.block_sum64(valid), &before);
     // kept: all larger than `cut`, and `ties` of those equal to it
     unsigned cut = 1u;
@@ -909,12 +947,13 @@ __global__ void __launch_bounds__(SF_THREADS, 2) sample_filtered_kernel(const __
     }
     auto kept_mass = [&](float least) {
       unsigned long long m = 0;
-      row.each_key(1u, [&](unsigned k, int) {
+      for (int i = threadIdx.x; i < row.n; i += SF_THREADS) {
+        const unsigned k = row.key(i);
         if (k > cut) {
           const double w = row.weight(k);
           if (w >= (double)least) m += row.fixed(w);
         }
-      });
+      }
       m = row.block_sum64(m);
       unsigned long long low, all = row.exchange_sum(m, &low);
       if (ties) {
@@ -967,7 +1006,7 @@ static int sf_run(SfArgs& a, int n_rows, cudaStream_t stream) {
   if (e != cudaSuccess) return BN_ERR_LAUNCH + (int)e;
   int blocks = SF_MAX_CLUSTER;
   while (blocks > 1 && a.vocab <= blocks / 2 * 4096) blocks /= 2;
-  while (blocks > 1 && (long long)n_rows * blocks > 2 * sms && (a.vocab + blocks / 2 - 1) / (blocks / 2) <= SF_COUNTED - 8) blocks /= 2;
+  while (blocks > 1 && (long long)n_rows * blocks > 1024 / SF_THREADS * sms && (a.vocab + blocks / 2 - 1) / (blocks / 2) <= SF_COUNTED - 8) blocks /= 2;
   if (SF_FORCE) blocks = SF_FORCE;
   a.per = (((a.vocab + blocks - 1) / blocks) + 7) & ~7;
   const size_t base = (sizeof(SfShared) + 15) & ~(size_t)15, held = (((size_t)a.per * sizeof(Key)) + 15) & ~(size_t)15;
