@@ -24,7 +24,7 @@
 #define SF_STEPS 2048    // of the counts by weight: 64 octaves of 32 steps; the last one's keys weigh nothing
 #define SF_LIST 2048     // keys that the first block may be handed
 #define SF_FEW 128       // so many of them are one warp's work
-#define SF_COUNTED 65536 // keys of a block whose weights' halves add up in 32 bits whatever their steps
+#define SF_COUNTED 65000 // keys of a block whose weights' halves add up in 32 bits whatever their steps
 #define SF_POINT 56      // a weight of 1 is 2^56 while a thread adds up its own (at most 2^7 of them)
 #define SF_MAX_CLUSTER 8
 
@@ -52,22 +52,6 @@ __device__ __forceinline__ unsigned sf_key(float v) {
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ float sf_value(unsigned key) { return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key); }
-
-// What a block holds of a row: of a bfloat16 the upper half of its key (the lower half follows from the sign).
-template <typename T>
-struct SfHeld;
-template <>
-struct SfHeld<float> {
-  typedef unsigned Key;
-  static __device__ __forceinline__ Key pack(unsigned k) { return k; }
-  static __device__ __forceinline__ unsigned key(Key h) { return h; }
-};
-template <>
-struct SfHeld<__nv_bfloat16> {
-  typedef unsigned short Key;
-  static __device__ __forceinline__ Key pack(unsigned k) { return (Key)(k >> 16); }
-  static __device__ __forceinline__ unsigned key(Key h) { return h == 0 ? 0u : ((unsigned)h << 16) | (h & 0x8000u ? 0u : 0xffffu); }
-};
 
 __device__ __forceinline__ unsigned sf_rank() {
   unsigned r;
@@ -161,9 +145,8 @@ template <typename T, bool RESIDENT>
 struct SfRow {
   SfArgs a;
   SfShared& s;
-  typedef SfHeld<T> Held;
-  const typename Held::Key* keys;  // shared memory, RESIDENT
-  const T* row;          // this block's part of the row
+  const T* held;         // this block's part of the row in shared memory (RESIDENT), -inf behind its end
+  const T* row;          // and where it came from
   int n;                 // numbers of it
   unsigned rank, blocks;
   int turn = 0;
@@ -173,7 +156,7 @@ struct SfRow {
   int fine;                // steps are 2^-fine of a 32nd of an octave: as fine as lets the smallest weight have a step in front of the last
   float steps;             // to an octave
 
-  __device__ __forceinline__ unsigned key(int i) const { return RESIDENT ? Held::key(keys[i]) : sf_key(to_f32<T>(row[i])); }
+  __device__ __forceinline__ unsigned key(int i) const { return sf_key(to_f32<T>(RESIDENT ? held[i] : row[i])); }
   __device__ __forceinline__ double weight(unsigned k) const {
     const double v = (double)sf_value(k);
     return infinite ? (v == top ? 1.0 : 0.0) : exp((v - top) * per_t);
@@ -291,21 +274,24 @@ struct SfRow {
   }
 
   // ---- by steps of weight ----
-  // The step of a key (falling keys, rising steps), and what its y is behind the 32nd of an octave that the step lies in.
-  __device__ __forceinline__ int step_of(unsigned k, float* rest) const {
-    const float v = sf_value(k), d = topf - v, bb = d - topf, dl = (topf - (d - bb)) - (v + bb);
+  // The step of a logit (falling logits, rising steps: the nearest to y), and what its y is from the 32nd of an octave that the step lies in.  Conversions
+  // by adding 1.5 * 2^23: those of the conversion unit take four times the issue slots.
+  __device__ __forceinline__ int step_of(float v, float* rest) const {
+    const float d = topf - v, bb = d - topf, dl = (topf - (d - bb)) - (v + bb);
     const float y = d * c_hi, yl = fmaf(d, c_hi, -y) + fmaf(d, c_lo, dl * c_hi);
-    const int n = min(__float2int_rd(y * steps), SF_STEPS - 1);
-    *rest = fmaf((float)(n >> fine), -1.f / 32.f, y) + yl;
+    const int n = min(__float_as_int(fmaf(fminf(y, 64.f), steps, 12582912.f)) - 0x4B400000, SF_STEPS - 1);
+    *rest = fmaf(__int_as_float((n >> fine) + 0x4B400000) - 12582912.f, -1.f / 32.f, y) + yl;
     return n;
   }
-  __device__ __forceinline__ int step_of(unsigned k) const { return min(__float2int_rd((topf - sf_value(k)) * c_hi * steps), SF_STEPS - 1); }
+  __device__ __forceinline__ int step_of(float v) const {
+    return min(__float_as_int(fmaf(fminf((topf - v) * c_hi, 64.f), steps, 12582912.f)) - 0x4B400000, SF_STEPS - 1);
+  }
   // 1 - 2^-rest
   static __device__ __forceinline__ float short_of(float rest) {
     const float g = rest * 0.69314718f;
     return g * (1.f - g * (0.5f - g * (0.16666667f - g * 0.041666668f)));
   }
-  // The largest weight in a step's 32nd of an octave.
+  // The weight that a step's 32nd of an octave has its keys' weights from.
   __device__ __forceinline__ unsigned long long most_at(int n) const { return s.table[(n >> fine) & 31] >> (n >> fine >> 5); }
   // 2^-y, 1 = 2^SF_POINT, to 2^-30 of itself
   __device__ __forceinline__ unsigned long long weight_at(int n, float e) const {
@@ -322,48 +308,37 @@ struct SfRow {
   // A thread adds up its weights with SF_POINT bits behind the point while it has few of them (a row that is held), else with as many as the sums have.
   __device__ __forceinline__ void add(unsigned long long& sum, unsigned long long w) const { sum += RESIDENT ? w : to_scale(w); }
   __device__ __forceinline__ unsigned long long added(unsigned long long sum) const { return RESIDENT ? to_scale(sum) : sum; }
-  // f(keys, index of the first) for this block's keys, a few at a time, 0 among them for -inf.
+  // f(logits, index of the first) for this block's logits, a few at a time (-inf and NaN among them).
   template <class F>
-  __device__ __forceinline__ void each_keys(F f) const {
-    if (RESIDENT) {  // (the keys behind the last are 0)
-      constexpr int V = 16 / (int)sizeof(typename Held::Key);
-#pragma unroll 1
-      for (int i = threadIdx.x * V; i < n; i += SF_THREADS * V) {
-        const uint4 raw = *reinterpret_cast<const uint4*>(keys + i);
-        const typename Held::Key* h = reinterpret_cast<const typename Held::Key*>(&raw);
-        unsigned k[V];
+  __device__ __forceinline__ void each_value(F f) const {
+    constexpr int V = 16 / (int)sizeof(T);
+    float v[V];
+    const auto take = [&](const uint4& raw, int i) {
+      const T* x = reinterpret_cast<const T*>(&raw);
 #pragma unroll
-        for (int e = 0; e < V; ++e) k[e] = Held::key(h[e]);
-        f(k, i);
-      }
+      for (int e = 0; e < V; ++e) v[e] = to_f32<T>(x[e]);
+      f(v, i);
+    };
+    if (RESIDENT) {
+#pragma unroll 1
+      for (int i = threadIdx.x * V; i < n; i += SF_THREADS * V) take(*reinterpret_cast<const uint4*>(held + i), i);
       return;
     }
-    constexpr int V = 16 / (int)sizeof(T);
     int done = 0;
     if ((((uintptr_t)row) & 15) == 0) {
       const int nv = n / V;
       done = nv * V;
 #pragma unroll 1
-      for (int i = threadIdx.x; i < nv; i += 4 * SF_THREADS) {  // four loads in flight
-        uint4 raw[4];
-#pragma unroll
-        for (int q = 0; q < 4; ++q) raw[q] = __ldg(reinterpret_cast<const uint4*>(row) + min(i + q * SF_THREADS, nv - 1));
-#pragma unroll 1
-        for (int q = 0; q < 4; ++q) {
-          if (i + q * SF_THREADS >= nv) break;
-          const T* x = reinterpret_cast<const T*>(&raw[0]);
-          unsigned k[V];
-#pragma unroll
-          for (int e = 0; e < V; ++e) k[e] = sf_key(to_f32<T>(x[e]));
-          f(k, (i + q * SF_THREADS) * V);
-          raw[0] = raw[1]; raw[1] = raw[2]; raw[2] = raw[3];
-        }
+      for (int i = threadIdx.x; i < nv; i += 2 * SF_THREADS) {  // two loads in flight
+        const uint4 a0 = __ldg(reinterpret_cast<const uint4*>(row) + i), a1 = __ldg(reinterpret_cast<const uint4*>(row) + min(i + SF_THREADS, nv - 1));
+        take(a0, i * V);
+        if (i + SF_THREADS < nv) take(a1, (i + SF_THREADS) * V);
       }
     }
 #pragma unroll 1
     for (int i = done + threadIdx.x; i < n; i += SF_THREADS) {
-      unsigned k[1] = {key(i)};
-      f(k, i);
+      const float x[1] = {to_f32<T>(row[i])};
+      f(x, i);
     }
   }
 
@@ -373,19 +348,20 @@ struct SfRow {
     const int none = SF_STEPS + (int)(threadIdx.x & 31);
     if (numbers) {
       unsigned* mine = threadIdx.x & 1 ? s.two : s.one;
-      each_keys([&](const auto& k, int) {
+      each_value([&](const auto& v, int) {
 #pragma unroll
-        for (const unsigned x : k) atomicAdd(mine + (x ? step_of(x) : none), 1u);
+        for (const float x : v) atomicAdd(mine + (x > -INFINITY ? step_of(x) : none), 1u);
       });
     } else {
-      each_keys([&](const auto& k, int) {
+      each_value([&](const auto& v, int) {
 #pragma unroll
-        for (const unsigned x : k) {
+        for (const float x : v) {
           float rest;
-          const int n = step_of(x, &rest), at = x ? n : none;
-          const unsigned w = 0x80000000u - (unsigned)__float2int_rn(short_of(rest) * 2147483648.f);
-          atomicAdd(&s.one[at], w >> 16);
-          atomicAdd(&s.two[at], w & 0xffffu);
+          const int n = step_of(x, &rest), at = x > -INFINITY ? n : none;
+          // 2^31 - e 2^31 in halves: e 2^15 is cut to a whole number, what is left of it has 16 bits more
+          const float e = short_of(rest), z = fmaf(e, 32768.f, -0.5f) + 12582912.f, left = fmaf(e, 32768.f, 12582912.f - z);
+          atomicAdd(&s.one[at], (unsigned)(0x4B400000 + 32767 - __float_as_int(z)));
+          atomicAdd(&s.two[at], (unsigned)(0x4B400000 + 65536 - __float_as_int(fmaf(left, 65536.f, 12582912.f))));
         }
       });
     }
@@ -430,9 +406,8 @@ struct SfRow {
       const unsigned long long t = most_at(n);
       if (k_on) {
         c[e] = (unsigned)(one[e] + two[e]);
-        const unsigned long long t1 = most_at(n + (1 << fine));
-        up[e] = c[e] * (to_scale(t + (t >> 10)) + 1);
-        lo[e] = c[e] * to_scale(t1 - (t1 >> 10));
+        up[e] = c[e] * (to_scale(t + (t >> 6)) + 1);  // (2^(1/64) at most, 2^(-1/32) at least)
+        lo[e] = c[e] * to_scale(t - (t >> 5));
       } else {
         const unsigned long long w = (one[e] << 16) + two[e];  // 1 = 2^31, below 2^51
         c[e] = (unsigned)((w + (w >> 5)) >> 31) + (w ? 1u : 0u);
@@ -494,7 +469,7 @@ struct SfRow {
       if (lane == 0 && by_lo != ~0u) atomicMin((unsigned*)&s.steps[slot + 1], by_lo);
     };
     const unsigned kth = min(top_k, total);
-    const int m_step = m_on ? step_of(s.plan.least) : SF_STEPS;
+    const int m_step = m_on ? step_of(sf_value(s.plan.least)) : SF_STEPS;
 #pragma unroll
     for (int e = 0; e < EACH; ++e) {
       if (k_on && ci[e] - c[e] < kth && ci[e] >= kth) {
@@ -527,7 +502,7 @@ struct SfRow {
       cut = p1;
       kept_low = part(top_p, all_low);
       const unsigned long long t = most_at(p0);  // the token that crosses stays
-      kept_up = part(top_p, all_up) + to_scale(t + (t >> 10)) + 1;
+      kept_up = part(top_p, all_up) + to_scale(t + (t >> 6)) + 1;
     }
     if (m_on && (m_step <= cut || !(k_on || p_on))) {
       if (m_step < (p_on ? range[SF_TOP_P].first : k_step) || !(k_on || p_on)) {  // what lies behind does not matter
@@ -588,39 +563,31 @@ struct SfRow {
     }
     unsigned long long over[4] = {0, 0, 0, 0};
     const int offset = (int)rank * a.per;
-    // Each block fills the list of its own first; the first block's is the one that counts.  (Lanes that come here together take their places with one atomic.)
+    // Each block fills the list of its own first; the first block's is the one that counts.
     const auto give = [&](unsigned k, int i) {
-      const unsigned with = __activemask(), lead = __ffs(with) - 1, lane = threadIdx.x & 31;
-      unsigned at = 0;
-      if (lane == lead) at = atomicAdd(&s.listed, (unsigned)__popc(with));
-      at = __shfl_sync(with, at, lead) + __popc(with & ((1u << lane) - 1));
+      const unsigned at = atomicAdd(&s.listed, 1u);
       if (at < SF_LIST) s.list[at] = ((unsigned long long)~k << 32) | (unsigned)(offset + i);
     };
-    // The keys of a range lie between about these (the steps are looked at again); with top-k all keys above the last are needed.
-    unsigned from[4], span[4];
+    // The logits of a range lie between about these (the steps are looked at again); with top-k all above the last are needed.
+    float from[4], to[4];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const float y0 = topf - (float)(last[r] + 2) / (steps * c_hi), y1 = topf - (float)(first[r] - 1) / (steps * c_hi);
-      from[r] = max(sf_key(y0 - fminf(fabsf(y0), 1e38f) * 1e-6f), 1u);
-      span[r] = numbers ? 0xffffffffu - from[r] : sf_key(y1 + fminf(fabsf(y1), 1e38f) * 1e-6f) - from[r];
-      if (first[r] < 0) {
-        from[r] = 0xffffffffu;
-        span[r] = 0;
-      }
+      const float y0 = topf - (float)(last[r] + 2) / (steps * c_hi), y1 = topf - (float)(first[r] - 2) / (steps * c_hi);
+      from[r] = fmaxf(y0 - fminf(fabsf(y0), 1e38f) * 1e-6f, -3.4028235e38f);
+      to[r] = numbers ? INFINITY : y1 + fminf(fabsf(y1), 1e38f) * 1e-6f;
+      if (first[r] < 0) from[r] = INFINITY, to[r] = -INFINITY;
     }
-    const auto near = [&](unsigned x) {
-      bool is = false;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) is |= x - from[r] <= span[r];
-      return is;
+    if (numbers) from[1] = fminf(fminf(from[0], from[1]), fminf(from[2], from[3]));
+    const auto near = [&](float x) {  // (there is no border of top-k without its numbers)
+      return numbers ? x >= from[1] : (x >= from[1] && x <= to[1]) || (x >= from[2] && x <= to[2]) || (x >= from[3] && x <= to[3]);
     };
-    each_keys([&](const auto& k, int i0) {
+    each_value([&](const auto& v, int i0) {
       bool any = false;
 #pragma unroll
-      for (const unsigned x : k) any |= near(x);
+      for (const float x : v) any |= near(x);
       if (!any) return;
       int i = i0;
-      for (const unsigned x : k) {
+      for (const float x : v) {
         if (near(x)) {
           float rest;
           const int n = step_of(x, &rest);
@@ -633,7 +600,7 @@ struct SfRow {
             for (int r = 0; r < 4; ++r)
               if (n < first[r]) add(over[r], w);
           }
-          if (in) give(x, i);
+          if (in) give(sf_key(x), i);
         }
         ++i;
       }
@@ -696,7 +663,7 @@ struct SfRow {
 #pragma unroll 1
       for (int i = i0; i < i1; ++i) {
         float rest;
-        const int n = step_of(~(unsigned)(s.list[i] >> 32), &rest);
+        const int n = step_of(sf_value(~(unsigned)(s.list[i] >> 32)), &rest);
         const unsigned long long next = run + to_scale(weight_at(n, short_of(rest)));
         f(i, n, run, next);
         run = next;
@@ -736,7 +703,7 @@ struct SfRow {
     if (tid == 0) { s.sum[0] = is_in(SF_TOP_K) ? over[SF_TOP_K] : s.all_mass; s.sum[1] = is_in(SF_MIN_P) ? over[SF_MIN_P] : ~0ull; }
     sync();
     // where each range begins, and the running sum in front of it
-    int prev = i0 > 0 ? step_of(~(unsigned)(s.list[i0 - 1] >> 32)) : -1;
+    int prev = i0 > 0 ? step_of(sf_value(~(unsigned)(s.list[i0 - 1] >> 32))) : -1;
     walk(run0, [&](int i, int n, unsigned long long before, unsigned long long) {
 #pragma unroll
       for (int r = 0; r < 4; ++r)
@@ -817,38 +784,35 @@ struct SfRow {
   }
 };
 
-// Keys of one block's part of a row into shared memory (RESIDENT); the largest, and the smallest above -inf.
+// One block's part of a row into shared memory (RESIDENT); the largest of it, and the smallest above -inf (or +inf).
 template <typename T, bool RESIDENT>
-__device__ __forceinline__ unsigned sf_read(const T* row, int n, int per, typename SfHeld<T>::Key* keys, unsigned* smallest) {
-  typedef SfHeld<T> Held;
-  unsigned high = 0, low = 0;  // (low: of 0 - key, which is 0 for -inf)
+__device__ __forceinline__ float sf_read(const T* row, int n, int per, T* held, float* smallest) {
+  float high = -INFINITY, low = INFINITY;
   constexpr int V = 16 / (int)sizeof(T);
   int done = 0;
   if ((((uintptr_t)row) & 15) == 0) {
     const int nv = n / V;
 #pragma unroll 8
     for (int i = threadIdx.x; i < nv; i += SF_THREADS) {
-      const uint4 raw = __ldcs(reinterpret_cast<const uint4*>(row) + i);
+      const uint4 raw = __ldg(reinterpret_cast<const uint4*>(row) + i);
       const T* x = reinterpret_cast<const T*>(&raw);
-      uint4 packed;
-      typename Held::Key* h = reinterpret_cast<typename Held::Key*>(&packed);
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        const unsigned k = sf_key(to_f32<T>(x[e]));
-        high = max(high, k);
-        low = max(low, 0u - k);
-        h[e] = Held::pack(k);
+        const float v = to_f32<T>(x[e]);
+        high = fmaxf(high, v);
+        low = fminf(low, v > -INFINITY ? v : INFINITY);
       }
-      if (RESIDENT) reinterpret_cast<uint4*>(keys)[i] = packed;
+      if (RESIDENT) reinterpret_cast<uint4*>(held)[i] = raw;
     }
     done = nv * V;
   }
 #pragma unroll 8
   for (int i = done + threadIdx.x; i < (RESIDENT ? per : n); i += SF_THREADS) {
-    const unsigned k = i < n ? sf_key(to_f32<T>(row[i])) : 0u;
-    high = max(high, k);
-    low = max(low, 0u - k);
-    if (RESIDENT) keys[i] = Held::pack(k);
+    const T x = i < n ? row[i] : from_f32<T>(-INFINITY);
+    const float v = to_f32<T>(x);
+    high = fmaxf(high, v);
+    low = fminf(low, v > -INFINITY ? v : INFINITY);
+    if (RESIDENT) held[i] = x;
   }
   *smallest = low;
   return high;
@@ -859,11 +823,11 @@ __global__ void __launch_bounds__(SF_THREADS, 1024 / SF_THREADS) sample_filtered
   pdl_launch_dependents();
   extern __shared__ __align__(16) unsigned char smem_raw[];
   SfShared& s = *reinterpret_cast<SfShared*>(smem_raw);
-  typename SfHeld<T>::Key* keys = reinterpret_cast<typename SfHeld<T>::Key*>(smem_raw + ((sizeof(SfShared) + 15) & ~(size_t)15));
+  T* held = reinterpret_cast<T*>(smem_raw + ((sizeof(SfShared) + 15) & ~(size_t)15));
   const unsigned rank = sf_rank(), blocks = sf_size();
   const int r = blockIdx.x / blocks;
   const int first = min(a.vocab, (int)rank * a.per);
-  SfRow<T, RESIDENT> row{a, s, keys, (const T*)a.logits + (size_t)r * a.ld + first, min(a.vocab, first + a.per) - first, rank, blocks};
+  SfRow<T, RESIDENT> row{a, s, held, (const T*)a.logits + (size_t)r * a.ld + first, min(a.vocab, first + a.per) - first, rank, blocks};
   if (blocks > 1) sf_arrive();
   for (int b = threadIdx.x; b < SF_STEPS; b += SF_THREADS) s.one[b] = s.two[b] = 0;  // (nothing reads what lies behind)
   if (threadIdx.x < 32) {
@@ -877,7 +841,8 @@ __global__ void __launch_bounds__(SF_THREADS, 1024 / SF_THREADS) sample_filtered
   const float top_p = a.top_ps ? a.top_ps[r] : a.top_p, asked = a.min_ps ? a.min_ps[r] : a.min_p;
   const float min_p = asked > 0.f ? fminf(asked, 1.f) : 0.f;  // the most probable token always stays
   const int top_k = a.top_ks ? a.top_ks[r] : a.top_k;
-  unsigned low, high = sf_read<T, RESIDENT>(row.row, row.n, a.per, keys, &low);
+  float smallest;
+  unsigned high = sf_key(sf_read<T, RESIDENT>(row.row, row.n, a.per, held, &smallest)), low = 0u - sf_key(smallest);
   if (blocks > 1) sf_wait();
   else __syncthreads();  // every block of the cluster runs: its shared memory may be written
   // the random number, drawn once for the whole cluster
@@ -999,7 +964,6 @@ static int sf_launch(const SfArgs& a, int n_rows, int blocks, size_t smem, cudaS
 }
 template <typename T>
 static int sf_run(SfArgs& a, int n_rows, cudaStream_t stream) {
-  typedef typename SfHeld<T>::Key Key;
   int device = 0, sms = 0;
   cudaError_t e = cudaGetDevice(&device);
   if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
@@ -1009,7 +973,7 @@ static int sf_run(SfArgs& a, int n_rows, cudaStream_t stream) {
   while (blocks > 1 && (long long)n_rows * blocks > 1024 / SF_THREADS * sms && (a.vocab + blocks / 2 - 1) / (blocks / 2) <= SF_COUNTED - 8) blocks /= 2;
   if (SF_FORCE) blocks = SF_FORCE;
   a.per = (((a.vocab + blocks - 1) / blocks) + 7) & ~7;
-  const size_t base = (sizeof(SfShared) + 15) & ~(size_t)15, held = (((size_t)a.per * sizeof(Key)) + 15) & ~(size_t)15;
+  const size_t base = (sizeof(SfShared) + 15) & ~(size_t)15, held = (((size_t)a.per * sizeof(T)) + 15) & ~(size_t)15;
   const size_t room = (long long)n_rows * blocks <= sms ? 220 * 1024 : 112 * 1024;
   bool resident = base + held <= room && a.per <= 128 * SF_THREADS;
   if (SF_RES >= 0) resident = SF_RES && base + held <= 220 * 1024 && a.per <= 128 * SF_THREADS;
