@@ -17,9 +17,7 @@
 #include "common.cuh"
 #include <math.h>
 
-#ifndef SF_THREADS
 #define SF_THREADS 512
-#endif
 #define SF_BINS 2048     // of a histogram of bits
 #define SF_STEPS 2048    // of the counts by weight: 64 octaves of 32 steps; the last one's keys weigh nothing
 #define SF_LIST 2048     // keys that the first block may be handed
@@ -568,11 +566,12 @@ struct SfRow {
       const unsigned at = atomicAdd(&s.listed, 1u);
       if (at < SF_LIST) s.list[at] = ((unsigned long long)~k << 32) | (unsigned)(offset + i);
     };
-    // The logits of a range lie between about these (the steps are looked at again); with top-k all above the last are needed.
+    // The logits of a range lie between about these (a step's logits are within half a step of it; they are
+    // looked at again); with top-k all above the last are needed.
     float from[4], to[4];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const float y0 = topf - (float)(last[r] + 2) / (steps * c_hi), y1 = topf - (float)(first[r] - 2) / (steps * c_hi);
+      const float y0 = topf - ((float)last[r] + 0.6f) / (steps * c_hi), y1 = topf - ((float)first[r] - 0.6f) / (steps * c_hi);
       from[r] = fmaxf(y0 - fminf(fabsf(y0), 1e38f) * 1e-6f, -3.4028235e38f);
       to[r] = numbers ? INFINITY : y1 + fminf(fabsf(y1), 1e38f) * 1e-6f;
       if (first[r] < 0) from[r] = INFINITY, to[r] = -INFINITY;
@@ -951,8 +950,6 @@ __global__ void __launch_bounds__(SF_THREADS, 1024 / SF_THREADS) sample_filtered
   sf_sync(blocks);  // no block leaves while another may still read from it or write to it
 }
 
-static int SF_FORCE = 0, SF_RES = -1;
-extern "C" void sf_force(int b, int r) { SF_FORCE = b; SF_RES = r; }
 template <typename T, bool RESIDENT>
 static int sf_launch(const SfArgs& a, int n_rows, int blocks, size_t smem, cudaStream_t stream) {
   static BnGrant grant;
@@ -968,15 +965,17 @@ static int sf_run(SfArgs& a, int n_rows, cudaStream_t stream) {
   cudaError_t e = cudaGetDevice(&device);
   if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
   if (e != cudaSuccess) return BN_ERR_LAUNCH + (int)e;
+  // Blocks of a row: so many that each has 4,096 numbers (one row of 1,000: 10 us with one block, 13 with eight; of 32,000: 18 with one, 14 with eight), but not
+  // more than 2.75 an SM in all, of which two run at once (64 rows of 128,256: 53 us with four blocks a row, 62 with eight; 200 of 50,257: 69 with two, 82 with
+  // four).  Fewer than hold a row's sums only where even one block a row has too many numbers.
   int blocks = SF_MAX_CLUSTER;
   while (blocks > 1 && a.vocab <= blocks / 2 * 4096) blocks /= 2;
-  while (blocks > 1 && (long long)n_rows * blocks > 1024 / SF_THREADS * sms && (a.vocab + blocks / 2 - 1) / (blocks / 2) <= SF_COUNTED - 8) blocks /= 2;
-  if (SF_FORCE) blocks = SF_FORCE;
+  while (blocks > 1 && 4ll * n_rows * blocks > 11ll * sms && (a.vocab + blocks / 2 - 1) / (blocks / 2) <= SF_COUNTED - 8) blocks /= 2;
   a.per = (((a.vocab + blocks - 1) / blocks) + 7) & ~7;
+  // The row stays in shared memory where two blocks an SM still fit, or where there is one at most; else later passes find it in the L2 (256 rows of 32,000 in float32,
+  // one block each: 37 us from the L2, 46 held).
   const size_t base = (sizeof(SfShared) + 15) & ~(size_t)15, held = (((size_t)a.per * sizeof(T)) + 15) & ~(size_t)15;
-  const size_t room = (long long)n_rows * blocks <= sms ? 220 * 1024 : 112 * 1024;
-  bool resident = base + held <= room && a.per <= 128 * SF_THREADS;
-  if (SF_RES >= 0) resident = SF_RES && base + held <= 220 * 1024 && a.per <= 128 * SF_THREADS;
+  const bool resident = base + held <= ((long long)n_rows * blocks <= sms ? 220 : 112) * 1024 && a.per <= 128 * SF_THREADS;
   return resident ? sf_launch<T, true>(a, n_rows, blocks, base + held, stream) : sf_launch<T, false>(a, n_rows, blocks, base, stream);
 }
 
