@@ -64,6 +64,13 @@ __device__ __forceinline__ float dt_ld_dsmem(unsigned local_addr, unsigned rank)
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote) : "memory");
   return v;
 }
+__device__ __forceinline__ float4 dt_ld_dsmem4(unsigned local_addr, unsigned rank) {  // 16-byte aligned
+  unsigned remote;
+  float4 v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(local_addr), "r"(rank));
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(remote) : "memory");
+  return v;
+}
 struct DtArgs {
   const __nv_bfloat16* qkv;  // [n_seqs, q_stride]: raw query heads, key heads at k_off, value heads at v_off
   int q_stride, k_off, v_off;
@@ -97,25 +104,40 @@ struct DtArgs {
   int n_shared;           // results that there are
 };
 
-// A row's element d from this kernel's keys (maximum m, sum den, unnormalised num) and from the shared ones: num and den over both, by the larger maximum.
-__device__ __forceinline__ float dt_join(const DtArgs& a, const int4& sh, int h, int d, float m, float den, float num) {
-  if (sh.y < 0 || sh.y + sh.z > a.n_shared) return num / den;  // (a list that does not go with this launch: nothing is read past its end)
-  const float* ml = a.shared_ml + ((size_t)sh.y * a.n_heads + h) * 2;
+// Four neighbouring elements of a row, d and on, from this kernel's keys (maximum m, sum den, unnormalised num) and from the shared ones: by the largest maximum.
+// The loads of eight results are in flight together.
+__device__ __forceinline__ float4 dt_join(const DtArgs& a, const int4& sh, int h, int d, float m, float den, float4 num) {
+  const int parts = sh.y < 0 || sh.y + sh.z > a.n_shared ? 0 : sh.z;  // (a list that does not go with this launch: nothing is read past its end)
+  const float2* ml = reinterpret_cast<const float2*>(a.shared_ml) + (size_t)sh.y * a.n_heads + h;
   const float* o = a.shared_o + ((size_t)sh.y * a.n_heads + h) * a.head_dim + d;
-  float top = m;
-#pragma unroll 4
-  for (int p = 0; p < sh.z; ++p) top = fmaxf(top, __ldcg(ml + (size_t)p * a.n_heads * 2));
-  const float own = (m == -INFINITY) ? 0.f : exp2f(m - top);
-  den *= own;
-  num *= own;
-#pragma unroll 4
-  for (int p = 0; p < sh.z; ++p) {
-    const float2 one = __ldcg(reinterpret_cast<const float2*>(ml + (size_t)p * a.n_heads * 2));
-    const float w = (one.x == -INFINITY) ? 0.f : exp2f(one.x - top);
-    den += w * one.y;
-    num += w * __ldcg(o + (size_t)p * a.n_heads * a.head_dim);
+  const size_t o_next = (size_t)a.n_heads * a.head_dim;
+  for (int p0 = 0; p0 < parts; p0 += 8) {
+    float2 s[8];
+    float4 v[8];
+    float top = m;
+#pragma unroll
+    for (int p = 0; p < 8; ++p) {
+      const bool on = p0 + p < parts;
+      s[p] = on ? __ldcg(ml + (size_t)(p0 + p) * a.n_heads) : make_float2(-INFINITY, 0.f);
+      v[p] = on ? __ldcg(reinterpret_cast<const float4*>(o + (p0 + p) * o_next)) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+#pragma unroll
+    for (int p = 0; p < 8; ++p) top = fmaxf(top, s[p].x);
+    const float own = (m == -INFINITY) ? 0.f : exp2f(m - top);
+    m = top;
+    den *= own;
+    num.x *= own; num.y *= own; num.z *= own; num.w *= own;
+#pragma unroll
+    for (int p = 0; p < 8; ++p) {
+      const float w = (s[p].x == -INFINITY) ? 0.f : exp2f(s[p].x - top);
+      den += w * s[p].y;
+      if (p0 + p < parts) { num.x += w * v[p].x; num.y += w * v[p].y; num.z += w * v[p].z; num.w += w * v[p].w; }
+    }
   }
-  return num / den;
+  return make_float4(num.x / den, num.y / den, num.z / den, num.w / den);
+}
+__device__ __forceinline__ void dt_store4(__nv_bfloat16* p, float4 v) {  // 8-byte aligned
+  *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
 }
 
 // JOIN: the first pages of a sequence are attended to by the kernel in front of this one (attention_shared.cu), which lets this one start as soon as
@@ -482,14 +504,27 @@ attention_decode_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
     ml_fin[tid * 2 + 1] = l;  // rows past G hold zeros: maximum -inf, sum 0
   }
   __syncthreads();
+  if (JOIN && alone) {
+    for (int i = tid; i < G * (head_dim >> 2); i += DT_THREADS) {
+      const int g = i / (head_dim >> 2), d = 4 * (i - g * (head_dim >> 2));
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const float4 x = *reinterpret_cast<const float4*>(o_part + (size_t)(w * DT_ROWS + g) * OSTRIDE + d);
+        const float s = wsc[w * DT_ROWS + g];
+        acc.x += s * x.x; acc.y += s * x.y; acc.z += s * x.z; acc.w += s * x.w;
+      }
+      dt_store4(a.out + (size_t)b * a.out_stride + (size_t)(h0 + g) * head_dim + d, dt_join(a, sh, h0 + g, d, ml_fin[g * 2], ml_fin[g * 2 + 1], acc));
+    }
+    return;
+  }
   for (int i = tid; i < G * head_dim; i += DT_THREADS) {
     int g = i / head_dim, d = i - g * head_dim;
     float acc = 0.f;
 #pragma unroll
     for (int w = 0; w < 4; ++w) acc += wsc[w * DT_ROWS + g] * o_part[(size_t)(w * DT_ROWS + g) * OSTRIDE + d];
     if (alone)  // the only split of this sequence: normalise and store
-      a.out[(size_t)b * a.out_stride + (size_t)(h0 + g) * head_dim + d] =
-          __float2bfloat16_rn(JOIN ? dt_join(a, sh, h0 + g, d, ml_fin[g * 2], ml_fin[g * 2 + 1], acc) : acc / ml_fin[g * 2 + 1]);
+      a.out[(size_t)b * a.out_stride + (size_t)(h0 + g) * head_dim + d] = __float2bfloat16_rn(acc / ml_fin[g * 2 + 1]);
     else if (clustered) o_fin[g * HD + d] = acc;
     else a.part_o[(((size_t)b * n_heads + h0 + g) * n_splits + zi) * head_dim + d] = acc;
   }
@@ -504,6 +539,34 @@ attention_decode_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
     BN_TRACE_ONLY(if (tr) tr[8] = global_timer();)
     const unsigned a_ml = smem_u32(ml_fin), a_o = smem_u32(o_fin);
     const int n_act = z_hi - z_lo + 1, mine = zi - z_lo;
+    if (JOIN) {  // four elements at a time
+      const int quads = head_dim >> 2, total = G * quads, per = (total + n_act - 1) / n_act;
+      for (int i = mine * per + tid; i < min(total, (mine + 1) * per); i += DT_THREADS) {
+        const int g = i / quads, d = 4 * (i - g * quads);
+        float mz[8], lz[8], m = -INFINITY;
+        float4 v[8];
+#pragma unroll
+        for (int z = 0; z < 8; ++z) {
+          const bool on = z >= z_lo && z <= z_hi;
+          mz[z] = on ? dt_ld_dsmem(a_ml + (unsigned)(g * 2) * 4, (unsigned)z) : -INFINITY;
+          lz[z] = on ? dt_ld_dsmem(a_ml + (unsigned)(g * 2 + 1) * 4, (unsigned)z) : 0.f;
+          v[z] = on ? dt_ld_dsmem4(a_o + (unsigned)(g * HD + d) * 4, (unsigned)z) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+#pragma unroll
+        for (int z = 0; z < 8; ++z) m = fmaxf(m, mz[z]);
+        float den = 0.f;
+        float4 num = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int z = 0; z < 8; ++z) {
+          const float w = (mz[z] == -INFINITY) ? 0.f : exp2f(mz[z] - m);
+          den += w * lz[z];
+          num.x += w * v[z].x; num.y += w * v[z].y; num.z += w * v[z].z; num.w += w * v[z].w;
+        }
+        dt_store4(a.out + (size_t)b * a.out_stride + (size_t)(h0 + g) * head_dim + d, dt_join(a, sh, h0 + g, d, m, den, num));
+      }
+      dt_cluster_sync();
+      return;
+    }
     const int total = G * head_dim, per = (total + n_act - 1) / n_act;
     for (int i = mine * per + tid; i < min(total, (mine + 1) * per); i += DT_THREADS) {
       int g = i / head_dim, d = i - g * head_dim;
@@ -526,12 +589,13 @@ attention_decode_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
         den += w * lz[z];
         num += w * v[z];
       }
-      a.out[(size_t)b * a.out_stride + (size_t)(h0 + g) * head_dim + d] = __float2bfloat16_rn(JOIN ? dt_join(a, sh, h0 + g, d, m, den, num) : num / den);
+      a.out[(size_t)b * a.out_stride + (size_t)(h0 + g) * head_dim + d] = __float2bfloat16_rn(num / den);
     }
     BN_TRACE_ONLY(if (tr) tr[10] = global_timer();)
     dt_cluster_sync();  // no block leaves while another still reads its result
     return;
   }
+  if (JOIN) return;  // (never: at most eight splits, which are a cluster)
   if (tid < G) {
     size_t oo = (((size_t)b * n_heads + h0 + tid) * n_splits + zi) * 2;
     a.part_ml[oo] = ml_fin[tid * 2];
@@ -567,8 +631,7 @@ attention_decode_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
     const float* po = a.part_o + ((size_t)b * n_heads + h0 + g) * n_splits * head_dim;
     float m = ml_fin[g * 2], num = 0.f;
     for (int z = z_lo; z <= z_hi; ++z) num += exp2f(__ldcg(ml + 2 * z) - m) * __ldcg(po + (size_t)z * head_dim + d);
-    a.out[(size_t)b * a.out_stride + (size_t)(h0 + g) * head_dim + d] =
-        __float2bfloat16_rn(JOIN ? dt_join(a, sh, h0 + g, d, m, ml_fin[g * 2 + 1], num) : num / ml_fin[g * 2 + 1]);
+    a.out[(size_t)b * a.out_stride + (size_t)(h0 + g) * head_dim + d] = __float2bfloat16_rn(num / ml_fin[g * 2 + 1]);
   }
   BN_TRACE_ONLY(if (tr) tr[10] = global_timer();)
 }
@@ -712,6 +775,7 @@ static int dt_run(const void* qkv, int q_stride, int k_off, int v_off, void* out
       !tma_map_bf16_pages(&mv, v_cache, n_cache_pages, (unsigned long long)n_kv_heads * BN_PAGE, head_dim, BN_PAGE))
     return BN_ERR_BAD_ARG;
   if (shared != nullptr) {
+    if (n_splits > 8 || out_stride % 4 || (((uintptr_t)out) & 7)) return BN_ERR_BAD_ARG;  // (splits are merged within a cluster)
     if (head_dim <= 64) return launch_dt<64, true>(mk, mv, a, grid, cluster, stream);
     return launch_dt<128, true>(mk, mv, a, grid, cluster, stream);
   }
@@ -742,8 +806,8 @@ extern "C" int bn_attention_decode_tc_items(const void* qkv, int q_stride, int k
 }
 // With the first shared[4 b] pages of each sequence b attended to by attention_shared.cu, launched directly in front (it lets this kernel start early): its
 // results shared[4 b + 1] .. + shared[4 b + 2] - 1 of shared_o / shared_ml are joined with those of the other pages, of which there is at least one (the
-// new token's).  n_splits blocks share a sequence's other pages, about
-// pages_per_block each.  No window, no rotation (the rows are rotated), head_dim at most 128.
+// new token's).  n_splits blocks (at most 8) share a sequence's other
+// pages, about pages_per_block each.  No window, no rotation (the rows are rotated), head_dim at most 128.
 extern "C" int bn_attention_decode_tc_join(const void* qkv, int q_stride, int k_off, int v_off, void* out, int out_stride,
                                            int n_seqs, int n_heads, int n_kv_heads, int head_dim, float scale, const int* tok_pos, const int* slots,
                                            const int* page_table, int pt_stride, void* k_cache, void* v_cache,

@@ -166,16 +166,26 @@ attention_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
     }
   } else {
     pdl_wait();
-    // ---- the queries, into the layout that TMA would leave: boxes of 128 rows x 64 numbers, 16-byte pieces XORed with the row
-    constexpr int PIECES = HD / 8;
-    for (int e = tid - 64; e < AS_ROWS * PIECES; e += 128) {
-      const int row = e / PIECES, c = e % PIECES;
-      uint4 v = make_uint4(0u, 0u, 0u, 0u);
-      if (row < rows && c * 8 < a.head_dim) {
-        const int seq = members[row / a.per_group].x, h = kvh * a.per_group + row % a.per_group;
-        v = *reinterpret_cast<const uint4*>(a.q + (size_t)seq * a.q_stride + (size_t)h * a.head_dim + c * 8);
+    // ---- the queries, into the layout that TMA would leave: boxes of 128 rows x 64 numbers, 16-byte pieces XORed with the row.  A thread copies one piece
+    // of every eighth (or fourth) row, all of its loads in flight before the first store.
+    {
+      constexpr int PIECES = HD / 8, EACH = PIECES, APART = 128 / PIECES;
+      const int t = tid - 64, c = t % PIECES, row0 = t / PIECES;
+      uint4 v[EACH];
+#pragma unroll
+      for (int e = 0; e < EACH; ++e) {
+        const int row = row0 + e * APART;
+        v[e] = make_uint4(0u, 0u, 0u, 0u);
+        if (row < rows && c * 8 < a.head_dim) {
+          const int member = row / a.per_group, h = kvh * a.per_group + row - member * a.per_group;
+          v[e] = *reinterpret_cast<const uint4*>(a.q + (size_t)members[member].x * a.q_stride + (size_t)h * a.head_dim + c * 8);
+        }
       }
-      *reinterpret_cast<uint4*>(q_smem + (c >> 3) * Q_BOX + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = v;
+#pragma unroll
+      for (int e = 0; e < EACH; ++e) {
+        const int row = row0 + e * APART;
+        *reinterpret_cast<uint4*>(q_smem + (c >> 3) * Q_BOX + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = v[e];
+      }
     }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncwarp();
@@ -243,16 +253,25 @@ attention_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
       const bool store = part >= 0 && part < a.n_parts;
       const size_t at = (size_t)part * a.n_heads + h;
       if (store) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(m_ref, l_run);
+      // A row of O lies in one lane: by way of shared memory (the queries and pages are done with), where rows of OSTRIDE bytes keep the lanes of a store
+      // on different banks, it goes out as one copy of the row
+      constexpr int OSTRIDE = HD * 4 + 16;
+      static_assert(AS_ROWS * OSTRIDE <= BOXES * Q_BOX + (KS + VS) * PAGE_BYTES, "the rows of O reuse the queries' and pages' room");
+      unsigned char* orow = q_smem + r * OSTRIDE;
 #pragma unroll
       for (int c = 0; c < HD; c += 32) {
         float o[32];
         tmem_ld32(lane_addr + O_COL + c, o);
-        if (store) {
 #pragma unroll
-          for (int i = 0; i < 32; i += 4)
-            if (c + i < a.head_dim) *reinterpret_cast<float4*>(a.part_o + at * a.head_dim + c + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
-        }
+        for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4*>(orow + (c + i) * 4) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
       }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      if (store) {
+        asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(a.part_o + at * a.head_dim), "r"(smem_u32(orow)), "r"(a.head_dim * 4)
+                     : "memory");
+      }
+      asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+      asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }
   }
 
