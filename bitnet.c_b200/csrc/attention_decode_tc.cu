@@ -98,7 +98,8 @@ struct DtArgs {
   __nv_bfloat16* out;
   int out_stride;
   // with JOIN: what attention_shared.cu found for pages that a sequence shares with others
-  const int4* shared;     // per sequence: pages covered there (its first ones), the first of its results, their number
+  const int4* shared;     // per sequence: pages covered there (its first ones), the first of its results, their number; and of the sequences the one that
+                          // the blocks of this place take (those with the most pages of their own come first)
   const float* shared_o;  // [results][n_heads][head_dim], unnormalised
   const float* shared_ml; // [results][n_heads][2]: maximum and sum, as part_ml
   int n_shared;           // results that there are
@@ -179,6 +180,7 @@ attention_decode_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
     }
     b = item & 0xFFFF; zi = (item >> 16) & 0xFF; nz = (item >> 24) & 0x7F;
   }
+  if (JOIN) b = min(max(a.shared[b].w, 0), (int)gridDim.x - 1);
   const int g4 = lane >> 2, t4 = lane & 3;
   const int head_dim = a.head_dim, n_kv_heads = a.n_kv_heads, n_heads = a.n_heads;
   const int group = n_heads / n_kv_heads;
@@ -703,7 +705,8 @@ static long long dt_slots() {
 // sequences = 320 blocks: 77 us with three stages in two waves, 53 us with two stages in one).
 template <int HD, bool JOIN>
 static int launch_dt(const CUtensorMap& mk, const CUtensorMap& mv, const DtArgs& a, dim3 grid, dim3 cluster, cudaStream_t stream) {
-  if (a.pages_per_block <= 2) return launch_dt2<HD, 2, JOIN>(mk, mv, a, grid, cluster, stream);
+  // (with JOIN always two: a third block an SM gains more beside the shared pages' blocks; 64 sequences of up to 9 pages of their own: 38 us, 40 with three)
+  if (JOIN || a.pages_per_block <= 2) return launch_dt2<HD, 2, JOIN>(mk, mv, a, grid, cluster, stream);
   const long long blocks = (long long)grid.x * grid.y * grid.z;
   const long long s3 = dt_slots<HD, 3>(), s2 = dt_slots<HD, 2>();
   const long long w3 = (blocks + s3 - 1) / s3, w2 = (blocks + s2 - 1) / s2;

@@ -165,22 +165,22 @@ attention_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
       }
     }
   } else {
-    pdl_wait();
     // ---- the queries, into the layout that TMA would leave: boxes of 128 rows x 64 numbers, 16-byte pieces XORed with the row.  A thread copies one piece
-    // of every eighth (or fourth) row, all of its loads in flight before the first store.
+    // of every eighth (or sixteenth) row, all of its loads in flight before the first store; whose rows they are is known before the wait.
     {
       constexpr int PIECES = HD / 8, EACH = PIECES, APART = 128 / PIECES;
       const int t = tid - 64, c = t % PIECES, row0 = t / PIECES;
-      uint4 v[EACH];
+      int from[EACH];
 #pragma unroll
       for (int e = 0; e < EACH; ++e) {
-        const int row = row0 + e * APART;
-        v[e] = make_uint4(0u, 0u, 0u, 0u);
-        if (row < rows && c * 8 < a.head_dim) {
-          const int member = row / a.per_group, h = kvh * a.per_group + row - member * a.per_group;
-          v[e] = *reinterpret_cast<const uint4*>(a.q + (size_t)members[member].x * a.q_stride + (size_t)h * a.head_dim + c * 8);
-        }
+        const int row = row0 + e * APART, member = row / a.per_group;
+        from[e] = -1;
+        if (row < rows && c * 8 < a.head_dim) from[e] = members[member].x * a.q_stride + (kvh * a.per_group + row - member * a.per_group) * a.head_dim + c * 8;
       }
+      pdl_wait();
+      uint4 v[EACH];
+#pragma unroll
+      for (int e = 0; e < EACH; ++e) v[e] = from[e] >= 0 ? *reinterpret_cast<const uint4*>(a.q + from[e]) : make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
       for (int e = 0; e < EACH; ++e) {
         const int row = row0 + e * APART;
@@ -308,7 +308,7 @@ extern "C" int bn_attention_shared(const void* q, int q_stride, int n_seqs, int 
                                    int n_parts, int* status, cudaStream_t stream) {
   if (n_items <= 0 || n_seqs <= 0) return BN_OK;
   if (head_dim <= 0 || head_dim % 16 || head_dim > 128 || n_kv_heads <= 0 || n_heads % n_kv_heads || n_heads / n_kv_heads > AS_ROWS || !(scale > 0.f) ||
-      q_stride % 8 || n_items > 65535 || n_cache_pages <= 0 || !items || !members || !part_o || !part_ml || !status ||
+      q_stride % 8 || (long long)n_seqs * q_stride > 0x7fffffffll || n_items > 65535 || n_cache_pages <= 0 || !items || !members || !part_o || !part_ml || !status ||
       (((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)items | (uintptr_t)part_o) & 15) || (((uintptr_t)members | (uintptr_t)part_ml) & 7))
     return BN_ERR_BAD_ARG;
   CUtensorMap mk, mv;

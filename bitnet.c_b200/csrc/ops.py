@@ -1112,6 +1112,7 @@ class SharedPlan:
         self.device = torch.device(device)
         self.runs, self.first_own = shared_runs([p[:-1] for p in pages])  # the last page takes the new token: it is nobody else's
         self.own_pages = max((len(p) - f for p, f in zip(pages, self.first_own)), default=0)
+        self.lengths = [len(p) for p in pages]
         self.deepest = max(self.first_own, default=0)
         self._grid = None
         self.fits = self._lay_out(sms if sms is not None else n_sms(self.device), room)
@@ -1136,11 +1137,12 @@ class SharedPlan:
 
     def _lay_out(self, sms: int, room) -> bool:
         """The list of work, ``host``: items (first member, members, first page, pages), of every sequence (pages read together, first place of its
-        results, places, 0), and members (sequence, place)."""
+        results, places; and which sequence is the n-th by its own pages, the most first), and members (sequence, place)."""
         most = SHARED_ROWS // (self.n_heads // self.n_kv_heads)  # sequences of a block
         tiles = [(members[i:i + most], first, n) for members, first, n in self.runs for i in range(0, len(members), most)]
-        # two blocks fit an SM: as many as run at once share all pages evenly
-        budget = max(1, 2 * sms // self.n_kv_heads)
+        # one block an SM, which share all pages evenly: two would fit, but then the sequences' own pages wait until they have ended (8 prompts of 2,048 tokens by
+        # 8 sequences: 31 us with one, 37 with two; 64 sequences behind one of 8,192: 37 and 40)
+        budget = max(1, sms // self.n_kv_heads)
         longest = max((n for _m, _f, n in tiles), default=1)
         each = min(longest, max(SHARED_MIN_PAGES, -(-sum(n for _m, _f, n in tiles) // budget)))
         if room is not None:
@@ -1160,7 +1162,8 @@ class SharedPlan:
             place.append(at)
             at += c
         self.n_parts, self.n_items = at, len(work)
-        items, entries, sequences = [], [], [x for b in range(self.n_seqs) for x in (self.first_own[b], place[b], count[b], 0)]
+        order = sorted(range(self.n_seqs), key=lambda b: self.first_own[b] - self.lengths[b])
+        items, entries, sequences = [], [], [x for b in range(self.n_seqs) for x in (self.first_own[b], place[b], count[b], order[b])]
         for members, first, n in work:
             items += (len(entries) // 2, len(members), first, n)
             for b in members:

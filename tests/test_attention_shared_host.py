@@ -65,6 +65,9 @@ def look_over(plan, pages):
         assert sorted(got[b]) == list(range(place, place + n)) and place + n <= plan.n_parts
         assert sorted(x for piece in got[b].values() for x in piece) == list(range(first_own))
         assert first_own < len(pages[b]) and plan.own_pages >= len(pages[b]) - first_own
+    order = [s[3] for s in sequences]
+    own = [len(p) - f for p, f in zip(pages, plan.first_own)]
+    assert sorted(order) == list(range(len(pages))) and [own[b] for b in order] == sorted(own, reverse=True)
     # a run's members really share its pages, and nobody outside begins with them
     for members, first, n in plan.runs:
         begin = pages[members[0]][:first + n]
