@@ -35,8 +35,9 @@ def llamas(tmp_path_factory, cuda_device):
 
 @pytest.fixture
 def shared_calls(monkeypatch):
-    """How often attention over shared pages was launched."""
+    """How often attention over shared pages was launched; it is wherever pages are shared, also where so few that it does not pay."""
     calls, real = [], ops.attention_decode_shared
+    monkeypatch.setattr(ops, "shared_pays", lambda plan: bool(plan.runs))
     monkeypatch.setattr(ops, "attention_decode_shared", lambda *a, **k: (calls.append(1), real(*a, **k))[1])
     return calls
 
@@ -123,7 +124,7 @@ def test_filtered_completions_of_shared_pages(llamas, shared_calls, name, graphs
     assert eng.cache.tokens_free() == eng.cache.max_tokens
 
 
-def test_compaction_between_recorded_steps(llamas):
+def test_compaction_between_recorded_steps(llamas, shared_calls):
     model, _ = llamas["c", "bfloat16"]
     V = TINY_C["vocab_size"]
     got = []
