@@ -1099,10 +1099,9 @@ class SharedPlan:
     """Which sequences of a decode step share which pages, as ``attention_decode_shared`` takes it: made by ``shared_plan``, good while no sequence
     takes a new page (one that only fills its last page changes nothing).
 
-    ``first_own[b]``: so many of sequence b's first pages are read together with others'.  ``runs``: (sequences, first page, pages) of what is shared.
-    ``room`` = (items, places) pads the list of work to that size, for a recorded step whose list is data; ``fits`` is then false if it is too long for it."""
+    ``first_own[b]``: so many of sequence b's first pages are read together with others'.  ``runs``: (sequences, first page, pages) of what is shared."""
 
-    def __init__(self, pages, n_heads: int, n_kv_heads: int, head_dim: int, device, sms: Optional[int] = None, room=None):
+    def __init__(self, pages, n_heads: int, n_kv_heads: int, head_dim: int, device, sms: Optional[int] = None):
         if n_kv_heads <= 0 or n_heads % n_kv_heads or n_heads // n_kv_heads > SHARED_ROWS or head_dim % 16 or not 0 < head_dim <= 128:
             raise KernelError(f"shared_plan: heads {n_heads}/{n_kv_heads} of {head_dim} are not supported")
         if any(len(p) == 0 for p in pages):
@@ -1115,7 +1114,7 @@ class SharedPlan:
         self.lengths = [len(p) for p in pages]
         self.deepest = max(self.first_own, default=0)
         self._grid = None
-        self.fits = self._lay_out(sms if sms is not None else n_sms(self.device), room)
+        self._lay_out(sms if sms is not None else n_sms(self.device))
         self.table = None
 
     def upload(self, to: Optional[torch.Tensor] = None) -> "SharedPlan":
@@ -1135,7 +1134,18 @@ class SharedPlan:
             self._grid = self.own_pages, ((splits, each) if splits <= 8 else (8, -(-self.own_pages // 8)))
         return self._grid[1]
 
-    def _lay_out(self, sms: int, room) -> bool:
+    def pad(self, items: int, parts: int) -> "SharedPlan":
+        """Bring the list of work to a size, for a recorded step whose list is data: so many items, and places for results."""
+        if items < self.n_items or parts < self.n_parts:
+            raise KernelError(f"shared_plan: {self.n_items} items and {self.n_parts} results do not fit {items} and {parts}")
+        sequences, members = self.host[self.at[2]:self.at[1]], self.host[self.at[1]:]
+        self.host = (self.host[:self.at[2]] + [0] * (4 * (items - self.n_items)) + sequences  # items without members: nothing to do
+                     + members + [0] * (2 * (parts - self.n_parts)))
+        self.at = (0, 4 * items + len(sequences), 4 * items)
+        self.n_items, self.n_parts = items, parts
+        return self
+
+    def _lay_out(self, sms: int) -> None:
         """The list of work, ``host``: items (first member, members, first page, pages), of every sequence (pages read together, first place of its
         results, places; and which sequence is the n-th by its own pages, the most first), and members (sequence, place)."""
         most = SHARED_ROWS // (self.n_heads // self.n_kv_heads)  # sequences of a block
@@ -1145,9 +1155,6 @@ class SharedPlan:
         budget = max(1, sms // self.n_kv_heads)
         longest = max((n for _m, _f, n in tiles), default=1)
         each = min(longest, max(SHARED_MIN_PAGES, -(-sum(n for _m, _f, n in tiles) // budget)))
-        if room is not None:
-            while each < longest and (sum(-(-n // each) for _m, _f, n in tiles) > room[0] or sum(-(-n // each) * len(m) for m, _f, n in tiles) > room[1]):
-                each = min(longest, 2 * each)
         work = []
         for members, first, n in tiles:
             pieces = -(-n // each)
@@ -1169,15 +1176,8 @@ class SharedPlan:
             for b in members:
                 entries += (b, place[b])
                 place[b] += 1
-        if room is not None:
-            if self.n_items > room[0] or self.n_parts > room[1]:
-                return False
-            items += [0] * (4 * (room[0] - self.n_items))  # items without members: nothing to do
-            entries += [0] * (2 * (room[1] - self.n_parts))
-            self.n_items, self.n_parts = room
         self.host = items + sequences + entries  # (rows of four first: they are read 16 bytes at a time)
         self.at = (0, len(items) + len(sequences), len(items))  # items, members, sequences
-        return True
 
 
 def shared_runs(pages):

@@ -28,7 +28,12 @@ from ..sampling import Sampler
 from .batch import StepContext
 
 
-SHARED_PLACES = 24  # results of shared pages per sequence that a recorded step has room for (ops.SharedPlan cuts its runs into fewer pieces to fit)
+def _bucket(n: int) -> int:
+    """The smallest of 4, 6, 8, 12, 16, 24, ... that is at least ``n``."""
+    size = 4
+    while size < n:
+        size = size * 3 // 2 if size & (size - 1) == 0 else size * 4 // 3
+    return size
 
 
 class DecodeRunner:
@@ -56,15 +61,12 @@ class DecodeRunner:
         self.host_items: Optional[List[int]] = None  # what the device buffer holds
         self.items_for = None  # (bucket, page counts) that ``next_items`` was made for
         self.next_items: List[int] = []
-        # Sequences that share pages: what is shared is data in a buffer of fixed size (``ops.SharedPlan``), the longest run of own
-        # pages a bucket like that of the lengths.
-        heads = model.shared_heads()
-        self.shared_room = None
-        if heads is not None:
-            self.shared_room = (2 * ops.n_sms(dev) // heads[0][1] + B, SHARED_PLACES * B)
-            self.shared_table = torch.zeros(4 * self.shared_room[0] + 4 * B + 2 * self.shared_room[1], dtype=torch.int32, device=dev)
-        self.shared_for = None  # (slots, page counts, the cache's turns) that ``ctx.shared`` was made for
-        self.graphs = {}  # (length bucket, bucket of own pages where pages are shared) -> recorded graph
+        # Sequences that share pages: what is shared is data (``ops.SharedPlan``), the length of its list and the longest run of own pages are
+        # buckets like that of the lengths.
+        self.can_share = model.shared_heads() is not None
+        self.shared_tables = {}  # bucket -> its buffer, which its recordings point at, and what the buffer holds
+        self.shared_for = None  # (slots, the cache's turns) that ``ctx.shared`` was made for
+        self.graphs = {}  # (length bucket, buckets of the shared pages' list and of own pages, or None) -> recorded graph
         self.pool = pool
         self.warmed = set()  # whether a step with and without shared pages has run
         self.host_slots: Optional[List[int]] = None
@@ -107,7 +109,7 @@ class DecodeRunner:
             self.launches_per_step[kind] = ops.LAUNCHES - before
             self.warmed.add(kind)
         else:
-            key = (self.ctx.max_len, self.ctx.shared.own_pages if kind else 0)
+            key = (self.ctx.max_len, (self.ctx.shared.n_items, self.ctx.shared.n_parts, self.ctx.shared.own_pages) if kind else None)
             g = self.graphs.get(key)
             if g is None:
                 g = torch.cuda.CUDAGraph()
@@ -124,25 +126,33 @@ class DecodeRunner:
         return self.sampled
 
     def _shared_pages(self, slots: Sequence[int], positions: Sequence[int]) -> None:
-        """Bring what the sequences share up to date: it changes when one of them takes a new page, and when one is forked or ends."""
-        if self.shared_room is None:
+        """Bring what the sequences share up to date: it changes when one is forked or ends.  (One that takes a new page of its own changes the longest run of
+        those only.)"""
+        if not self.can_share:
             return
-        now = (slots, [p // PAGE + 1 for p in positions], self.cache.turns) if self.cache.shares_pages() else None
-        if now == self.shared_for:
-            return
-        self.shared_for = now
-        before, self.ctx.shared = self.ctx.shared, None
-        plan = self.model.shared_pages(self.cache, slots, positions, room=self.shared_room) if now is not None else None
-        if plan is not None:
-            bucket = 4
-            while bucket < plan.own_pages:
-                bucket *= 2
-            plan.own_pages = bucket
-            if before is None or before.host != plan.host:
-                self.h2d_bytes += 4 * len(plan.host)
-                plan.upload(self.shared_table)
-            plan.table = self.shared_table
-            self.ctx.shared = plan
+        now = (slots, self.cache.turns) if self.cache.shares_pages() else None
+        if now != self.shared_for:
+            self.shared_for = now
+            self.ctx.shared = self._shared_plan(slots, positions) if now is not None else None
+        if self.ctx.shared is not None:
+            own = max(p // PAGE + 1 - first for p, first in zip(positions, self.ctx.shared.first_own))
+            self.ctx.shared.own_pages = _bucket(own)
+
+    def _shared_plan(self, slots: Sequence[int], positions: Sequence[int]):
+        plan = self.model.shared_pages(self.cache, slots, positions)
+        if plan is None:
+            return None
+        plan.pad(_bucket(plan.n_items), _bucket(plan.n_parts))
+        size = plan.n_items, plan.n_parts
+        table, held = self.shared_tables.get(size, (None, None))
+        if table is None:
+            table = torch.zeros(len(plan.host), dtype=torch.int32, device=self.model.device)
+        if held != plan.host:
+            self.h2d_bytes += 4 * len(plan.host)
+            plan.upload(table)
+            self.shared_tables[size] = table, plan.host
+        plan.table = table
+        return plan
 
     def _work_list(self, positions: Sequence[int]) -> None:
         """Bring the work list of this step's bucket up to date (the grid's shape was fixed when the

@@ -113,15 +113,15 @@ class Model:
                 return heads, i
         return None
 
-    def shared_pages(self, cache: Cache, slots: Sequence[int], lengths: Sequence[int], room=None):
+    def shared_pages(self, cache: Cache, slots: Sequence[int], lengths: Sequence[int]):
         """For a decode step of these sequences (``lengths``: before it): the plan of what they share, not yet on the device, or None if that is nothing, too
         little to pay, or nothing that a mixer of this model can make use of."""
         found = self.shared_heads() if cache.shares_pages() and ops.USE_SHARED_PAGES else None
         if found is None:
             return None
         heads, entry = found
-        plan = ops.SharedPlan([cache.pages_of(entry, s, n // PAGE + 1) for s, n in zip(slots, lengths)], *heads, self.device, room=room)
-        return plan if plan.fits and ops.shared_pays(plan) else None
+        plan = ops.SharedPlan([cache.pages_of(entry, s, n // PAGE + 1) for s, n in zip(slots, lengths)], *heads, self.device)
+        return plan if ops.shared_pays(plan) else None
 
     def kernel_families(self) -> List[str]:
         # (a model in bfloat16 may have parameters that stay float32: their products of many rows are linear_split's)

@@ -49,13 +49,11 @@ def test_every_shared_page_is_read_once_for_every_sequence(heads, kv, seed):
     plan = ops.SharedPlan(pages, heads, kv, 64, "cpu", sms=148)
     look_over(plan, pages)
     # a list of fixed size for a recorded step
-    padded = ops.SharedPlan(pages, heads, kv, 64, "cpu", sms=148, room=(plan.n_items + 5, plan.n_parts + 9))
-    assert padded.fits and len(padded.host) == 4 * (plan.n_items + 5) + 4 * len(pages) + 2 * (plan.n_parts + 9)
-    assert padded.runs == plan.runs and [x for x in padded.host if x] == [x for x in plan.host if x]
-    tight = ops.SharedPlan(pages, heads, kv, 64, "cpu", sms=148, room=(max(1, plan.n_items // 2), max(1, plan.n_parts // 2)))
-    if tight.fits and plan.runs:
-        look_over(tight, pages)
-    assert not plan.runs or not ops.SharedPlan(pages, heads, kv, 64, "cpu", sms=148, room=(4096, 1)).fits
+    items, parts = plan.n_items, plan.n_parts
+    assert len(plan.pad(items + 5, parts + 9).host) == 4 * (items + 5) + 4 * len(pages) + 2 * (parts + 9)
+    look_over(plan, pages)
+    with pytest.raises(ops.KernelError, match="do not fit"):
+        plan.pad(items, parts)
 
 
 def look_over(plan, pages):

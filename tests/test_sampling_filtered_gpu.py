@@ -129,11 +129,41 @@ def test_own_generators(cuda_device):
         assert got == want and dev.tolist() == host
 
 
-def test_more_numbers_than_a_cluster_holds(cuda_device):
-    # 8 blocks hold 409,600 numbers: a longer row is read anew in each pass
-    logits, u = rows(2, 500009, 2.0, 11)
+@pytest.mark.parametrize("vocab", [500009, 600011])
+def test_more_numbers_than_blocks_hold_or_add_up(cuda_device, vocab):
+    # 8 blocks hold 430,000 float32 numbers, a longer row is read anew in each pass; from 520,000 on borders are found by the bits of the keys
+    logits, u = rows(2, vocab, 2.0, 11)
     check(logits, 1.0, 0, 0.9, 0.0, u, cuda_device)
     check(logits, 0.7, 300, 0.9, 0.01, u, cuda_device)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_many_rows_stay_in_memory_between_passes(cuda_device, dtype):
+    # one block a row, rows too long to be held; rows that do not begin on 16 bytes
+    n, vocab = 310, 40007
+    logits, u = rows(n, vocab, 2.0, 14, dtype)
+    g = torch.Generator().manual_seed(15)
+    top_k = torch.where(torch.rand(n, generator=g) < 0.5, torch.randint(1, 3000, (n,), generator=g), torch.zeros(n, dtype=torch.int64)).int()
+    top_p = torch.rand(n, generator=g)
+    check(logits, 0.8, top_k, top_p, 0.001, u, cuda_device)
+
+
+def test_rows_with_most_tokens_masked(cuda_device):
+    # a grammar leaves a few of many tokens; the others are -inf, or the lowest number
+    n, vocab = 24, 60000
+    logits, u = rows(n, vocab, 2.0, 16)
+    keep = torch.rand(n, vocab, generator=torch.Generator().manual_seed(17)) < 2e-3
+    for mask in (float("-inf"), torch.finfo(torch.float32).min):
+        masked = torch.where(keep, logits, torch.full((), mask))
+        for case in [(0.8, 0, 1.0, 0.0), (0.8, 50, 0.9, 0.0), (1.2, 500, 1.0, 0.0), (1.0, 0, 0.95, 0.01), (0.9, 59999, 0.9, 0.0)]:
+            check(masked, *case, u, cuda_device)
+
+
+def test_weights_far_apart(cuda_device):
+    # logits that span thousands of units: nearly all weights vanish, top-k and min-p reach into what weighs nothing
+    logits, u = rows(16, 30000, 400.0, 18)
+    for case in [(1.0, 0, 1.0, 0.0), (1.0, 200, 0.9999, 0.0), (0.3, 0, 1.0, 1e-25), (5.0, 3000, 1.0, 1e-9), (30.0, 0, 0.99, 0.0)]:
+        check(logits, *case, u, cuda_device)
 
 
 def test_in_a_graph_and_on_two_streams(cuda_device):
