@@ -124,7 +124,6 @@ attention_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
     }
   } else if (warp == 1) {
     pdl_wait();
-    pdl_launch_dependents();  // behind the wait: what the next kernel reads of this one's predecessor is then there
     // the whole warp walks the loop, one elected lane issues
     const bool issuer = elect_one();
     const unsigned tbase = __shfl_sync(0xffffffffu, tmem_base, 0);
@@ -190,6 +189,9 @@ attention_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncwarp();
     if (lane == 0) mbar_arrive(q_full);
+    // behind the wait, so that what the next kernel reads of this one's predecessor is there; and behind the queries, so that they do not queue
+    // behind the pages that it asks for
+    pdl_launch_dependents();
     // ---- softmax: thread <-> row <-> lane of tensor memory
     const int quad = warp & 3, r = quad * 32 + lane;
     const unsigned lane_addr = tmem_base + ((unsigned)(quad * 32) << 16);
