@@ -72,12 +72,13 @@ __global__ void __launch_bounds__(CP_THREADS) copy_pages_kernel(const __grid_con
   __threadfence();
 }
 
-// moves: n_groups times (source page, rows, number of destinations); dst: their destinations, group by group.  A destination is no
+// groups: n_groups times (source page, rows, number of destinations), then their n_dst destinations, group by group.  A destination is no
 // group's source and no other's destination.  k (and v, or null): [planes, pages, heads, 64, row bytes].
 extern "C" int bn_copy_pages(void* k, void* v, int planes, int pages, int heads, int k_row, int v_row, const int* groups, int n_groups,
-                             const int* dst, int n_dst, cudaStream_t stream) {
+                             int n_dst, cudaStream_t stream) {
   if (n_groups <= 0) return BN_OK;
-  if (!k || !groups || !dst || planes <= 0 || pages <= 0 || heads <= 0 || k_row <= 0 || (v && v_row <= 0)) return BN_ERR_BAD_ARG;
+  const int* dst = groups ? groups + 3 * (size_t)n_groups : nullptr;
+  if (!k || !groups || planes <= 0 || pages <= 0 || heads <= 0 || k_row <= 0 || (v && v_row <= 0)) return BN_ERR_BAD_ARG;
   const int sides = v ? 2 : 1;
   if ((long long)planes * sides > 65535 || (long long)heads * BN_PAGE * (k_row > v_row ? k_row : v_row) > 0x7fffffffll) return BN_ERR_BAD_ARG;
   long long all = 0;

@@ -1125,7 +1125,13 @@ class SharedPlan:
         self.table = host.to(self.device, non_blocking=True) if to is None else to
         if to is not None:
             to[:host.numel()].copy_(host, non_blocking=True)
+        self.point_at(self.table)
         return self
+
+    def point_at(self, table: torch.Tensor) -> None:
+        """The list of work is in ``table``."""
+        self.table = table
+        self.pointers = tuple(c_void_p(table.data_ptr() + 4 * i) for i in self.at)  # items, members, sequences
 
     def own_grid(self):
         """``decode_grid`` of the sequences' own pages, at most 8 blocks a sequence: those are one cluster and share no workspace with other launches."""
@@ -1259,8 +1265,7 @@ def attention_decode_shared(qkv: torch.Tensor, k_off: int, v_off: int, out: torc
         results = plan.n_parts * n_heads
         room = torch.empty(results * (head_dim + 2), dtype=torch.float32, device=device)
         shared_o, shared_ml = c_void_p(room.data_ptr()), c_void_p(room.data_ptr() + 4 * results * head_dim)
-        table = plan.table.data_ptr()
-        items, members, sequences = (c_void_p(table + 4 * i) for i in plan.at)
+        items, members, sequences = plan.pointers
         status, stream, f_scale = _tc_status_arg(device), _stream(), c_float(scale)
         p_qkv, p_pos, p_slots, p_table, p_k, p_v = _ptr(qkv), _ptr(tok_pos), _ptr(slots), _ptr(page_table), _ptr(k_cache), _ptr(v_cache)
         pages, width = k_cache.shape[0], page_table.shape[1]
@@ -1806,16 +1811,20 @@ def zero_slot(rows: torch.Tensor, slot: int) -> None:
 def _page_moves(moves, pages: int):
     """``copy_pages``' moves as the kernel takes them: groups of (source, rows, number of destinations) and their destinations; refuses what does not
     name pages of the cache, and destinations that another move reads or writes."""
-    groups, sources = {}, set()
+    groups = {}
     for src, dst, rows in moves:
         if not (0 <= src < pages and 0 <= dst < pages):
             raise KernelError(f"copy_pages: page {src if not 0 <= src < pages else dst} is outside the {pages} pages of the cache")
         if not 0 < rows <= PAGE:
             raise KernelError(f"copy_pages: {rows} rows of a page of {PAGE}")
-        groups.setdefault((src, rows), []).append(dst)
-        sources.add(src)
+        to = groups.get((src, rows))
+        if to is None:
+            groups[src, rows] = [dst]
+        else:
+            to.append(dst)
     to = [d for g in groups.values() for d in g]
-    if len(set(to)) != len(to) or not sources.isdisjoint(to):
+    written = set(to)
+    if len(written) != len(to) or any(src in written for src, _rows in groups):
         raise KernelError("copy_pages: a page that is written must be written once and not read")
     return [x for (src, rows), dst in groups.items() for x in (src, rows, len(dst))], to
 
@@ -1825,22 +1834,27 @@ def copy_pages(k: torch.Tensor, v: Optional[torch.Tensor], moves) -> None:
     all planes, of keys and of values.  ``k`` [planes, pages, heads, 64, numbers] of any type, ``v`` the same with a width of its own, or None;
     ``moves`` is a sequence on the host, read before the call returns.  A page that is written is written once and not read."""
     _need(k, "k", dims=5)
-    if k.shape[3] != PAGE:
+    planes, pages, heads, page, dim = k.shape
+    if page != PAGE:
         raise KernelError(f"copy_pages: k {tuple(k.shape)} is not [planes, pages, heads, {PAGE}, numbers]")
+    both = [(k, heads, dim, None, 0)]
     if v is not None:
         _need(v, "v", dims=5)
-        if v.shape[:2] != k.shape[:2] or v.shape[3] != PAGE or v.device != k.device:
+        v_planes, v_pages, v_heads, v_page, v_dim = v.shape
+        if v_planes != planes or v_pages != pages or v_page != PAGE or v.get_device() != k.get_device():
             raise KernelError(f"copy_pages: v {tuple(v.shape)} on {v.device} does not go with k {tuple(k.shape)} on {k.device}")
-    groups, to = _page_moves(moves, k.shape[1])
-    if not to or 0 in k.shape:
-        return
-    g, d = (c_int * len(groups))(*groups), (c_int * len(to))(*to)
-    with _on(k.device):
         # keys and values with different numbers of heads are copied one after the other
-        for one, other in ([(k, v)] if v is None or v.shape[2] == k.shape[2] else [(k, None), (v, None)]):
-            _check(_fn("cache_pages", "bn_copy_pages")(
-                _ptr(one), _ptr(other), int(one.shape[0]), int(one.shape[1]), int(one.shape[2]), int(one.shape[4] * one.element_size()),
-                int(other.shape[4] * other.element_size()) if other is not None else 0, g, len(groups) // 3, d, len(to), _stream()), "copy_pages")
+        both = [(k, heads, dim, v, v_dim)] if v_heads == heads and dim and v_dim else [*both, (v, v_heads, v_dim, None, 0)]
+    groups, to = _page_moves(moves, pages)
+    if not to:
+        return
+    n, listed = len(groups) // 3, (c_int * (len(groups) + len(to)))(*groups, *to)
+    with _on(k.device):
+        for one, h, width, other, other_width in both:
+            if planes and h and width:
+                _check(_fn("cache_pages", "bn_copy_pages")(
+                    _ptr(one), _ptr(other), planes, pages, h, width * one.element_size(), other_width * other.element_size() if other is not None else 0,
+                    listed, n, len(to), _stream()), "copy_pages")
 
 
 class StateSlots:

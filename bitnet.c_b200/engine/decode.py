@@ -151,7 +151,7 @@ class DecodeRunner:
             self.h2d_bytes += 4 * len(plan.host)
             plan.upload(table)
             self.shared_tables[size] = table, plan.host
-        plan.table = table
+        plan.point_at(table)
         return plan
 
     def _work_list(self, positions: Sequence[int]) -> None:
