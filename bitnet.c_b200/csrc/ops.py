@@ -1164,6 +1164,8 @@ class SharedPlan:
         work = []
         for members, first, n in tiles:
             pieces = -(-n // each)
+            if pieces > 8:  # the join has eight results in flight: no round of it for a few
+                pieces -= pieces % 8
             work += [(members, first + n * i // pieces, n * (i + 1) // pieces - n * i // pieces) for i in range(pieces)]
         work.sort(key=lambda w: -w[2])  # the longest start first
         count = [0] * self.n_seqs
