@@ -159,10 +159,12 @@ class KvGroup:
         return [(part, p, rest) for p in own]
 
     def compact(self) -> List[Tuple[int, int, int]]:
-        """Renumber the held pages so that they are the first ones; returns what is to be copied."""
+        """Renumber the held pages so that they are the first ones, and copy those that move; returns what was copied."""
         held = sorted({p for h in self.held.values() for p in h.values()})
         gaps = [p for p in range(len(held)) if not self.pool.holders(p)]
         moved = dict(zip([p for p in held if p >= len(held)], gaps))
+        moves = [(old, new, PAGE) for old, new in moved.items()]
+        self.copy(moves)  # in front of the bookkeeping: a copy that is refused changes nothing
         if moved:
             self.pool.renumber({p: moved.get(p, p) for p in held})
             for slot, h in self.held.items():
@@ -170,7 +172,7 @@ class KvGroup:
                     if p in moved:
                         h[i] = self.host_table[slot, i] = moved[p]
                         self.dirty.add(slot)
-        return [(old, new, PAGE) for old, new in moved.items()]
+        return moves
 
     def copy(self, moves: List[Tuple[int, int, int]]) -> None:
         if moves and self.k is not None:
@@ -270,7 +272,7 @@ class Cache:
     def fork(self, slot: int, n: int = 1) -> List[int]:
         """``n`` new sequences that go on from where the one in ``slot`` is: their slots.  They share its full pages (a page is free again when
         its last holder has given it back); the rows of its last page, if that is not full, and its states are copied, in one launch
-        for every group of runs and one for all states.  If the slots or pages for them are not there, nothing has changed."""
+        for every group of runs and one for all states.  If the slots or pages for them are not there, or a copy is refused, nothing has changed."""
         length = self.slots.length(slot)  # raises if not open
         if n < 1:
             raise CacheError(f"a sequence is forked into at least one, not {n}")
@@ -278,33 +280,27 @@ class Cache:
             raise CacheFull(f"{n} slots wanted, {self.slots.n_free} of {self.slots.n_slots} free")
         new = [self.slots.open() for _ in range(n)]
         try:
-            moves = [g.fork(slot, length, new) for g in self.groups]
-        except CacheFull:
-            for s in new:
+            for g, moves in [(g, g.fork(slot, length, new)) for g in self.groups]:
+                g.copy(moves)
+            if self.states:
+                from ..csrc import ops
+                if self._state_slots is None:
+                    self._state_slots = ops.StateSlots(self.states.values())
+                ops.copy_slots(self._state_slots, slot, new)
+        except BaseException:
+            for s in reversed(new):  # (the free slots are in their order again)
                 self.close(s)
             raise
         for s in new:
             self.slots.set_length(s, length)
         self.turns += 1
-        for g, m in zip(self.groups, moves):
-            g.copy(m)
-        if self.states:
-            from ..csrc import ops
-            if self._state_slots is None:
-                self._state_slots = ops.StateSlots(self.states.values())
-            ops.copy_slots(self._state_slots, slot, new)
         return new
 
     def compact(self) -> int:
         """Move pages so that the held ones of each group are its first, ``g.k[:, :n]`` and ``g.v[:, :n]`` for ``n`` of them: what is to be saved, or
         sent elsewhere, is then one slice.  Returns the number of pages that were moved.  Sequences keep their slots, what they hold and whom
         they share it with; recorded steps stay valid (page tables are data)."""
-        moved = 0
-        for g in self.groups:
-            moves = g.compact()
-            g.copy(moves)
-            moved += len(moves)
-        return moved
+        return sum(len(g.compact()) for g in self.groups)
 
     def close(self, slot: int) -> None:
         """The sequence has ended: its pages and its slot are free for the next one."""

@@ -137,3 +137,38 @@ def test_a_pool_counts_its_holders():
     with pytest.raises(CacheError, match="shared"):
         p.share([a])
     p.check()
+
+
+@pytest.mark.parametrize("states", [False, True])
+def test_a_copy_that_is_refused_changes_nothing(states):
+    """(On the CPU every copy is.)"""
+    from bitnet_c_b200.parts import StateRequest
+    c = Cache([KvRequest(2, 16)], [None], [StateRequest((3,), torch.float32) if states else None], 640, 512, torch.bfloat16, torch.device("cpu"), max_seqs=6)
+    g = c.groups[0]
+    a, b = c.open(), c.open()
+    put(c, a, 128 if states else 100)
+    put(c, b, 10)
+    c.close(a)
+    a = c.open()
+    put(c, a, 130)
+    put(c, b, 60)
+    c.close(a)
+    a = c.open()
+    put(c, a, 128 if states else 100)
+
+    def facts():
+        return {s: dict(h) for s, h in g.held.items() if h}, g.pool.n_free, c.slots.n_free, c.slots.active(), [c.length(s) for s in c.slots.active()]
+    before = facts()
+    with pytest.raises(ops.KernelError, match="CUDA"):
+        c.fork(a, 2)
+    assert facts() == before
+    c.check()
+    g.pool.alloc(1)
+    c.close(a)
+    a = c.open()
+    put(c, a, 300)
+    c.close(b)
+    before = facts()
+    with pytest.raises(ops.KernelError, match="CUDA"):
+        c.compact()
+    assert facts() == before
