@@ -2846,7 +2846,8 @@ def sample_filtered(logits: torch.Tensor, temperature, top_k=0, top_p=1.0, min_p
     the ones of at least ``min_p`` times the largest weight; then the first whose running sum exceeds u times the sum of what is left.  A
     temperature of 0 takes the first maximum; where there are logits of +inf, they share everything equally.
     Each parameter is a number or a tensor with one per row (``top_k`` int32, the others float32; numbers are rounded to float32).
-    The random numbers are ``u`` [rows] in [0, 1), or row r draws from (and advances) the xorshift64* state ``rng_state[index[r]]`` (or [r])."""
+    The random numbers are ``u`` [rows] in [0, 1), or row r draws from (and advances) the xorshift64* state ``rng_state[index[r]]`` (or [r]; no
+    two rows one state)."""
     _need_rows(logits, "logits")
     n, vocab = logits.shape
     device = logits.device

@@ -881,7 +881,7 @@ __global__ void __launch_bounds__(SF_THREADS, 1024 / SF_THREADS) sample_filtered
     while (row.fine < 5 && octaves * (float)(64 << row.fine) < (float)(SF_STEPS - 2)) ++row.fine;
     row.steps = (float)(32 << row.fine);
     const bool k_on = top_k > 0 && top_k < a.vocab, p_on = top_p > 0.f && top_p < 1.f, m_on = min_p > 0.f;
-      bool by_bits = row.infinite || !(c > 1e-30 && c < 1e30) || a.per > SF_COUNTED;
+    bool by_bits = row.infinite || !(c > 1e-30 && c < 1e30) || a.per > SF_COUNTED;
     if (!by_bits) {
       row.count_steps(k_on);
       sf_sync(blocks);

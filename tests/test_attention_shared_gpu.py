@@ -194,3 +194,46 @@ def test_refused(cuda_device):
                    dict(tok_pos=b.tok_pos.long()), dict(v_cache=b.v.cpu())):
         with pytest.raises(ops.KernelError):
             call(**change)
+
+
+def test_two_calls_at_once(cuda_device):
+    a, b = Batch(*forked(2, 16, 64 * 40, [0, 300]), 32, 8, 128, cuda_device), Batch(*forked(1, 40, 64 * 30, [5, 64 * 9]), 32, 8, 128, cuda_device, seed=4)
+    plans = [x.plan() for x in (a, b)]
+    want = [x.check(p).clone() for x, p in zip((a, b), plans)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for x in (a, b):
+            x.out.zero_()
+        for s in streams:
+            s.wait_stream(torch.cuda.current_stream())
+        for s, x, p in zip(streams, (a, b), plans):
+            with torch.cuda.stream(s):
+                x.run(p)
+        torch.cuda.synchronize()
+        assert all(torch.equal(x.out, w) for x, w in zip((a, b), want))
+
+
+def test_no_sequence(cuda_device):
+    b = Batch(*forked(1, 3, 192, [4]), 4, 2, 64, cuda_device)
+    plan = ops.shared_plan([], 4, 2, 64, cuda_device)
+    before = b.k.clone()
+    out = ops.attention_decode_shared(b.qkv[:0], 256, 384, b.out[:0], 0, 4, 2, 64, 0.1, b.tok_pos[:0], b.slots[:0], b.table, b.k, b.v, plan)
+    assert out.shape == (0, 256) and torch.equal(b.k.view(torch.int16), before.view(torch.int16))
+
+
+def test_a_cache_behind_the_reach_of_32_bits(cuda_device):
+    # 2^31 numbers of keys and as many of values in front of the pages
+    pages, pos = forked(1, 5, 64 * 3, [7, 64])
+    b = Batch(pages, pos, 4, 1, 128, cuda_device)
+    far = (1 << 31) // (PAGE * 128) + 3
+    k, v = (torch.empty((far + b.k.shape[0], 1, PAGE, 128), dtype=torch.bfloat16, device=cuda_device) for _ in range(2))
+    k[far:], v[far:] = b.k, b.v
+    b.k, b.v = k, v
+    b.pages = [[p + far for p in row] for row in pages]
+    b.table = torch.where(b.table >= 0, b.table + far, b.table)
+    got = b.run(b.plan())
+    small = Batch(pages, pos, 4, 1, 128, cuda_device)
+    want = small.check()
+    assert torch.equal(got, want)
+    assert torch.equal(k[far:].view(torch.int16), small.k.view(torch.int16)) and torch.equal(v[far:].view(torch.int16), small.v.view(torch.int16))

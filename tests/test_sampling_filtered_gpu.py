@@ -197,3 +197,12 @@ def test_shares_of_many_draws(cuda_device):
     for t in kept:
         assert abs((got == t).sum() - n * w[t] / w[kept].sum()) <= 1.0
     assert set(got.tolist()) <= set(kept.tolist())
+
+
+def test_more_rows_than_16_bits_count(cuda_device):
+    x = torch.randn((70001, 50), generator=torch.Generator().manual_seed(2)).to(cuda_device)
+    u = torch.rand(70001, generator=torch.Generator().manual_seed(3)).to(cuda_device)
+    assert torch.equal(ops.sample_filtered(x, 0.8, top_k=1, u=u), x.argmax(1).int())
+    k = torch.randint(1, 4, (70001,), generator=torch.Generator().manual_seed(4)).int().to(cuda_device)
+    got = ops.sample_filtered(x, 1e-6, top_k=k, u=torch.full_like(u, 0.999))  # (the first two logits of a row may be as good as equal)
+    assert (x.gather(1, got[:, None].long())[:, 0] >= x.amax(1) - 2e-5).all()
