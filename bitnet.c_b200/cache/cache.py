@@ -10,7 +10,7 @@ own storage, page pool and page table, so runs with different needs never share 
     page_table    [slots, pages_per_sequence]  int32, on the device and mirrored on the host
 
 A sequence lives in a *slot* from its first token to its end and holds, in each group, the
-pages its length needs; a group with a window gives pages back as soon as they lie wholly
+pages its length needs (a forked one shares the full ones with what it was forked from); a group with a window gives pages back as soon as they lie wholly
 before the window, except the pages of the first ``keep_first`` positions when the request asks to
 keep those.  A run that reads another run's cache (``cache_of``) gets a view of that
 run's plane and writes nothing; what the owner's group keeps is then the union of what the owner

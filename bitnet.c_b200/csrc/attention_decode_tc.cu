@@ -26,6 +26,9 @@
 // split size only.  Head sizes in steps of 16 run on the instantiation for 64, 128 or 256 with the
 // missing dimensions zero in shared memory.
 //
+// JOIN (several sequences share their first pages, which attention_shared.cu reads once for all of them): the same walk over a sequence's other pages
+// beside that kernel, the rows already rotated; what it found is read at the end and joined by the largest maximum.  Two stages, up to eight splits.
+//
 // Reference: scores = q.k * scale over the causal range, softmax with the maximum subtracted,
 // weighted sum of values, query head h uses key/value head h / (H / KV)
 // (src/transformer/gqa_scalar.c:61-121; online form gqa_scalar.c:127-207); rotary pairs

@@ -12,6 +12,10 @@
 // results go).  Blocks and roles as in attention_prefill_tc.cu: warp 0 requests pages (TMA, 128-byte swizzle), warp 1 issues the MMAs,
 // S of the next page ahead of P V of this one, warps 2 to 5 copy the queries into shared memory and do the softmax, one row per thread.
 // P goes back to tensor memory over the columns S came from.  Every wait is bounded; a block whose wait gave up records it and stores nothing.
+//
+// A page takes a block about 0.8 us (its products, 17 % of the tensor cores' cycles, and its softmax follow one another); the list of work spreads the pages over one
+// block an SM, beside which the blocks of the sequences' own pages run.  Both kernels together, 32 heads on 8 of 128: 64 sequences behind 8,192 tokens with 500 of
+// their own 37 us (234 where each reads all its pages), 8 prompts of 2,048 by 8 with 300 of their own 31 us.
 #include "tma.cuh"
 #include "umma.cuh"
 
@@ -322,7 +326,7 @@ extern "C" int bn_attention_shared(const void* q, int q_stride, int n_seqs, int 
   a.per_group = n_heads / n_kv_heads; a.scale_log2e = scale * 1.4426950408889634f; a.items = (const int4*)items; a.members = (const int2*)members;
   a.n_members = n_members; a.n_parts = n_parts; a.slots = slots; a.page_table = page_table; a.pt_stride = pt_stride; a.part_o = part_o;
   a.part_ml = part_ml; a.status = status;
-  // 64 KB and 96 KB: two blocks share an SM (tensor memory allows no more), one's softmax beside the other's products
+  // 64 KB and 96 KB: room for blocks of the sequences' own pages on the same SM (rings of three pages at head size 128: 36 and 40 us, 36 and 39 with two)
   if (head_dim <= 64) return as_launch<64, 3, 3>(mk, mv, a, n_items, stream);
   return as_launch<128, 2, 2>(mk, mv, a, n_items, stream);
 }
