@@ -23,9 +23,8 @@
 
 #define SF_THREADS 512
 #define SF_BINS 2048     // of a histogram of bits
-#define SF_STEPS 2048    // of the counts by weight: 64 octaves of 32 steps; the last one's keys weigh nothing
+#define SF_STEPS 2048    // of the counts by weight: 64 octaves of 32 steps; the last one's keys weigh nothing (and are not counted)
 #define SF_LIST 2048     // keys that the first block may be handed
-#define SF_FEW 128       // so many of them are one warp's work
 #define SF_COUNTED 65000 // keys of a block whose weights' halves add up in 32 bits whatever their steps
 #define SF_POINT 56      // a weight of 1 is 2^56 while a thread adds up its own (at most 2^7 of them)
 #define SF_MAX_CLUSTER 8
@@ -121,7 +120,7 @@ struct SfShared {
     unsigned long long hist[SF_BINS];
     struct {
       // of a step's keys their number, in two parts; or the sum of their weights in parts of 2^-31 of its largest, upper and lower 16 bits apart
-      unsigned one[SF_STEPS + 32], two[SF_STEPS + 32];  // (what -inf brings goes behind the last step, for each lane apart)
+      unsigned one[SF_STEPS], two[SF_STEPS];
     };
     unsigned long long list[SF_LIST];  // keys falling, equal ones by index: (~key, index)
   };
@@ -139,8 +138,7 @@ struct SfShared {
   unsigned long long warp4[SF_THREADS / 32][4];
   unsigned long long got[4];
   int steps[8];
-  unsigned long long base[4], sum[2];
-  int at[4];
+  int place;  // of this block's keys in the first block's list
 };
 
 template <typename T, bool RESIDENT>
@@ -347,23 +345,27 @@ struct SfRow {
   // All blocks: the keys by their steps.  With top-k their numbers (in two histograms, for even and odd lanes, so that fewer lanes of a warp meet); without it
   // their weights, to 2^-31 of themselves.
   __device__ __forceinline__ void count_steps(bool numbers) const {
-    const int none = SF_STEPS + (int)(threadIdx.x & 31);
     if (numbers) {
       unsigned* mine = threadIdx.x & 1 ? s.two : s.one;
       each_value([&](const auto& v, int) {
 #pragma unroll
-        for (const float x : v) atomicAdd(mine + (x > -INFINITY ? step_of(x) : none), 1u);
+        for (const float x : v) {
+          const int n = step_of(x);
+          if (!nothing(n)) atomicAdd(mine + n, 1u);
+        }
       });
     } else {
       each_value([&](const auto& v, int) {
 #pragma unroll
         for (const float x : v) {
           float rest;
-          const int n = step_of(x, &rest), at = x > -INFINITY ? n : none;
+          const int n = step_of(x, &rest);
           // 2^31 - e 2^31 in halves: e 2^15 is cut to a whole number, what is left of it has 16 bits more
           const float e = short_of(rest), z = fmaf(e, 32768.f, -0.5f) + 12582912.f, left = fmaf(e, 32768.f, 12582912.f - z);
-          atomicAdd(&s.one[at], (unsigned)(0x4B400000 + 32767 - __float_as_int(z)));
-          atomicAdd(&s.two[at], (unsigned)(0x4B400000 + 65536 - __float_as_int(fmaf(left, 65536.f, 12582912.f))));
+          if (!nothing(n)) {
+            atomicAdd(&s.one[n], (unsigned)(0x4B400000 + 32767 - __float_as_int(z)));
+            atomicAdd(&s.two[n], (unsigned)(0x4B400000 + 65536 - __float_as_int(fmaf(left, 65536.f, 12582912.f))));
+          }
         }
       });
     }
@@ -580,11 +582,16 @@ struct SfRow {
       to[r] = numbers ? INFINITY : y1 + fminf(fabsf(y1), 1e38f) * 1e-6f;
       if (first[r] < 0) from[r] = INFINITY, to[r] = -INFINITY;
     }
-    if (numbers) from[1] = fminf(fminf(from[0], from[1]), fminf(from[2], from[3]));
+    const float lowest = fminf(fminf(from[0], from[1]), fminf(from[2], from[3]));
+    if (numbers) from[1] = lowest, to[1] = INFINITY;
     const auto near = [&](float x) {  // (there is no border of top-k without its numbers)
-      return numbers ? x >= from[1] : (x >= from[1] && x <= to[1]) || (x >= from[2] && x <= to[2]) || (x >= from[3] && x <= to[3]);
+      return (x >= from[1] && x <= to[1]) || (x >= from[2] && x <= to[2]) || (x >= from[3] && x <= to[3]);
     };
     each_value([&](const auto& v, int i0) {
+      float most = -INFINITY;  // (most logits lie below all of them)
+#pragma unroll
+      for (const float x : v) most = fmaxf(most, x);
+      if (!(most >= lowest)) return;
       bool any = false;
 #pragma unroll
       for (const float x : v) any |= near(x);
@@ -614,10 +621,10 @@ struct SfRow {
       if (threadIdx.x == 0) {
         unsigned at;
         asm volatile("atom.relaxed.cluster.shared::cluster.add.u32 %0, [%1], %2;" : "=r"(at) : "r"(sf_remote(&s.listed, 0)), "r"(mine) : "memory");
-        s.base[0] = at;
+        s.place = (int)at;
       }
       __syncthreads();
-      const int at = (int)s.base[0];
+      const int at = s.place;
       for (int i = threadIdx.x; i < mine && at + i < SF_LIST; i += SF_THREADS) sf_store(&s.list[at + i], 0, s.list[i]);
     }
     if (!numbers) return;
@@ -638,60 +645,99 @@ struct SfRow {
     }
   }
 
-  // First block: sort what was handed over and walk the borders; the token.  GROUP: the threads that do it, one warp or all of the block.
-  template <int GROUP>
+  // First block (GROUP threads of it, EACH keys a thread): sorts the keys that it was handed and finds the token.  Whatever is asked of the sorted keys holds for
+  // a beginning of them, or from some key on up to another: the borders are counts.
+  template <int GROUP, int EACH>
   __device__ void decide(float top_p, float u, int* out) {
+    const int m = min((int)s.listed, SF_LIST), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const auto sync = [] {
       if (GROUP == 32) __syncwarp();
       else __syncthreads();
     };
-    const int m = min((int)s.listed, SF_LIST), tid = threadIdx.x;
-    int size = 2;
-    while (size < m) size *= 2;
-    for (int i = m + tid; i < size; i += GROUP) s.list[i] = ~0ull;
-    sync();
-    for (int k = 2; k <= size; k *= 2) {
-      for (int j = k / 2; j > 0; j /= 2) {
-        for (int i = tid; i < size / 2; i += GROUP) {
-          const int x = 2 * i - (i & (j - 1)), y = x + j;
-          const unsigned long long p = s.list[x], q = s.list[y];
-          if ((p > q) == ((x & k) == 0)) { s.list[x] = q; s.list[y] = p; }
+    unsigned long long entry[EACH];
+    if (EACH == 1) {  // each key counts those in front of it
+      entry[0] = tid < m ? s.list[tid] : ~0ull;
+      int place = tid < m ? 0 : tid;
+      if (GROUP == 32) {
+        for (int j = 0; j < m; ++j) {  // (all lanes take part in the shuffle)
+          const unsigned long long other = __shfl_sync(0xffffffffu, entry[0], j);
+          place += tid < m && other < entry[0];
         }
-        sync();
+      } else if (tid < m) {
+#pragma unroll 4
+        for (int j = 0; j < m; ++j) place += s.list[j] < entry[0];
       }
-    }
-    // running sums: thread t has entries t * each and on; f(entry, its step, the running sum in front of it, with it)
-    const int each = (m + GROUP - 1) / GROUP, i0 = min(tid * each, m), i1 = min(i0 + each, m);
-    auto walk = [&](unsigned long long run, auto f) {
-#pragma unroll 1
-      for (int i = i0; i < i1; ++i) {
-        float rest;
-        const int n = step_of(sf_value(~(unsigned)(s.list[i] >> 32)), &rest);
-        const unsigned long long next = run + to_scale(weight_at(n, short_of(rest)));
-        f(i, n, run, next);
-        run = next;
+      sync();
+      if (tid < m) s.list[place] = entry[0];
+      sync();
+      if (tid < m) entry[0] = s.list[tid];
+    } else {
+      int size = 2;
+      while (size < m) size *= 2;
+      for (int i = m + tid; i < size; i += GROUP) s.list[i] = ~0ull;
+      sync();
+      for (int k = 2; k <= size; k *= 2) {
+        for (int j = k / 2; j > 0; j /= 2) {
+          for (int i = tid; i < size / 2; i += GROUP) {
+            const int x = 2 * i - (i & (j - 1)), y = x + j;
+            const unsigned long long p = s.list[x], q = s.list[y];
+            if ((p > q) == ((x & k) == 0)) { s.list[x] = q; s.list[y] = p; }
+          }
+          sync();
+        }
       }
-      return run;
-    };
-    const unsigned long long sum = walk(0ull, [](int, int, unsigned long long, unsigned long long) {});
-    const int lane = tid & 31, warp = tid >> 5;
-    unsigned long long run0 = sum;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const unsigned long long t = __shfl_up_sync(0xffffffffu, run0, o);
-      if (lane >= o) run0 += t;
+      for (int e = 0; e < EACH; ++e) entry[e] = tid + e * GROUP < m ? s.list[tid + e * GROUP] : ~0ull;
+      sync();
     }
-    unsigned long long total = __shfl_sync(0xffffffffu, run0, 31);
-    if (GROUP > 32) {
-      if (lane == 31) s.warp[warp] = run0;
-      __syncthreads();
-      total = 0;
-      for (int x = 0; x < GROUP / 32; ++x) {
-        if (x < warp) run0 += s.warp[x];
-        total += s.warp[x];
+    // the keys' steps, and the running sums in front of them and with them (those in runs[], too)
+    unsigned long long* runs = EACH == 1 ? s.list + SF_LIST / 2 : s.list;  // (beside the keys, or over them: the threads have those)
+    unsigned long long before[EACH], run[EACH], total = 0;
+    int n[EACH];
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+      float rest;
+      n[e] = step_of(sf_value(~(unsigned)(entry[e] >> 32)), &rest);
+      const unsigned long long w = tid + e * GROUP < m ? to_scale(weight_at(n[e], short_of(rest))) : 0ull;
+      run[e] = w;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const unsigned long long t = __shfl_up_sync(0xffffffffu, run[e], o);
+        if (lane >= o) run[e] += t;
       }
+      if (GROUP > 32) {
+        if (lane == 31) s.warp[warp] = run[e];
+        __syncthreads();
+        unsigned long long chunk = 0;
+#pragma unroll 4
+        for (int x = 0; x < GROUP / 32; ++x) {
+          if (x < warp) run[e] += s.warp[x];
+          chunk += s.warp[x];
+        }
+        run[e] += total;
+        total += chunk;
+        runs[tid + e * GROUP] = run[e];
+        __syncthreads();
+      }
+      before[e] = run[e] - w;
     }
-    run0 -= sum;
+    const auto run_at = [&](int i) {  // the running sum with the i-th key (0 in front of the first)
+      if (GROUP == 32) {
+        const unsigned long long x = __shfl_sync(0xffffffffu, run[0], max(i, 0));
+        return i < 0 ? 0ull : x;
+      }
+      return i < 0 ? 0ull : runs[i];
+    };
+    const auto count = [&](auto holds) {  // the keys for which holds(their place, which of this thread's)
+      int c = 0;
+#pragma unroll
+      for (int e = 0; e < EACH; ++e) {
+        const int i = tid + e * GROUP;
+        const bool is = i < m && holds(i, e);
+        c += GROUP == 32 ? __popc(__ballot_sync(0xffffffffu, is)) : __syncthreads_count(is);
+      }
+      return c;
+    };
     unsigned long long over[4], part4 = 0;  // lane: block lane / 4 and 8 more, range lane % 4
     for (unsigned b = lane >> 2; b < blocks; b += 8) part4 += s.over[b][lane & 3];
 #pragma unroll
@@ -702,60 +748,33 @@ struct SfRow {
 #pragma unroll
     for (int r = 0; r < 4; ++r) range[r] = s.plan.range[r];
     const auto is_in = [&](int r) { return range[r].last >= range[r].first; };
-    if (tid < 4) { s.base[tid] = total; s.at[tid] = m; }
-    if (tid == 0) { s.sum[0] = is_in(SF_TOP_K) ? over[SF_TOP_K] : s.all_mass; s.sum[1] = is_in(SF_MIN_P) ? over[SF_MIN_P] : ~0ull; }
-    sync();
-    // where each range begins, and the running sum in front of it
-    int prev = i0 > 0 ? step_of(sf_value(~(unsigned)(s.list[i0 - 1] >> 32))) : -1;
-    walk(run0, [&](int i, int n, unsigned long long before, unsigned long long) {
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-        if (n >= range[r].first && prev < range[r].first) { s.base[r] = before; s.at[r] = i; }
-      prev = n;
-    });
-    sync();
-    if (is_in(SF_TOP_K)) {  // (in the last step, whose keys are not here, all that weighs lies above)
-      const int at = s.at[SF_TOP_K] + (int)s.plan.rest - 1;
-      if (range[SF_TOP_K].first != SF_STEPS - 1) walk(run0, [&](int i, int, unsigned long long, unsigned long long run) {
-        if (i == at) s.sum[0] = over[SF_TOP_K] + run - s.base[SF_TOP_K];
-      });
+    const auto begin = [&](int r) { return count([&](int, int e) { return n[e] < range[r].first; }); };  // the place of a range's first key
+    unsigned long long kept = s.all_mass;
+    if (is_in(SF_TOP_K)) {
+      const int at = begin(SF_TOP_K);
+      kept = over[SF_TOP_K] + run_at(min(at + (int)s.plan.rest, m) - 1) - run_at(at - 1);
     }
-    if (is_in(SF_MIN_P)) {  // the last entry that stays; without one nothing of the range does
-      const int at0 = s.at[SF_MIN_P];
-      const unsigned least = s.plan.least;
-      walk(run0, [&](int i, int, unsigned long long, unsigned long long run) {
-        if (i >= at0 && ~(unsigned)(s.list[i] >> 32) >= least && (i + 1 >= m || ~(unsigned)(s.list[i + 1] >> 32) < least))
-          s.sum[1] = over[SF_MIN_P] + run - s.base[SF_MIN_P];
-      });
-    }
-    sync();
-    unsigned long long kept = s.sum[0];
-    if (is_in(SF_TOP_P)) {
+    if (is_in(SF_TOP_P)) {  // up to the last whose predecessors do not exceed it
       const unsigned long long thr = min((unsigned long long)((double)top_p * (double)kept), kept - 1);
-      const int at0 = s.at[SF_TOP_P];
-      const unsigned long long off = over[SF_TOP_P] - s.base[SF_TOP_P];
-      sync();
-      if (tid == 0) s.sum[0] = over[SF_TOP_P];
-      sync();
-      // the last whose predecessors do not exceed it
-      walk(run0, [&](int i, int n, unsigned long long before, unsigned long long run) {
-        if (i >= at0 && n <= range[SF_TOP_P].last && before + off <= thr) atomicMax(&s.sum[0], run + off);
-      });
-      sync();
-      kept = s.sum[0];
+      const int at = begin(SF_TOP_P);
+      const unsigned long long off = over[SF_TOP_P] - run_at(at - 1);
+      kept = off + run_at(at + count([&](int i, int e) { return i >= at && n[e] <= range[SF_TOP_P].last && before[e] + off <= thr; }) - 1);
     }
-    // (where min-p alone decides, the plan has no other range, and its sum is the smaller one)
-    if (is_in(SF_MIN_P)) kept = is_in(SF_TOP_K) || is_in(SF_TOP_P) ? min(kept, s.sum[1]) : s.sum[1];
+    if (is_in(SF_MIN_P)) {
+      const unsigned least = s.plan.least;
+      const int at = begin(SF_MIN_P), stay = count([&](int, int e) { return ~(unsigned)(entry[e] >> 32) >= least; });
+      const unsigned long long sum = over[SF_MIN_P] + run_at(max(stay, at) - 1) - run_at(at - 1);
+      // (where min-p alone decides, the plan has no other range, and its sum is the smaller one)
+      kept = is_in(SF_TOP_K) || is_in(SF_TOP_P) ? min(kept, sum) : sum;
+    }
     const unsigned long long thr = min((unsigned long long)((double)u * (double)kept), kept - 1);
-    const int at0 = s.at[SF_DRAW];
-    const unsigned long long off = over[SF_DRAW] - s.base[SF_DRAW];
-    if (tid == 0) s.at[0] = max(min(at0, m - 1), 0);
-    sync();
-    walk(run0, [&](int i, int n, unsigned long long before, unsigned long long) {
-      if (i >= at0 && n <= range[SF_DRAW].last && before + off <= thr) atomicMax(&s.at[0], i);
-    });
-    sync();
-    if (tid == 0) *out = (int)(unsigned)s.list[s.at[0]];
+    const int at = begin(SF_DRAW);
+    const unsigned long long off = over[SF_DRAW] - run_at(at - 1);
+    const int c = count([&](int i, int e) { return i >= at && n[e] <= range[SF_DRAW].last && before[e] + off <= thr; });
+    const int chosen = c ? at + c - 1 : max(min(at, m - 1), 0);
+#pragma unroll
+    for (int e = 0; e < EACH; ++e)
+      if (tid + e * GROUP == chosen) *out = (int)(unsigned)entry[e];
   }
 
   // The index of the j-th (from 0) of the row's numbers with key k, in the block that has it; -1 elsewhere.
@@ -832,7 +851,7 @@ __global__ void __launch_bounds__(SF_THREADS, 1024 / SF_THREADS) sample_filtered
   const int first = min(a.vocab, (int)rank * a.per);
   SfRow<T, RESIDENT> row{a, s, held, (const T*)a.logits + (size_t)r * a.ld + first, min(a.vocab, first + a.per) - first, rank, blocks};
   if (blocks > 1) sf_arrive();
-  for (int b = threadIdx.x; b < SF_STEPS; b += SF_THREADS) s.one[b] = s.two[b] = 0;  // (nothing reads what lies behind)
+  for (int b = threadIdx.x; b < SF_STEPS; b += SF_THREADS) s.one[b] = s.two[b] = 0;
   if (threadIdx.x < 32) {
     const unsigned long long x = a.table[threadIdx.x];
     s.table[threadIdx.x] = x;
@@ -896,8 +915,9 @@ __global__ void __launch_bounds__(SF_THREADS, 1024 / SF_THREADS) sample_filtered
         row.hand_over(k_on);
         sf_sync(blocks);  // the last time that another block is needed
         if (rank == 0) {
-          if (s.listed > SF_FEW) row.template decide<SF_THREADS>(top_p, u, a.out + r);
-          else if (threadIdx.x < 32) row.template decide<32>(top_p, u, a.out + r);
+          if (s.listed > SF_THREADS) row.template decide<SF_THREADS, SF_LIST / SF_THREADS>(top_p, u, a.out + r);
+          else if (s.listed > 32) row.template decide<SF_THREADS, 1>(top_p, u, a.out + r);
+          else if (threadIdx.x < 32) row.template decide<32, 1>(top_p, u, a.out + r);
         }
         return;
       }
