@@ -119,7 +119,7 @@ struct SfShared {
   union {
     unsigned long long hist[SF_BINS];
     struct {
-      // of a step's keys their number, in two parts; or the sum of their weights in parts of 2^-31 of its largest, upper and lower 16 bits apart
+      // of a step's keys their number; or the sum of their weights in parts of 2^-31 of its largest, upper and lower 16 bits apart
       unsigned one[SF_STEPS], two[SF_STEPS];
     };
     unsigned long long list[SF_LIST];  // keys falling, equal ones by index: (~key, index)
@@ -342,16 +342,15 @@ struct SfRow {
     }
   }
 
-  // All blocks: the keys by their steps.  With top-k their numbers (in two histograms, for even and odd lanes, so that fewer lanes of a warp meet); without it
+  // All blocks: the keys by their steps.  With top-k their numbers (in one histogram: two, for fewer lanes that meet, cost the first block 0.6 us of loads); without it
   // their weights, to 2^-31 of themselves.
   __device__ __forceinline__ void count_steps(bool numbers) const {
     if (numbers) {
-      unsigned* mine = threadIdx.x & 1 ? s.two : s.one;
       each_value([&](const auto& v, int) {
 #pragma unroll
         for (const float x : v) {
           const int n = step_of(x);
-          if (!nothing(n)) atomicAdd(mine + n, 1u);
+          if (!nothing(n)) atomicAdd(&s.one[n], 1u);
         }
       });
     } else {
@@ -385,7 +384,7 @@ struct SfRow {
 #pragma unroll
         for (int q = 0; q < EACH / 4; ++q) {
           ones[r][q] = r0 + r < blocks ? sf_load4(&s.one[n0 + 4 * q], r0 + r) : make_uint4(0u, 0u, 0u, 0u);
-          twos[r][q] = r0 + r < blocks ? sf_load4(&s.two[n0 + 4 * q], r0 + r) : make_uint4(0u, 0u, 0u, 0u);
+          twos[r][q] = !k_on && r0 + r < blocks ? sf_load4(&s.two[n0 + 4 * q], r0 + r) : make_uint4(0u, 0u, 0u, 0u);
         }
 #pragma unroll
       for (unsigned r = 0; r < 4; ++r)
@@ -409,7 +408,7 @@ struct SfRow {
       const int n = n0 + e;
       const unsigned long long t = most_at(n);
       if (k_on) {
-        c[e] = (unsigned)(one[e] + two[e]);
+        c[e] = (unsigned)one[e];
         up[e] = c[e] * (to_scale(t + (t >> 6)) + 1);  // (2^(1/64) at most, 2^(-1/32) at least)
         lo[e] = c[e] * to_scale(t - (t >> 5));
       } else {
