@@ -101,8 +101,8 @@ struct DtArgs {
   __nv_bfloat16* out;
   int out_stride;
   // with JOIN: what attention_shared.cu found for pages that a sequence shares with others
-  const int4* shared;     // per sequence: pages covered there (its first ones), the first of its results, their number; and of the sequences the one that
-                          // the blocks of this place take (those with the most pages of their own come first)
+  const int4* shared;     // per place of the grid (those with the most pages of their own come first): of a sequence the pages covered there (its first
+                          // ones), the first of its results, their number, and which sequence
   const float* shared_o;  // [results][n_heads][head_dim], unnormalised
   const float* shared_ml; // [results][n_heads][2]: maximum and sum, as part_ml
   int n_shared;           // results that there are
@@ -183,7 +183,8 @@ attention_decode_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
     }
     b = item & 0xFFFF; zi = (item >> 16) & 0xFF; nz = (item >> 24) & 0x7F;
   }
-  if (JOIN) b = min(max(a.shared[b].w, 0), (int)gridDim.x - 1);
+  const int4 sh = JOIN ? a.shared[b] : make_int4(0, 0, 0, 0);
+  if (JOIN) b = min(max(sh.w, 0), (int)gridDim.x - 1);
   const int g4 = lane >> 2, t4 = lane & 3;
   const int head_dim = a.head_dim, n_kv_heads = a.n_kv_heads, n_heads = a.n_heads;
   const int group = n_heads / n_kv_heads;
@@ -191,8 +192,7 @@ attention_decode_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
   const int kvh = blockIdx.y / gblocks, gb = blockIdx.y % gblocks;
   const int h0 = kvh * group + gb * DT_ROWS;
   const int G = min(DT_ROWS, group - gb * DT_ROWS);
-  const int pos = a.tok_pos[b];
-  const int4 sh = JOIN ? a.shared[b] : make_int4(0, 0, 0, 0);
+  const int pos = a.tok_pos[b], slot = a.slots[b];  // (both asked for at once: what follows waits for both)
   const int lo = JOIN ? min(sh.x, pos / BN_PAGE) * BN_PAGE : a.window > 0 ? max(0, pos - a.window + 1) : 0;
   // pages that hold a visible key, and this block's run of them
   const int p_lo = lo / BN_PAGE, p_hi = pos / BN_PAGE;
@@ -216,7 +216,7 @@ attention_decode_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
   }
   const int n_pages = my_hi - my_lo + 1;
   const int n_splits = nz;
-  const int* pt = a.page_table + (size_t)a.slots[b] * a.pt_stride;
+  const int* pt = a.page_table + (size_t)slot * a.pt_stride;
   const bool has_new = (p_hi >= my_lo && p_hi <= my_hi);  // the new token's page is in this run
   const int new_row = pos - p_hi * BN_PAGE;
 
@@ -810,9 +810,9 @@ extern "C" int bn_attention_decode_tc_items(const void* qkv, int q_stride, int k
                 theta_scale, tok_pos, slots, page_table, pt_stride, k_cache, v_cache, n_cache_pages, status, part_o, part_ml,
                 1, 1, tickets, n_tickets, items, n_items, item_group, nullptr, nullptr, nullptr, 0, stream);
 }
-// With the first shared[4 b] pages of each sequence b attended to by attention_shared.cu, launched directly in front (it lets this kernel start early): its
-// results shared[4 b + 1] .. + shared[4 b + 2] - 1 of shared_o / shared_ml are joined with those of the other pages, of which there is at least one (the
-// new token's).  n_splits blocks (at most 8) share a sequence's other
+// shared: n_seqs rows (pages, first result, results, sequence).  With the first pages of each sequence attended to by attention_shared.cu, launched directly in
+// front (it lets this kernel start early): its results of shared_o / shared_ml are joined with those of the other pages, of which there is at least one
+// (the new token's).  n_splits blocks (at most 8) share a sequence's other
 // pages, about pages_per_block each.  No window, no rotation (the rows are rotated), head_dim at most 128.
 extern "C" int bn_attention_decode_tc_join(const void* qkv, int q_stride, int k_off, int v_off, void* out, int out_stride,
                                            int n_seqs, int n_heads, int n_kv_heads, int head_dim, float scale, const int* tok_pos, const int* slots,

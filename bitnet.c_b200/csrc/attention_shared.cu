@@ -8,7 +8,7 @@
 // pages (attention_decode_tc.cu) reads them and joins them with its own.  All keys of a run are visible to all its rows (a run ends in front of
 // every new token), so nothing is masked.
 //
-// Which block works on what is a list made on the host: (first member, members, first page, pages) per item, members as (sequence, where its
+// Which block works on what is a list made on the host: (first member, members and the first one's sequence, first page, pages) per item, members as (sequence, where its
 // results go).  Blocks and roles as in attention_prefill_tc.cu: warp 0 requests pages (TMA, 128-byte swizzle), warp 1 issues the MMAs,
 // S of the next page ahead of P V of this one, warps 2 to 5 copy the queries into shared memory and do the softmax, one row per thread.
 // P goes back to tensor memory over the columns S came from.  Every wait is bounded; a block whose wait gave up records it and stores nothing.
@@ -29,7 +29,7 @@ struct AsArgs {
   const __nv_bfloat16* q;  // [n_seqs, q_stride], rotated
   int q_stride, n_seqs, n_heads, n_kv_heads, head_dim, per_group;
   float scale_log2e;
-  const int4* items;       // first member, members, first page, pages; no members: nothing to do
+  const int4* items;       // first member, members + 256 * the first one's sequence, first page, pages; no members: nothing to do
   const int2* members;     // sequence, where its results go
   int n_members, n_parts;
   const int* slots;
@@ -73,14 +73,14 @@ attention_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, kvh = blockIdx.x;
   const int4 item = a.items[blockIdx.y];
-  const int n_tiles = item.w;
-  if (item.y <= 0 || n_tiles <= 0 || item.x < 0 || item.x + item.y > a.n_members || item.z < 0 || item.z + n_tiles > a.pt_stride) {
+  const int n_tiles = item.w, n_members = item.y & 255;
+  if (n_members <= 0 || n_tiles <= 0 || item.x < 0 || item.x + n_members > a.n_members || (item.y >> 8) >= a.n_seqs || item.z < 0 || item.z + n_tiles > a.pt_stride) {
     pdl_wait();
     return;
   }
-  const int rows = min(AS_ROWS, item.y * a.per_group);
+  const int rows = min(AS_ROWS, n_members * a.per_group);
   const int2* members = a.members + item.x;
-  const int* pt = a.page_table + (size_t)a.slots[members[0].x] * a.pt_stride + item.z;
+  const int* pt = a.page_table + (size_t)a.slots[item.y >> 8] * a.pt_stride + item.z;
 
   if (tid == 0) {
     *failed = 0;

@@ -1152,8 +1152,8 @@ class SharedPlan:
         return self
 
     def _lay_out(self, sms: int) -> None:
-        """The list of work, ``host``: items (first member, members, first page, pages), of every sequence (pages read together, first place of its
-        results, places; and which sequence is the n-th by its own pages, the most first), and members (sequence, place)."""
+        """The list of work, ``host``: items (first member, members + 256 * the first one's sequence, first page, pages), sequences (pages read together, first place of
+        its results, places, which sequence; those with the most pages of their own first), and members (sequence, place)."""
         most = SHARED_ROWS // (self.n_heads // self.n_kv_heads)  # sequences of a block
         tiles = [(members[i:i + most], first, n) for members, first, n in self.runs for i in range(0, len(members), most)]
         # one block an SM, which share all pages evenly: two would fit, but then the sequences' own pages wait until they have ended (8 prompts of 2,048 tokens by
@@ -1178,9 +1178,9 @@ class SharedPlan:
             at += c
         self.n_parts, self.n_items = at, len(work)
         order = sorted(range(self.n_seqs), key=lambda b: self.first_own[b] - self.lengths[b])
-        items, entries, sequences = [], [], [x for b in range(self.n_seqs) for x in (self.first_own[b], place[b], count[b], order[b])]
+        items, entries, sequences = [], [], [x for b in order for x in (self.first_own[b], place[b], count[b], b)]
         for members, first, n in work:
-            items += (len(entries) // 2, len(members), first, n)
+            items += (len(entries) // 2, len(members) + 256 * members[0], first, n)
             for b in members:
                 entries += (b, place[b])
                 place[b] += 1

@@ -25,14 +25,15 @@ def pieces_of(plan):
     most = ops.SHARED_ROWS // (plan.n_heads // plan.n_kv_heads)
     for i in range(plan.n_items):
         first, count, page, n = items[4 * i:4 * i + 4]
+        count, begin = count % 256, count // 256
         if not count:  # what a list of fixed size is padded with
             continue
-        assert 1 <= count <= most and n >= 1 and first + count <= plan.n_parts
+        assert 1 <= count <= most and n >= 1 and first + count <= plan.n_parts and begin == members[2 * first]
         for m in range(first, first + count):
             b, place = members[2 * m:2 * m + 2]
             assert place not in got[b]
             got[b][place] = list(range(page, page + n))
-    return got, [sequences[4 * b:4 * b + 4] for b in range(plan.n_seqs)]
+    return got, [sequences[4 * b:4 * b + 4] for b in range(plan.n_seqs)]  # in the order of their blocks
 
 
 @pytest.mark.parametrize("heads,kv", [(32, 8), (40, 40), (6, 2), (24, 1), (128, 1), (100, 1)])
@@ -58,8 +59,7 @@ def test_every_shared_page_is_read_once_for_every_sequence(heads, kv, seed):
 
 def look_over(plan, pages):
     got, sequences = pieces_of(plan)
-    for b in range(len(pages)):
-        first_own, place, n, _ = sequences[b]
+    for first_own, place, n, b in sequences:
         assert sorted(got[b]) == list(range(place, place + n)) and place + n <= plan.n_parts
         assert sorted(x for piece in got[b].values() for x in piece) == list(range(first_own))
         assert first_own < len(pages[b]) and plan.own_pages >= len(pages[b]) - first_own
