@@ -2850,49 +2850,56 @@ def sample_filtered(logits: torch.Tensor, temperature, top_k=0, top_p=1.0, min_p
     two rows one state)."""
     _need_rows(logits, "logits")
     n, vocab = logits.shape
-    device = logits.device
-
-    def given(x, name, dtype):
-        if not isinstance(x, torch.Tensor):
-            return None, (int(x) if dtype is torch.int32 else float(x))
-        _need(x, name, dtype, 1)
-        if x.shape[0] != n or x.device != device:
-            raise KernelError(f"sample_filtered: {name} {tuple(x.shape)} on {x.device} does not go with {n} rows on {device}")
-        return x, 0
-
-    temperatures, t = given(temperature, "temperature", torch.float32)
-    top_ks, k = given(top_k, "top_k", torch.int32)
-    top_ps, p = given(top_p, "top_p", torch.float32)
-    min_ps, m = given(min_p, "min_p", torch.float32)
+    at = logits.get_device()
+    # of each parameter its value or where the rows' values lie
+    t, ts = (0.0, _of_rows(temperature, "temperature", torch.float32, n, at)) if isinstance(temperature, torch.Tensor) else (float(temperature), _NOWHERE)
+    k, ks = (0, _of_rows(top_k, "top_k", torch.int32, n, at)) if isinstance(top_k, torch.Tensor) else (min(max(int(top_k), 0), 0x7fffffff), _NOWHERE)
+    p, ps = (0.0, _of_rows(top_p, "top_p", torch.float32, n, at)) if isinstance(top_p, torch.Tensor) else (float(top_p), _NOWHERE)
+    m, ms = (0.0, _of_rows(min_p, "min_p", torch.float32, n, at)) if isinstance(min_p, torch.Tensor) else (float(min_p), _NOWHERE)
     if not t >= 0.0:
         raise KernelError(f"sample_filtered: temperature={t} must not be negative")
-    k = min(max(k, 0), 0x7fffffff)
     if (u is None) == (rng_state is None):
         raise KernelError("sample_filtered: either u or rng_state")
+    us = states = indices = _NOWHERE
     if u is not None:
-        given(u, "u", torch.float32)
+        us = _of_rows(u, "u", torch.float32, n, at)
         if index is not None:
             raise KernelError("sample_filtered: index goes with rng_state")
     else:
         _need(rng_state, "rng_state", torch.int64, 1)
+        if rng_state.get_device() != at:
+            raise KernelError(f"sample_filtered: rng_state on {rng_state.device} does not go with logits on {logits.device}")
         if index is not None:
-            given(index, "index", torch.int32)
+            indices = _of_rows(index, "index", torch.int32, n, at)
         elif rng_state.shape[0] < n:
             raise KernelError("sample_filtered: one generator state per row is needed")
-    out = out if out is not None else torch.empty(n, dtype=torch.int32, device=device)
-    _need(out, "out", torch.int32, 1)
-    if out.shape[0] < n or out.device != device:
-        raise KernelError(f"sample_filtered: out {tuple(out.shape)} on {out.device} does not hold {n} tokens")
+        states = _ptr(rng_state)
+    if out is None:
+        out = torch.empty(n, dtype=torch.int32, device=logits.device)
+    else:
+        _need(out, "out", torch.int32, 1)
+        if out.shape[0] < n or out.get_device() != at:
+            raise KernelError(f"sample_filtered: out {tuple(out.shape)} on {out.device} does not hold {n} tokens")
     if n == 0:
         return out
     if vocab == 0:
         raise KernelError("sample_filtered: no logits")
-    with _on(device):
+    with _on(logits.device):
         _check(_fn("sampling_filtered", "bn_sample_filtered")(
-            _ptr(logits), _code(logits), ctypes.c_longlong(logits.stride(0) if n > 1 else vocab), int(n), int(vocab), c_float(t), _ptr(temperatures), k,
-            _ptr(top_ks), c_float(p), _ptr(top_ps), c_float(m), _ptr(min_ps), _ptr(u), _ptr(rng_state), _ptr(index), _ptr(out), _stream()),
-            "sample_filtered")
+            _ptr(logits), _code(logits), ctypes.c_longlong(logits.stride(0) if n > 1 else vocab), n, vocab, c_float(t), ts, k, ks, c_float(p), ps, c_float(m),
+            ms, us, states, indices, _ptr(out), _stream()), "sample_filtered")
     return out
+
+
+_NOWHERE = c_void_p(0)
+
+
+def _of_rows(x: torch.Tensor, name: str, dtype, n: int, at: int) -> c_void_p:
+    """Where a parameter of ``n`` rows on device ``at`` lies."""
+    _need(x, name, dtype, 1)
+    if x.shape[0] != n or x.get_device() != at:
+        raise KernelError(f"sample_filtered: {name} {tuple(x.shape)} on {x.device} does not go with {n} rows on cuda:{at}")
+    return c_void_p(x.data_ptr())
 
 
 def repeat_penalty(logits: torch.Tensor, recent: torch.Tensor, recent_len: torch.Tensor, penalty: float,
