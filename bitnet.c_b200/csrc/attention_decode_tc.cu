@@ -748,14 +748,14 @@ static int dt_run(const void* qkv, int q_stride, int k_off, int v_off, void* out
     pages_per_block = 1 << 20;
   }
   if (head_dim <= 0 || head_dim % 16 || head_dim > 256 || n_kv_heads <= 0 || n_heads % n_kv_heads || n_splits <= 0 ||
-      pages_per_block <= 0 || window < 0 || !part_o || !part_ml || !tickets || !status || n_cache_pages <= 0 ||
+      pages_per_block <= 0 || window < 0 || (shared == nullptr && (!part_o || !part_ml || !tickets)) || !status || n_cache_pages <= 0 ||
       (((uintptr_t)k_cache | (uintptr_t)v_cache) & 15) || rotary_dims < 0 ||
       rotary_dims > head_dim || (rotary_dims & 1))
     return BN_ERR_BAD_ARG;
   int group = n_heads / n_kv_heads;
   int gblocks = (group + DT_ROWS - 1) / DT_ROWS;
   if ((long long)n_kv_heads * gblocks > 65535 || n_splits > 65535 ||
-      (long long)n_seqs * n_kv_heads * gblocks > n_tickets)
+      (shared == nullptr && (long long)n_seqs * n_kv_heads * gblocks > n_tickets))
     return BN_ERR_BAD_ARG;
   DtArgs a = {};
   a.qkv = (const __nv_bfloat16*)qkv; a.q_stride = q_stride; a.k_off = k_off; a.v_off = v_off;
@@ -817,11 +817,10 @@ extern "C" int bn_attention_decode_tc_items(const void* qkv, int q_stride, int k
 extern "C" int bn_attention_decode_tc_join(const void* qkv, int q_stride, int k_off, int v_off, void* out, int out_stride,
                                            int n_seqs, int n_heads, int n_kv_heads, int head_dim, float scale, const int* tok_pos, const int* slots,
                                            const int* page_table, int pt_stride, void* k_cache, void* v_cache,
-                                           int n_cache_pages, int* status, float* part_o, float* part_ml, int n_splits, int pages_per_block, int* tickets,
-                                           int n_tickets, const int* shared, const float* shared_o, const float* shared_ml, int n_shared,
+                                           int n_cache_pages, int* status, int n_splits, int pages_per_block, const int* shared, const float* shared_o, const float* shared_ml, int n_shared,
                                            cudaStream_t stream) {
   if (!shared || !shared_o || !shared_ml || n_shared <= 0 || head_dim > 128 || (((uintptr_t)shared) & 15) || (((uintptr_t)shared_ml) & 7)) return BN_ERR_BAD_ARG;
   return dt_run(qkv, q_stride, k_off, v_off, out, out_stride, n_seqs, n_heads, n_kv_heads, head_dim, scale, 0, 0, 1.0f, tok_pos, slots,
-                page_table, pt_stride, k_cache, v_cache, n_cache_pages, status, part_o, part_ml, n_splits, pages_per_block, tickets, n_tickets,
+                page_table, pt_stride, k_cache, v_cache, n_cache_pages, status, nullptr, nullptr, n_splits, pages_per_block, nullptr, 0,
                 nullptr, 0, 0, shared, shared_o, shared_ml, n_shared, stream);
 }

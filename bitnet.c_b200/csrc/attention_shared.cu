@@ -304,29 +304,39 @@ static int as_launch(const CUtensorMap& mk, const CUtensorMap& mv, const AsArgs&
   return BN_OK;
 }
 
-// q: [n_seqs, q_stride] bfloat16, head h at element h * head_dim, 16-byte aligned, q_stride a multiple of 8.  items [n_items] and members
-// [n_members] as above; part_o [n_parts, n_heads, head_dim] and part_ml [n_parts, n_heads, 2] are written where members say.  The caches are
+// bn_attention_decode_tc_join of attention_decode_tc.cu
+typedef int (*BnDecodeJoin)(const void* qkv, int q_stride, int k_off, int v_off, void* out, int out_stride, int n_seqs, int n_heads, int n_kv_heads, int head_dim,
+                            float scale, const int* tok_pos, const int* slots, const int* page_table, int pt_stride, void* k_cache, void* v_cache,
+                            int n_cache_pages, int* status, int n_splits, int pages_per_block, const int* shared,
+                            const float* shared_o, const float* shared_ml, int n_shared, cudaStream_t stream);
+
+// The kernel above and behind it `join` (one call from the host: two take it 3 us more).  qkv: [n_seqs, q_stride] bfloat16 rows, rotated, query head h at
+// element h * head_dim, key heads at k_off, value heads at v_off, 16-byte aligned, q_stride a multiple of 8.  items [n_items], members [n_parts] and
+// sequences [n_seqs] as above and there; part_o [n_parts, n_heads, head_dim] and part_ml [n_parts, n_heads, 2] are written where members say.  The caches are
 // [n_cache_pages, n_kv_heads, 64, head_dim], contiguous and 16-byte aligned.  head_dim: a multiple of 16 up to 128; n_heads / n_kv_heads at
-// most 128.  status: one int, left as it is unless a wait gave up (then 9).
-extern "C" int bn_attention_shared(const void* q, int q_stride, int n_seqs, int n_heads, int n_kv_heads, int head_dim, float scale,
-                                   const int* items, int n_items, const int* members, int n_members, const int* slots, const int* page_table,
-                                   int pt_stride, const void* k_cache, const void* v_cache, int n_cache_pages, float* part_o, float* part_ml,
-                                   int n_parts, int* status, cudaStream_t stream) {
+// most 128.  status: one int, left as it is unless a wait gave up (then 9, or the other kernel's).
+extern "C" int bn_attention_shared(BnDecodeJoin join, const void* qkv, int q_stride, int k_off, int v_off, void* out, int out_stride, int n_seqs, int n_heads,
+                                   int n_kv_heads, int head_dim, float scale, const int* items, int n_items, const int* members, int n_parts,
+                                   const int* sequences, const int* tok_pos, const int* slots, const int* page_table, int pt_stride, void* k_cache,
+                                   void* v_cache, int n_cache_pages, float* part_o, float* part_ml, int n_splits, int pages_per_block,
+                                   int* status, cudaStream_t stream) {
   if (n_items <= 0 || n_seqs <= 0) return BN_OK;
   if (head_dim <= 0 || head_dim % 16 || head_dim > 128 || n_kv_heads <= 0 || n_heads % n_kv_heads || n_heads / n_kv_heads > AS_ROWS || !(scale > 0.f) ||
-      q_stride % 8 || (long long)n_seqs * q_stride > 0x7fffffffll || n_items > 65535 || n_cache_pages <= 0 || !items || !members || !part_o || !part_ml || !status ||
-      (((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)items | (uintptr_t)part_o) & 15) || (((uintptr_t)members | (uintptr_t)part_ml) & 7))
+      q_stride % 8 || (long long)n_seqs * q_stride > 0x7fffffffll || n_items > 65535 || n_cache_pages <= 0 || !join || !items || !members || !part_o || !part_ml || !status ||
+      (((uintptr_t)qkv | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)items | (uintptr_t)part_o) & 15) || (((uintptr_t)members | (uintptr_t)part_ml) & 7))
     return BN_ERR_BAD_ARG;
   CUtensorMap mk, mv;
   if (!tma_map_bf16_pages(&mk, k_cache, n_cache_pages, (unsigned long long)n_kv_heads * BN_PAGE, head_dim, BN_PAGE) ||
       !tma_map_bf16_pages(&mv, v_cache, n_cache_pages, (unsigned long long)n_kv_heads * BN_PAGE, head_dim, BN_PAGE))
     return BN_ERR_BAD_ARG;
   AsArgs a = {};
-  a.q = (const __nv_bfloat16*)q; a.q_stride = q_stride; a.n_seqs = n_seqs; a.n_heads = n_heads; a.n_kv_heads = n_kv_heads; a.head_dim = head_dim;
+  a.q = (const __nv_bfloat16*)qkv; a.q_stride = q_stride; a.n_seqs = n_seqs; a.n_heads = n_heads; a.n_kv_heads = n_kv_heads; a.head_dim = head_dim;
   a.per_group = n_heads / n_kv_heads; a.scale_log2e = scale * 1.4426950408889634f; a.items = (const int4*)items; a.members = (const int2*)members;
-  a.n_members = n_members; a.n_parts = n_parts; a.slots = slots; a.page_table = page_table; a.pt_stride = pt_stride; a.part_o = part_o;
+  a.n_members = n_parts; a.n_parts = n_parts; a.slots = slots; a.page_table = page_table; a.pt_stride = pt_stride; a.part_o = part_o;
   a.part_ml = part_ml; a.status = status;
   // 64 KB and 96 KB: room for blocks of the sequences' own pages on the same SM (rings of three pages at head size 128: 36 and 40 us, 36 and 39 with two)
-  if (head_dim <= 64) return as_launch<64, 3, 3>(mk, mv, a, n_items, stream);
-  return as_launch<128, 2, 2>(mk, mv, a, n_items, stream);
+  const int rc = head_dim <= 64 ? as_launch<64, 3, 3>(mk, mv, a, n_items, stream) : as_launch<128, 2, 2>(mk, mv, a, n_items, stream);
+  if (rc != BN_OK) return rc;
+  return join(qkv, q_stride, k_off, v_off, out, out_stride, n_seqs, n_heads, n_kv_heads, head_dim, scale, tok_pos, slots, page_table, pt_stride, k_cache, v_cache,
+              n_cache_pages, status, n_splits, pages_per_block, sequences, part_o, part_ml, n_parts, stream);
 }

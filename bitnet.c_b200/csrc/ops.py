@@ -1262,23 +1262,24 @@ def attention_decode_shared(qkv: torch.Tensor, k_off: int, v_off: int, out: torc
             return attention_decode_fused(qkv, k_off, v_off, out, n_seqs, n_heads, n_kv_heads, head_dim, scale, 0, 0, 1.0, tok_pos, slots, page_table,
                                           k_cache, v_cache, plan.own_pages * PAGE)
         n_splits, pages_per_block = plan.own_grid()
-        counters = _split_scratch(device)[1]
-        # results of the shared pages, values and then (maximum, sum); a sequence's own splits are one cluster and need no room (nor tickets)
+        # results of the shared pages, values and then (maximum, sum); a sequence's own splits are one cluster and need no room
         results = plan.n_parts * n_heads
         room = torch.empty(results * (head_dim + 2), dtype=torch.float32, device=device)
         shared_o, shared_ml = c_void_p(room.data_ptr()), c_void_p(room.data_ptr() + 4 * results * head_dim)
         items, members, sequences = plan.pointers
-        status, stream, f_scale = _tc_status_arg(device), _stream(), c_float(scale)
-        p_qkv, p_pos, p_slots, p_table, p_k, p_v = _ptr(qkv), _ptr(tok_pos), _ptr(slots), _ptr(page_table), _ptr(k_cache), _ptr(v_cache)
-        pages, width = k_cache.shape[0], page_table.shape[1]
+        global LAUNCHES
+        LAUNCHES += 1  # the kernel that joins
         _check(_fn("attention_shared", "bn_attention_shared")(
-            p_qkv, row, n_seqs, n_heads, n_kv_heads, head_dim, f_scale, items, plan.n_items, members, plan.n_parts, p_slots, p_table, width, p_k, p_v, pages,
-            shared_o, shared_ml, plan.n_parts, status, stream), "attention_decode_shared")
-        _check(_fn("attention_decode_tc", "bn_attention_decode_tc_join")(
-            p_qkv, row, k_off, v_off, _ptr(out), out.shape[1], n_seqs, n_heads, n_kv_heads, head_dim, f_scale, p_pos, p_slots, p_table, width, p_k, p_v, pages,
-            status, shared_o, shared_ml, n_splits, pages_per_block, _ptr(counters), counters.numel(), sequences, shared_o, shared_ml, plan.n_parts, stream),
-            "attention_decode_shared")
+            _join_entry(), _ptr(qkv), row, k_off, v_off, _ptr(out), out.shape[1], n_seqs, n_heads, n_kv_heads, head_dim, c_float(scale), items, plan.n_items, members,
+            plan.n_parts, sequences, _ptr(tok_pos), _ptr(slots), _ptr(page_table), page_table.shape[1], _ptr(k_cache), _ptr(v_cache), k_cache.shape[0],
+            shared_o, shared_ml, n_splits, pages_per_block, _tc_status_arg(device), _stream()), "attention_decode_shared")
     return out
+
+
+@functools.lru_cache(maxsize=None)
+def _join_entry() -> c_void_p:
+    """``bn_attention_decode_tc_join``, which attention_shared.cu calls."""
+    return ctypes.cast(build.library("attention_decode_tc").bn_attention_decode_tc_join, c_void_p)
 
 
 SKINNY_MAX_ROWS = 16  # float32: warp-per-column kernel up to this many rows

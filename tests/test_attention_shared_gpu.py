@@ -237,3 +237,8 @@ def test_a_cache_behind_the_reach_of_32_bits(cuda_device):
     want = small.check()
     assert torch.equal(got, want)
     assert torch.equal(k[far:].view(torch.int16), small.k.view(torch.int16)) and torch.equal(v[far:].view(torch.int16), small.v.view(torch.int16))
+
+
+def test_seven_hundred_sequences(cuda_device):
+    # (more heads of sequences than there are tickets for splits that meet in memory: none are needed)
+    Batch(*forked(1, 700, 128, [3, 70]), 16, 16, 16, cuda_device).check()
