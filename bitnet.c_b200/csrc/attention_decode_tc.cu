@@ -174,7 +174,12 @@ attention_decode_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   // which sequence, which of its splits, of how many
-  int b = blockIdx.x, zi = blockIdx.z, nz = gridDim.z;
+  int b = blockIdx.x, y = blockIdx.y, zi = blockIdx.z, nz = gridDim.z;
+  if (JOIN) {  // blocks start in the order of x: all heads of a sequence, then the next one's, so that the longest start first
+    const int i = blockIdx.y * gridDim.x + blockIdx.x;
+    b = i / (int)gridDim.y;
+    y = i - b * (int)gridDim.y;
+  }
   if (a.items != nullptr) {
     const int item = a.items[blockIdx.x];
     if (item < 0) {  // padding: the whole cluster is, or its other blocks work alone
@@ -189,7 +194,7 @@ attention_decode_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
   const int head_dim = a.head_dim, n_kv_heads = a.n_kv_heads, n_heads = a.n_heads;
   const int group = n_heads / n_kv_heads;
   const int gblocks = (group + DT_ROWS - 1) / DT_ROWS;
-  const int kvh = blockIdx.y / gblocks, gb = blockIdx.y % gblocks;
+  const int kvh = y / gblocks, gb = y % gblocks;
   const int h0 = kvh * group + gb * DT_ROWS;
   const int G = min(DT_ROWS, group - gb * DT_ROWS);
   const int pos = a.tok_pos[b], slot = a.slots[b];  // (both asked for at once: what follows waits for both)
