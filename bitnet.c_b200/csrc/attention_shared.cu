@@ -13,9 +13,9 @@
 // S of the next page ahead of P V of this one, warps 2 to 5 copy the queries into shared memory and do the softmax, one row per thread.
 // P goes back to tensor memory over the columns S came from.  Every wait is bounded; a block whose wait gave up records it and stores nothing.
 //
-// A page takes a block about 0.8 us (its products, 17 % of the tensor cores' cycles, and its softmax follow one another); the list of work spreads the pages over one
-// block an SM, beside which the blocks of the sequences' own pages run.  Both kernels together, 32 heads on 8 of 128: 64 sequences behind 8,192 tokens with 500 of
-// their own 37 us (234 where each reads all its pages), 8 prompts of 2,048 by 8 with 300 of their own 31 us.
+// The bytes bound it, the list of work spreads the pages over five blocks on four SMs, beside which the blocks of the sequences' own pages run: a page takes a
+// block about 0.9 us, the tensor cores' part of which is a sixth.  Both kernels together, 32 heads on 8 of 128: 64 sequences behind 8,192 tokens with 500 of
+// their own 31.5 us (231 where each reads all its pages), 8 prompts of 2,048 by 8 with 300 of their own 25.7 us.
 #include "tma.cuh"
 #include "umma.cuh"
 
@@ -334,8 +334,9 @@ extern "C" int bn_attention_shared(BnDecodeJoin join, const void* qkv, int q_str
   a.per_group = n_heads / n_kv_heads; a.scale_log2e = scale * 1.4426950408889634f; a.items = (const int4*)items; a.members = (const int2*)members;
   a.n_members = n_parts; a.n_parts = n_parts; a.slots = slots; a.page_table = page_table; a.pt_stride = pt_stride; a.part_o = part_o;
   a.part_ml = part_ml; a.status = status;
-  // 64 KB and 96 KB: room for blocks of the sequences' own pages on the same SM (rings of three pages at head size 128: 36 and 40 us, 36 and 39 with two)
-  const int rc = head_dim <= 64 ? as_launch<64, 3, 3>(mk, mv, a, n_items, stream) : as_launch<128, 2, 2>(mk, mv, a, n_items, stream);
+  // 64 KB and 112 KB: room for blocks of the sequences' own pages on the same SM, or for a second one of these (128 KB with rings of three and three: 36 us where it is
+  // 27; 96 KB with two and two: 27.9)
+  const int rc = head_dim <= 64 ? as_launch<64, 3, 3>(mk, mv, a, n_items, stream) : as_launch<128, 3, 2>(mk, mv, a, n_items, stream);
   if (rc != BN_OK) return rc;
   return join(qkv, q_stride, k_off, v_off, out, out_stride, n_seqs, n_heads, n_kv_heads, head_dim, scale, tok_pos, slots, page_table, pt_stride, k_cache, v_cache,
               n_cache_pages, status, n_splits, pages_per_block, sequences, part_o, part_ml, n_parts, stream);

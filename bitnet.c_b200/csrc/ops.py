@@ -1156,9 +1156,9 @@ class SharedPlan:
         its results, places, which sequence; those with the most pages of their own first), and members (sequence, place)."""
         most = SHARED_ROWS // (self.n_heads // self.n_kv_heads)  # sequences of a block
         tiles = [(members[i:i + most], first, n) for members, first, n in self.runs for i in range(0, len(members), most)]
-        # one block an SM, which share all pages evenly: two would fit, but then the sequences' own pages wait until they have ended (8 prompts of 2,048 tokens by
-        # 8 sequences: 31 us with one, 37 with two; 64 sequences behind one of 8,192: 37 and 40)
-        budget = max(1, sms // self.n_kv_heads)
+        # five blocks on four SMs, which share all pages evenly: with one an SM some wait longest for their pages, with two the sequences' own pages wait until they
+        # have ended (8 prompts of 2,048 tokens by 8 sequences: 25.9 us, 27.2 with one, 32.8 with two; 64 sequences behind one of 8,192: 31.7, 31.6 and 36.2)
+        budget = max(1, 5 * sms // (4 * self.n_kv_heads))
         longest = max((n for _m, _f, n in tiles), default=1)
         each = min(longest, max(SHARED_MIN_PAGES, -(-sum(n for _m, _f, n in tiles) // budget)))
         work = []
@@ -1221,11 +1221,12 @@ def shared_plan(pages, n_heads: int, n_kv_heads: int, head_dim: int, device) -> 
 def shared_pays(plan: SharedPlan) -> bool:
     """Whether ``attention_decode_shared`` (with the rotation in front of it) gains over every sequence reading its pages for itself, by the pages of single heads
     that are read fewer times and the longest run.  Measured (us, without and with; 32 query heads on 8 of 128, completions of one prompt, 100 tokens
-    behind it): 4 of 4,096 tokens 12.8 / 12.3, 8 of 1,024 9.8 / 10.9, 8 of 2,048 14.4 / 12.9, 16 of 1,024 13.4 / 11.5, 64 of 256 16.9 / 18.3, 64 of 8,192 234 / 33;
-    8 prompts by 2 of 1,024 13.8 / 14.6, of 2,048 21.5 / 19.2; 40 heads on 40: 16 of 256 17.2 / 19.3, 8 by 2 of 1,024 43 / 49, 64 of 8,192 811 / 81."""
+    behind it): 4 of 4,096 tokens 12.6 / 12.9, 8 of 1,024 9.6 / 11.1, 8 of 2,048 14.2 / 13.2, 16 of 1,024 13.3 / 11.7, 64 of 256 16.6 / 17.7, 64 of 8,192 231 / 32;
+    8 prompts by 2 of 1,024 13.7 / 14.1, of 2,048 21.3 / 18.1; 40 heads on 40: 16 of 256 17.3 / 18.3, 8 by 2 of 1,024 43 / 47, 64 of 8,192 817 / 76.  In a recorded step,
+    between the products (what is saved in a layer): 4 of 4,096 -0.5, 8 of 2,048 -1.0, 16 of 1,024 0.4, 8 of 3,000 1.4, 8 of 4,096 4, 16 of 2,048 5.7."""
     saved = sum((len(members) - 1) * n for members, _first, n in plan.runs)
     longest = max((n for _members, _first, n in plan.runs), default=0)
-    return saved * plan.n_kv_heads >= 1500 and (longest >= 32 or (longest >= 8 and saved >= 0.6 * sum(plan.lengths)))
+    return saved * plan.n_kv_heads >= 1900 and (longest >= 32 or (longest >= 8 and saved >= 0.6 * sum(plan.lengths)))
 
 
 def attention_decode_shared(qkv: torch.Tensor, k_off: int, v_off: int, out: torch.Tensor, n_seqs: int, n_heads: int, n_kv_heads: int, head_dim: int,

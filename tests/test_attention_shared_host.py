@@ -80,7 +80,7 @@ def test_refused():
         ops.SharedPlan([[1], []], 8, 8, 64, "cpu", sms=148)
 
 
-@pytest.mark.parametrize("shared,each,prompts,kv,pays", [(64, 4, 1, 8, True), (16, 8, 1, 8, False), (32, 8, 1, 8, True), (16, 16, 1, 8, True), (4, 64, 1, 8, False),
+@pytest.mark.parametrize("shared,each,prompts,kv,pays", [(64, 4, 1, 8, False), (128, 4, 1, 8, True), (16, 8, 1, 8, False), (32, 8, 1, 8, False), (46, 8, 1, 8, True), (16, 16, 1, 8, True), (4, 64, 1, 8, False),
                                                          (16, 2, 8, 8, False), (32, 2, 8, 8, True), (16, 2, 8, 40, False), (1, 64, 1, 40, False), (0, 64, 1, 8, False)])
 def test_where_it_pays(shared, each, prompts, kv, pays):
     pages = [[10 ** 4 * p + i for i in range(shared)] + [10 ** 6 + p * each + e, 10 ** 7 + p * each + e] for p in range(prompts) for e in range(each)]
