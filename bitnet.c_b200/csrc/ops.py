@@ -7,9 +7,11 @@ back to the CPU: tensors that are not on a CUDA device are refused.
 """
 from __future__ import annotations
 
+import array
 import contextlib
 import ctypes
 import functools
+import itertools
 from ctypes import c_float, c_int, c_void_p
 from typing import Optional
 
@@ -1815,22 +1817,30 @@ def zero_slot(rows: torch.Tensor, slot: int) -> None:
 def _page_moves(moves, pages: int):
     """``copy_pages``' moves as the kernel takes them: groups of (source, rows, number of destinations) and their destinations; refuses what does not
     name pages of the cache, and destinations that another move reads or writes."""
-    groups = {}
-    for src, dst, rows in moves:
-        if not (0 <= src < pages and 0 <= dst < pages):
-            raise KernelError(f"copy_pages: page {src if not 0 <= src < pages else dst} is outside the {pages} pages of the cache")
-        if not 0 < rows <= PAGE:
-            raise KernelError(f"copy_pages: {rows} rows of a page of {PAGE}")
-        to = groups.get((src, rows))
-        if to is None:
-            groups[src, rows] = [dst]
-        else:
-            to.append(dst)
-    to = [d for g in groups.values() for d in g]
-    written = set(to)
-    if len(written) != len(to) or any(src in written for src, _rows in groups):
+    moves = list(moves)
+    if not moves:
+        return [], []
+    src, dst, rows = zip(*moves)
+    if min(src) < 0 or max(src) >= pages or min(dst) < 0 or max(dst) >= pages:
+        raise KernelError(f"copy_pages: page {next(p for p in (*src, *dst) if not 0 <= p < pages)} is outside the {pages} pages of the cache")
+    fewest, most = min(rows), max(rows)
+    if fewest < 1 or most > PAGE:
+        raise KernelError(f"copy_pages: {next(r for r in rows if not 0 < r <= PAGE)} rows of a page of {PAGE}")
+    sources = set(src)
+    if len(set(dst)) != len(dst) or not sources.isdisjoint(dst):
         raise KernelError("copy_pages: a page that is written must be written once and not read")
-    return [x for (src, rows), dst in groups.items() for x in (src, rows, len(dst))], to
+    if len(sources) == 1 and fewest == most:  # one group
+        return [src[0], most, len(dst)], list(dst)
+    if len(sources) == len(src):  # every move is a group of its own
+        return list(itertools.chain.from_iterable(zip(src, rows, itertools.repeat(1)))), list(dst)
+    groups = {}
+    for p, d, r in moves:
+        to = groups.get((p, r))
+        if to is None:
+            groups[p, r] = [d]
+        else:
+            to.append(d)
+    return [x for (p, r), to in groups.items() for x in (p, r, len(to))], [d for to in groups.values() for d in to]
 
 
 def copy_pages(k: torch.Tensor, v: Optional[torch.Tensor], moves) -> None:
@@ -1852,13 +1862,14 @@ def copy_pages(k: torch.Tensor, v: Optional[torch.Tensor], moves) -> None:
     groups, to = _page_moves(moves, pages)
     if not to:
         return
-    n, listed = len(groups) // 3, (c_int * (len(groups) + len(to)))(*groups, *to)
+    n, listed = len(groups) // 3, array.array("i", groups + to)
+    where = c_void_p(listed.buffer_info()[0])
     with _on(k.device):
         for one, h, width, other, other_width in both:
             if planes and h and width:
                 _check(_fn("cache_pages", "bn_copy_pages")(
                     _ptr(one), _ptr(other), planes, pages, h, width * one.element_size(), other_width * other.element_size() if other is not None else 0,
-                    listed, n, len(to), _stream()), "copy_pages")
+                    where, n, len(to), _stream()), "copy_pages")
 
 
 class StateSlots:
