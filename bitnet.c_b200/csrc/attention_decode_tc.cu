@@ -713,7 +713,7 @@ static long long dt_slots() {
 // sequences = 320 blocks: 77 us with three stages in two waves, 53 us with two stages in one).
 template <int HD, bool JOIN>
 static int launch_dt(const CUtensorMap& mk, const CUtensorMap& mv, const DtArgs& a, dim3 grid, dim3 cluster, cudaStream_t stream) {
-  // (with JOIN always two: a third block an SM gains more beside the shared pages' blocks; 64 sequences of up to 9 pages of their own: 38 us, 40 with three)
+  // (with JOIN always two: a third block an SM gains more beside the shared pages' blocks; 64 sequences of up to 9 pages of their own: 31.5 us, 36 with three)
   if (JOIN || a.pages_per_block <= 2) return launch_dt2<HD, 2, JOIN>(mk, mv, a, grid, cluster, stream);
   const long long blocks = (long long)grid.x * grid.y * grid.z;
   const long long s3 = dt_slots<HD, 3>(), s2 = dt_slots<HD, 2>();

@@ -15,9 +15,9 @@
 // same side as in a sum of doubles (a float sum would move a token in a thousand).  2^-y is taken apart into 2^-(j/32) from a table, a shift, and
 // 1 - e of a remainder below 1/32, whose e is small enough for a float: y = (max - l) / T * log2(e) is carried in two floats.
 //
-// Measured: one row of 32,000 with top-k 13.5 us, 8 rows of 128,256 with top-p 19.5, 64 rows of 128,256 with parameters of their own 54, 200 flat
-// rows of 50,257 in bfloat16 67.  Few rows are bound by latency (the first block's plan takes 6 us, handing over and deciding 5), many by the additions in shared
-// memory (2.8 cycles a warp's where no lanes meet) and some 40 instructions a key.
+// Measured: one row of 32,000 with top-k 11.3 us, 8 rows of 128,256 with top-p 17.9, 64 rows of 128,256 with parameters of their own 35.6, 200 flat
+// rows of 50,257 in bfloat16 53.5.  Few rows are bound by latency (the first block's plan takes 5.5 us, handing over and deciding 2.7, the cluster's barriers 2.5), many by some
+// 66 instructions a number, two additions in shared memory (2.8 cycles a warp's where no lanes meet) among them.
 #include "common.cuh"
 #include <math.h>
 
@@ -278,16 +278,16 @@ struct SfRow {
 
   // ---- by steps of weight ----
   // The step of a logit (falling logits, rising steps: the nearest to y), and what its y is from the 32nd of an octave that the step lies in.  Conversions
-  // by adding 1.5 * 2^23: those of the conversion unit take four times the issue slots.
+  // by adding 1.5 * 2^23: those of the conversion unit take four times the issue slots.  (Whatever the logit, the step is one of those that there are.)
   __device__ __forceinline__ int step_of(float v, float* rest) const {
     const float d = topf - v, bb = d - topf, dl = (topf - (d - bb)) - (v + bb);
     const float y = d * c_hi, yl = fmaf(d, c_hi, -y) + fmaf(d, c_lo, dl * c_hi);
-    const int n = min(__float_as_int(fmaf(fminf(y, 64.f), steps, 12582912.f)) - 0x4B400000, SF_STEPS - 1);
+    const int n = (int)min((unsigned)__float_as_int(fmaf(fminf(y, 64.f), steps, 12582912.f)) - 0x4B400000u, SF_STEPS - 1u);
     *rest = fmaf(__int_as_float((n >> fine) + 0x4B400000) - 12582912.f, -1.f / 32.f, y) + yl;
     return n;
   }
   __device__ __forceinline__ int step_of(float v) const {
-    return min(__float_as_int(fmaf(fminf((topf - v) * c_hi, 64.f), steps, 12582912.f)) - 0x4B400000, SF_STEPS - 1);
+    return (int)min((unsigned)__float_as_int(fmaf(fminf((topf - v) * c_hi, 64.f), steps, 12582912.f)) - 0x4B400000u, SF_STEPS - 1u);
   }
   // 1 - 2^-rest
   static __device__ __forceinline__ float short_of(float rest) {
@@ -859,7 +859,6 @@ __global__ void __launch_bounds__(SF_THREADS, 1024 / SF_THREADS) sample_filtered
   const int r = blockIdx.x / blocks;
   const int first = min(a.vocab, (int)rank * a.per);
   SfRow<T, RESIDENT> row{a, s, held, (const T*)a.logits + (size_t)r * a.ld + first, min(a.vocab, first + a.per) - first, rank, blocks};
-  if (blocks > 1) sf_arrive();
   for (int b = threadIdx.x; b < SF_STEPS; b += SF_THREADS) s.one[b] = s.two[b] = 0;
   if (threadIdx.x < 32) {
     const unsigned long long x = a.table[threadIdx.x];
@@ -867,6 +866,7 @@ __global__ void __launch_bounds__(SF_THREADS, 1024 / SF_THREADS) sample_filtered
     s.small_table[threadIdx.x] = (int)((x + (1ull << (SF_POINT - 31))) >> (SF_POINT - 30));
   }
   if (threadIdx.x == 0) s.high = s.low = s.listed = s.noted = 0;
+  if (blocks > 1) sf_arrive();  // behind what this thread has set: whoever has waited finds it, in this block too
   pdl_wait();
   const float temperature = a.temperatures ? a.temperatures[r] : a.temperature;
   const float top_p = a.top_ps ? a.top_ps[r] : a.top_p, asked = a.min_ps ? a.min_ps[r] : a.min_p;
@@ -998,15 +998,15 @@ static int sf_run(SfArgs& a, int n_rows, cudaStream_t stream) {
   cudaError_t e = cudaGetDevice(&device);
   if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
   if (e != cudaSuccess) return BN_ERR_LAUNCH + (int)e;
-  // Blocks of a row: so many that each has 4,096 numbers (one row of 1,000: 10 us with one block, 13 with eight; of 32,000: 18 with one, 14 with eight), but not
-  // more than 2.75 an SM in all, of which two run at once (64 rows of 128,256: 53 us with four blocks a row, 62 with eight; 200 of 50,257: 69 with two, 82 with
+  // Blocks of a row: so many that each has 4,096 numbers (one row of 32,000: 16.2 us with one block, 14.1 with two, 12.4 with eight), but not
+  // more than 2.75 an SM in all, of which two run at once (64 rows of 128,256: 37 us with four blocks a row, 51 with eight; 200 of 50,257: 54 with two, 65 with
   // four).  Fewer than hold a row's sums only where even one block a row has too many numbers.
   int blocks = SF_MAX_CLUSTER;
   while (blocks > 1 && a.vocab <= blocks / 2 * 4096) blocks /= 2;
   while (blocks > 1 && 4ll * n_rows * blocks > 11ll * sms && (a.vocab + blocks / 2 - 1) / (blocks / 2) <= SF_COUNTED - 8) blocks /= 2;
   a.per = (((a.vocab + blocks - 1) / blocks) + 7) & ~7;
   // The row stays in shared memory where two blocks an SM still fit, or where there is one at most; else later passes find it in the L2 (256 rows of 32,000 in float32,
-  // one block each: 37 us from the L2, 46 held).
+  // one block each: 45 us from the L2, 53 held).
   const size_t base = (sizeof(SfShared) + 15) & ~(size_t)15, held = (((size_t)a.per * sizeof(T)) + 15) & ~(size_t)15;
   const bool resident = base + held <= ((long long)n_rows * blocks <= sms ? 220 : 112) * 1024 && a.per <= 128 * SF_THREADS;
   return resident ? sf_launch<T, true>(a, n_rows, blocks, base + held, stream) : sf_launch<T, false>(a, n_rows, blocks, base, stream);

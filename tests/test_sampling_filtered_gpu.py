@@ -206,3 +206,19 @@ def test_more_rows_than_16_bits_count(cuda_device):
     k = torch.randint(1, 4, (70001,), generator=torch.Generator().manual_seed(4)).int().to(cuda_device)
     got = ops.sample_filtered(x, 1e-6, top_k=k, u=torch.full_like(u, 0.999))  # (the first two logits of a row may be as good as equal)
     assert (x.gather(1, got[:, None].long())[:, 0] >= x.amax(1) - 2e-5).all()
+
+
+@pytest.mark.parametrize("n,vocab", [(48, 32000), (80, 40000), (300, 32000)])
+def test_more_blocks_than_run_at_once_again_and_again(cuda_device, n, vocab):
+    # blocks of a second wave begin while others end: what a block sets at its beginning must be there for all of its warps
+    logits, u = rows(n, vocab, 3.0, 21)
+    x, u = logits.to(cuda_device), u.to(cuda_device)
+    want = ops.sample_filtered(x, 0.9, 0, 0.9, u=u)
+    best = ops.sample_filtered(x, 0.9, 1, u=u)
+    assert torch.equal(best, x.argmax(1).int())
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = [ops.sample_filtered(x, 0.9, 0, 0.9, u=u) for _ in range(20)]
+    for _ in range(30):
+        g.replay()
+        assert all(torch.equal(t, want) for t in got)
