@@ -1000,9 +1000,11 @@ static int sf_run(SfArgs& a, int n_rows, cudaStream_t stream) {
   if (e != cudaSuccess) return BN_ERR_LAUNCH + (int)e;
   // Blocks of a row: so many that each has 4,096 numbers (one row of 32,000: 16.2 us with one block, 14.1 with two, 12.4 with eight), but not
   // more than 2.75 an SM in all, of which two run at once (64 rows of 128,256: 37 us with four blocks a row, 51 with eight; 200 of 50,257: 54 with two, 65 with
-  // four).  Fewer than hold a row's sums only where even one block a row has too many numbers.
+  // four).  Clusters of eight only for some ten rows: more of them do not find their place at once (12 rows of 128,256: 22.0 us with eight, 20.3 with four; 10: 19.8 and 20.2;
+  // 40: 36.8 and 31.5).  No fewer blocks than add up a row's numbers.
   int blocks = SF_MAX_CLUSTER;
   while (blocks > 1 && a.vocab <= blocks / 2 * 4096) blocks /= 2;
+  if (blocks == 8 && 64ll * n_rows > 5ll * sms && (a.vocab + 3) / 4 <= SF_COUNTED - 8) blocks = 4;
   while (blocks > 1 && 4ll * n_rows * blocks > 11ll * sms && (a.vocab + blocks / 2 - 1) / (blocks / 2) <= SF_COUNTED - 8) blocks /= 2;
   a.per = (((a.vocab + blocks - 1) / blocks) + 7) & ~7;
   // The row stays in shared memory where two blocks an SM still fit, or where there is one at most; else later passes find it in the L2 (256 rows of 32,000 in float32,
