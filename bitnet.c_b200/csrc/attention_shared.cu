@@ -15,7 +15,7 @@
 //
 // The bytes bound it, the list of work spreads the pages over five blocks on four SMs, beside which the blocks of the sequences' own pages run: a page takes a
 // block about 0.9 us, the tensor cores' part of which is a sixth.  Both kernels together, 32 heads on 8 of 128: 64 sequences behind 8,192 tokens with 500 of
-// their own 31.5 us (231 where each reads all its pages), 8 prompts of 2,048 by 8 with 300 of their own 25.7 us.
+// their own 31.8 us (231 where each reads all its pages), 8 prompts of 2,048 by 8 with 300 of their own 26.3 us.
 #include "tma.cuh"
 #include "umma.cuh"
 
@@ -106,8 +106,8 @@ attention_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
   const unsigned tmem_base = *tmem_slot;
 
   if (warp == 0) {
+    pdl_wait();  // (whatever filled the pages may still run before that: pages asked for in front of it gain 0.5 us of 26 for 64 sequences, less for others)
     if (lane == 0) {
-      // Shared pages were filled before the kernel in front of this one began, which brings the queries: they are asked for before the wait.
       auto request = [&](int j, bool values) -> bool {
         const int n = values ? VS : KS, s = j % n, round = j / n;
         const unsigned empty = (values ? v_empty0 : k_empty0) + 8 * s, bar = (values ? v_full0 : k_full0) + 8 * s;

@@ -242,3 +242,36 @@ def test_a_cache_behind_the_reach_of_32_bits(cuda_device):
 def test_seven_hundred_sequences(cuda_device):
     # (more heads of sequences than there are tickets for splits that meet in memory: none are needed)
     Batch(*forked(1, 700, 128, [3, 70]), 16, 16, 16, cuda_device).check()
+
+
+@pytest.mark.parametrize("heads,kv,dim,prompts,each,shared,tails", [(32, 8, 64, 1, 4, 200, [40]), (32, 8, 128, 4, 8, 1000, [300, 2]), (12, 4, 80, 2, 7, 3000, [500, 0, 64])])
+def test_between_products(cuda_device, heads, kv, dim, prompts, each, shared, tails):
+    # recorded, every kernel may begin before the one in front has ended; the results are those of launches with a full stop in between, bit for bit
+    b = Batch(*forked(prompts, each, shared, tails), heads, kv, dim, cuda_device)
+    plan, n = b.plan(), prompts * each
+    g = torch.Generator().manual_seed(5)
+    w, w2 = ((torch.randn(s, generator=g) * 0.03).to(torch.bfloat16).to(cuda_device) for s in (((heads + 2 * kv) * dim, 512), (512, heads * dim)))
+    x = torch.zeros(n, 512, dtype=torch.bfloat16, device=cuda_device)
+
+    def run(stop):
+        wait = torch.cuda.synchronize if stop else (lambda: None)
+        qkv = ops.linear(x, w)
+        wait()
+        ops.rope_append(qkv, heads + kv, dim, dim, 0.9, b.tok_pos)
+        wait()
+        out = torch.empty_like(b.out)
+        ops.attention_decode_shared(qkv, heads * dim, (heads + kv) * dim, out, n, heads, kv, dim, b.scale, b.tok_pos, b.slots, b.table, b.k, b.v, plan)
+        wait()
+        return out, ops.linear(out, w2)
+
+    run(True)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = [run(False) for _ in range(4)]
+    for turn in range(25):
+        x.copy_(torch.randn(n, 512, generator=g).to(torch.bfloat16))
+        graph.replay()
+        torch.cuda.synchronize()
+        want = run(True)
+        for pair in got:
+            assert torch.equal(pair[0], want[0]) and torch.equal(pair[1], want[1])
