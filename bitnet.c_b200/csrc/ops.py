@@ -1847,29 +1847,32 @@ def copy_pages(k: torch.Tensor, v: Optional[torch.Tensor], moves) -> None:
     """For every move (source page, destination page, rows) the first ``rows`` rows of every head of the source page are copied to the destination page, in
     all planes, of keys and of values.  ``k`` [planes, pages, heads, 64, numbers] of any type, ``v`` the same with a width of its own, or None;
     ``moves`` is a sequence on the host, read before the call returns.  A page that is written is written once and not read."""
-    _need(k, "k", dims=5)
+    _need(k, "k", None, 5)
     planes, pages, heads, page, dim = k.shape
     if page != PAGE:
         raise KernelError(f"copy_pages: k {tuple(k.shape)} is not [planes, pages, heads, {PAGE}, numbers]")
-    both = [(k, heads, dim, None, 0)]
+    v_row, apart = 0, False
     if v is not None:
-        _need(v, "v", dims=5)
+        _need(v, "v", None, 5)
         v_planes, v_pages, v_heads, v_page, v_dim = v.shape
         if v_planes != planes or v_pages != pages or v_page != PAGE or v.get_device() != k.get_device():
             raise KernelError(f"copy_pages: v {tuple(v.shape)} on {v.device} does not go with k {tuple(k.shape)} on {k.device}")
+        v_row = v_dim * v.element_size()
         # keys and values with different numbers of heads are copied one after the other
-        both = [(k, heads, dim, v, v_dim)] if v_heads == heads and dim and v_dim else [*both, (v, v_heads, v_dim, None, 0)]
+        apart = v_heads != heads or not dim or not v_dim
     groups, to = _page_moves(moves, pages)
-    if not to:
+    if not to or not planes:
         return
     n, listed = len(groups) // 3, array.array("i", groups + to)
-    where = c_void_p(listed.buffer_info()[0])
+    where, row = c_void_p(listed.buffer_info()[0]), dim * k.element_size()
     with _on(k.device):
-        for one, h, width, other, other_width in both:
-            if planes and h and width:
-                _check(_fn("cache_pages", "bn_copy_pages")(
-                    _ptr(one), _ptr(other), planes, pages, h, width * one.element_size(), other_width * other.element_size() if other is not None else 0,
-                    where, n, len(to), _stream()), "copy_pages")
+        if not apart:
+            if heads and row:
+                _check(_fn("cache_pages", "bn_copy_pages")(_ptr(k), _ptr(v), planes, pages, heads, row, v_row, where, n, len(to), _stream()), "copy_pages")
+            return
+        for t, h, width in ((k, heads, row), (v, v_heads, v_row)):
+            if h and width:
+                _check(_fn("cache_pages", "bn_copy_pages")(_ptr(t), _NOWHERE, planes, pages, h, width, 0, where, n, len(to), _stream()), "copy_pages")
 
 
 class StateSlots:
