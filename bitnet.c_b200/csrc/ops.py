@@ -1114,6 +1114,7 @@ class SharedPlan:
         self.runs, self.first_own = shared_runs([p[:-1] for p in pages])  # the last page takes the new token: it is nobody else's
         self.own_pages = max((len(p) - f for p, f in zip(pages, self.first_own)), default=0)
         self.lengths = [len(p) for p in pages]
+        self.longest = max(self.lengths, default=0)
         self.deepest = max(self.first_own, default=0)
         self._grid = None
         self._lay_out(sms if sms is not None else n_sms(self.device))
@@ -1233,10 +1234,19 @@ def shared_pays(plan: SharedPlan) -> bool:
 
 def attention_decode_shared(qkv: torch.Tensor, k_off: int, v_off: int, out: torch.Tensor, n_seqs: int, n_heads: int, n_kv_heads: int, head_dim: int,
                             scale: float, tok_pos: torch.Tensor, slots: torch.Tensor, page_table: torch.Tensor, k_cache: torch.Tensor,
-                            v_cache: torch.Tensor, plan: SharedPlan) -> torch.Tensor:
+                            v_cache: torch.Tensor, max_len=None, plan: Optional[SharedPlan] = None) -> torch.Tensor:
     """``attention_decode_fused`` for sequences that share pages: pages that several of them begin with are read once for all (``plan``, of
     ``shared_plan``), each sequence's own pages as ever, and the two are joined, in two launches.  ``qkv`` holds rotated q|k|v rows; the new key and
-    value are written into the cache at ``tok_pos``.  No window; heads of at most 128."""
+    value are written into the cache at ``tok_pos``.  No window; heads of at most 128.  ``max_len``: no sequence is longer, its new token included; it may be
+    left out, also where arguments go by their place (``..., v_cache, plan``): the plan knows it to a page."""
+    if isinstance(max_len, SharedPlan):
+        if plan is not None:
+            raise KernelError("attention_decode_shared: two plans")
+        max_len, plan = None, max_len
+    if not isinstance(plan, SharedPlan):
+        raise KernelError("attention_decode_shared: plan must be one of shared_plan")
+    if max_len is not None and max_len <= (plan.longest - 1) * PAGE:
+        raise KernelError(f"attention_decode_shared: the plan is for sequences of up to {plan.longest} pages, more than max_len={max_len} needs")
     _need(qkv, "qkv", torch.bfloat16, 2)
     _need(out, "out", torch.bfloat16, 2)
     for t, nm in ((tok_pos, "tok_pos"), (slots, "slots")):
