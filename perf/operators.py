@@ -134,7 +134,8 @@ def _prepare_attend(case, g, host):
     v = _normal((pool, KV, PAGE, D), torch.bfloat16, g)
     state = dict(case, k=k, v=v, qkv=_normal((B, (H + 2 * KV) * D), torch.bfloat16, g), scale=D ** -0.5,
                  pos=torch.tensor(pos, dtype=torch.int32, device=DEVICE), slots=torch.arange(B, dtype=torch.int32, device=DEVICE),
-                 table=torch.tensor(rows, dtype=torch.int32, device=DEVICE), out=torch.empty((B, H * D), dtype=torch.bfloat16, device=DEVICE))
+                 table=torch.tensor(rows, dtype=torch.int32, device=DEVICE), out=torch.empty((B, H * D), dtype=torch.bfloat16, device=DEVICE),
+                 longest=max(pos) + 1)
     if own:  # which sequences share which pages: follows the page tables alone, made when a sequence takes a new page
         from bitnet_c_b200.csrc import ops
         state["plan"] = ops.shared_plan([r[:p // PAGE + 1] for r, p in zip(rows, pos)], H, KV, D, DEVICE)
@@ -189,7 +190,7 @@ def _run_attend(s):
     if own:
         from bitnet_c_b200.csrc import ops
         ops.attention_decode_shared(s["qkv"], H * D, (H + KV) * D, s["out"], B, H, KV, D, s["scale"], s["pos"], s["slots"], s["table"],
-                                    s["k"], s["v"], s["plan"])
+                                    s["k"], s["v"], s["longest"], s["plan"])
         return s["out"], s["k"], s["v"]
     pos = s["pos"].long()
     q, new_k, new_v = s["qkv"].split([H * D, KV * D, KV * D], 1)
