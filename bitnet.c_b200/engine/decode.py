@@ -132,8 +132,9 @@ class DecodeRunner:
             return
         now = (slots, self.cache.turns) if self.cache.shares_pages() else None
         if now != self.shared_for:
-            self.shared_for = now
+            self.ctx.shared = self.shared_for = None  # (a plan that cannot be made leaves no old one behind)
             self.ctx.shared = self._shared_plan(slots, positions) if now is not None else None
+            self.shared_for = now
         if self.ctx.shared is not None:
             own = max(p // PAGE + 1 - first for p, first in zip(positions, self.ctx.shared.first_own))
             self.ctx.shared.own_pages = _bucket(own)
