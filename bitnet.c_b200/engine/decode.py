@@ -150,6 +150,7 @@ class DecodeRunner:
             table = torch.zeros(len(plan.host), dtype=torch.int32, device=self.model.device)
         if held != plan.host:
             self.h2d_bytes += 4 * len(plan.host)
+            self.shared_tables[size] = table, None  # what it holds is known again when the upload has been issued
             plan.upload(table)
             self.shared_tables[size] = table, plan.host
         plan.point_at(table)

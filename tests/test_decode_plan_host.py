@@ -64,3 +64,32 @@ def test_a_plan_that_could_not_be_made_leaves_no_old_one():
     model.fails = False
     runner._shared_pages(slots, positions)
     assert runner.ctx.shared.runs == [([0, 2, 3], 0, 5)] and runner.ctx.shared.first_own == [5, 0, 5, 5]
+
+
+def test_an_upload_that_failed_is_issued_again(monkeypatch):
+    cache, slots = cache_of(64 * 5 + 3, 4)
+    runner = DecodeRunner(TwoHeads(), cache, None, 4)
+    runner._shared_pages(slots, new_tokens(cache, slots))
+    table, first = runner.ctx.shared.table, list(runner.ctx.shared.host)
+    cache.close(slots[1])
+    cache.open()  # (the same slot)
+    cache.reserve(slots[1], 200)
+    cache.advance(slots[1], 200)
+    positions = new_tokens(cache, slots)
+    upload = ops.SharedPlan.upload
+
+    def half(plan, to=None):
+        upload(plan, to)
+        raise RuntimeError("the copy was cut short")
+
+    monkeypatch.setattr(ops.SharedPlan, "upload", half)
+    with pytest.raises(RuntimeError, match="cut short"):
+        runner._shared_pages(slots, positions)
+    monkeypatch.setattr(ops.SharedPlan, "upload", upload)
+    # the first plan again: the buffer of its size holds something else by now
+    cache2, slots2 = cache_of(64 * 5 + 3, 4)
+    runner.cache = cache2
+    assert slots2 == slots
+    runner._shared_pages(slots2, new_tokens(cache2, slots2))
+    assert runner.ctx.shared.host == first and runner.ctx.shared.table[:len(first)].tolist() == first
+    assert runner.ctx.shared.table is table
