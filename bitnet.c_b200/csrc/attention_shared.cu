@@ -9,7 +9,7 @@
 // every new token), so nothing is masked.
 //
 // Which block works on what is a list made on the host: (first member, members and the first one's sequence, first page, pages) per item, members as (sequence, where its
-// results go).  Blocks and roles as in attention_prefill_tc.cu: warp 0 requests pages (TMA, 128-byte swizzle), warp 1 issues the MMAs,
+// results go).  Copies bring it to the device, which no kernel overlaps, so it is read in front of the wait; all else is read behind it.  Blocks and roles as in attention_prefill_tc.cu: warp 0 requests pages (TMA, 128-byte swizzle), warp 1 issues the MMAs,
 // S of the next page ahead of P V of this one, warps 2 to 5 copy the queries into shared memory and do the softmax, one row per thread.
 // P goes back to tensor memory over the columns S came from.  Every wait is bounded; a block whose wait gave up records it and stores nothing.
 //
@@ -80,7 +80,6 @@ attention_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
   }
   const int rows = min(AS_ROWS, n_members * a.per_group);
   const int2* members = a.members + item.x;
-  const int* pt = a.page_table + (size_t)a.slots[item.y >> 8] * a.pt_stride + item.z;
 
   if (tid == 0) {
     *failed = 0;
@@ -106,8 +105,10 @@ attention_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
   const unsigned tmem_base = *tmem_slot;
 
   if (warp == 0) {
-    pdl_wait();  // (whatever filled the pages may still run before that: pages asked for in front of it gain 0.5 us of 26 for 64 sequences, less for others)
+    // (whatever filled the pages, or chose the slots, may still run before that: pages asked for in front of it gain 0.5 us of 26 for 64 sequences, less for others)
+    pdl_wait();
     if (lane == 0) {
+      const int* pt = a.page_table + (size_t)a.slots[item.y >> 8] * a.pt_stride + item.z;
       auto request = [&](int j, bool values) -> bool {
         const int n = values ? VS : KS, s = j % n, round = j / n;
         const unsigned empty = (values ? v_empty0 : k_empty0) + 8 * s, bar = (values ? v_full0 : k_full0) + 8 * s;

@@ -20,3 +20,39 @@ def test_with_the_length_bound(cuda_device, prompts, each, shared, tails):
         assert torch.equal(call(bound, plan), want)
     with pytest.raises(ops.KernelError, match="max_len"):
         call((longest - 1) // 64 * 64, plan)
+
+
+def test_slots_that_the_kernel_in_front_writes(cuda_device):
+    # the sampler lets its successor begin at once, and its tokens are the slots: a call that read them early would find those of the turn before
+    b = Batch(*forked(2, 4, 64 * 9, [5, 64 * 3, 130, 0]), 8, 2, 64, cuda_device)
+    plan, n = b.plan(), len(b.pos)
+    want = b.check(plan).clone()
+    rows = b.table.shape[0]
+    logits, u = torch.empty((n, rows), device=cuda_device), torch.zeros(n, device=cuda_device)
+    table = torch.empty_like(b.table)
+    slots, positions = b.slots.clone(), b.tok_pos.clone()
+    out = torch.empty_like(b.out)
+
+    def run():
+        ops.sample_filtered(logits, 1.0, u=u, out=slots)
+        ops.attention_decode_shared(b.qkv, 512, 640, out, n, 8, 2, 64, b.scale, positions, slots, table, b.k, b.v, plan)
+
+    def put(order):  # sequence i in slot order[i]
+        logits.fill_(-float("inf"))
+        logits[torch.arange(n), order] = 1.0
+        table.fill_(b.pages[0][0])  # (every entry names a page: another sequence's would be read)
+        table[order] = b.table[b.slots.long()]
+
+    orders = [torch.randperm(rows, generator=torch.Generator().manual_seed(s))[:n].to(cuda_device) for s in range(12)]
+    put(orders[0])
+    run()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run()
+    for order in orders[1:]:
+        put(order)
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(slots.long(), order) and torch.equal(out, want)
+    ops.check_tc_status(cuda_device)
