@@ -5,7 +5,7 @@
 // sequences, are the 128 rows of the products
 //     S = Q K^T  (per page: M=128, N=64, K=head size),   P = exp2(S * scale * log2(e) - m),   O += P V
 // and every row leaves its maximum m, its sum of P and its unnormalised O in float32.  The kernel that attends over a sequence's own
-// pages (attention_decode_tc.cu) reads them and joins them with its own.  All keys of a run are visible to all its rows (a run ends in front of
+// pages (attention_decode_tc.cuh) reads them and joins them with its own.  All keys of a run are visible to all its rows (a run ends in front of
 // every new token), so nothing is masked.
 //
 // Which block works on what is a list made on the host: (first member, members and the first one's sequence, first page, pages) per item, members as (sequence, where its
@@ -16,7 +16,7 @@
 // The bytes bound it, the list of work spreads the pages over five blocks on four SMs, beside which the blocks of the sequences' own pages run: a page takes a
 // block about 0.9 us, the tensor cores' part of which is a sixth.  Both kernels together, 32 heads on 8 of 128: 64 sequences behind 8,192 tokens with 500 of
 // their own 31.8 us (231 where each reads all its pages), 8 prompts of 2,048 by 8 with 300 of their own 26.3 us.
-#include "tma.cuh"
+#include "attention_decode_tc.cuh"
 #include "umma.cuh"
 
 #define AS_ROWS 128
@@ -305,26 +305,20 @@ static int as_launch(const CUtensorMap& mk, const CUtensorMap& mv, const AsArgs&
   return BN_OK;
 }
 
-// bn_attention_decode_tc_join of attention_decode_tc.cu
-typedef int (*BnDecodeJoin)(const void* qkv, int q_stride, int k_off, int v_off, void* out, int out_stride, int n_seqs, int n_heads, int n_kv_heads, int head_dim,
-                            float scale, const int* tok_pos, const int* slots, const int* page_table, int pt_stride, void* k_cache, void* v_cache,
-                            int n_cache_pages, int* status, int n_splits, int pages_per_block, const int* shared,
-                            const float* shared_o, const float* shared_ml, int n_shared, cudaStream_t stream);
-
-// The kernel above and behind it `join` (one call from the host: two take it 3 us more).  qkv: [n_seqs, q_stride] bfloat16 rows, rotated, query head h at
+// The kernel above and directly behind it the joining form of attention_decode_tc.cuh (one call from the host: two take it 3 us more; and that form relies on what is in front).  qkv: [n_seqs, q_stride] bfloat16 rows, rotated, query head h at
 // element h * head_dim, key heads at k_off, value heads at v_off, 16-byte aligned, q_stride a multiple of 8.  items [n_items], members [n_parts] and
-// sequences [n_seqs] as above and there; part_o [n_parts, n_heads, head_dim] and part_ml [n_parts, n_heads, 2] are written where members say.  The caches are
+// sequences [n_seqs] (pages, first result, results, which sequence; those with the most pages of their own first) as above and there; part_o [n_parts, n_heads, head_dim] and part_ml [n_parts, n_heads, 2] are written where members say.  The caches are
 // [n_cache_pages, n_kv_heads, 64, head_dim], contiguous and 16-byte aligned.  head_dim: a multiple of 16 up to 128; n_heads / n_kv_heads at
 // most 128.  status: one int, left as it is unless a wait gave up (then 9, or the other kernel's).
-extern "C" int bn_attention_shared(BnDecodeJoin join, const void* qkv, int q_stride, int k_off, int v_off, void* out, int out_stride, int n_seqs, int n_heads,
+extern "C" int bn_attention_shared(const void* qkv, int q_stride, int k_off, int v_off, void* out, int out_stride, int n_seqs, int n_heads,
                                    int n_kv_heads, int head_dim, float scale, const int* items, int n_items, const int* members, int n_parts,
                                    const int* sequences, const int* tok_pos, const int* slots, const int* page_table, int pt_stride, void* k_cache,
                                    void* v_cache, int n_cache_pages, float* part_o, float* part_ml, int n_splits, int pages_per_block,
                                    int* status, cudaStream_t stream) {
   if (n_items <= 0 || n_seqs <= 0) return BN_OK;
   if (head_dim <= 0 || head_dim % 16 || head_dim > 128 || n_kv_heads <= 0 || n_heads % n_kv_heads || n_heads / n_kv_heads > AS_ROWS || !(scale > 0.f) ||
-      q_stride % 8 || (long long)n_seqs * q_stride > 0x7fffffffll || n_items > 65535 || n_cache_pages <= 0 || !join || !items || !members || !part_o || !part_ml || !status ||
-      (((uintptr_t)qkv | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)items | (uintptr_t)part_o) & 15) || (((uintptr_t)members | (uintptr_t)part_ml) & 7))
+      q_stride % 8 || (long long)n_seqs * q_stride > 0x7fffffffll || n_items > 65535 || n_cache_pages <= 0 || n_parts <= 0 || !items || !members || !sequences || !part_o || !part_ml || !status ||
+      (((uintptr_t)qkv | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)items | (uintptr_t)part_o) & 15) || ((uintptr_t)sequences & 15) || (((uintptr_t)members | (uintptr_t)part_ml) & 7))
     return BN_ERR_BAD_ARG;
   CUtensorMap mk, mv;
   if (!tma_map_bf16_pages(&mk, k_cache, n_cache_pages, (unsigned long long)n_kv_heads * BN_PAGE, head_dim, BN_PAGE) ||
@@ -339,6 +333,7 @@ extern "C" int bn_attention_shared(BnDecodeJoin join, const void* qkv, int q_str
   // 27; 96 KB with two and two: 27.9)
   const int rc = head_dim <= 64 ? as_launch<64, 3, 3>(mk, mv, a, n_items, stream) : as_launch<128, 3, 2>(mk, mv, a, n_items, stream);
   if (rc != BN_OK) return rc;
-  return join(qkv, q_stride, k_off, v_off, out, out_stride, n_seqs, n_heads, n_kv_heads, head_dim, scale, tok_pos, slots, page_table, pt_stride, k_cache, v_cache,
-              n_cache_pages, status, n_splits, pages_per_block, sequences, part_o, part_ml, n_parts, stream);
+  return dt_run<true>(qkv, q_stride, k_off, v_off, out, out_stride, n_seqs, n_heads, n_kv_heads, head_dim, scale, 0, 0, 1.0f, tok_pos, slots, page_table, pt_stride,
+                      k_cache, v_cache, n_cache_pages, status, nullptr, nullptr, n_splits, pages_per_block, nullptr, 0, nullptr, 0, 0, sequences, part_o, part_ml, n_parts,
+                      stream);
 }

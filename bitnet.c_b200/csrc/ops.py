@@ -1040,7 +1040,7 @@ def attention_decode_fused(qkv: torch.Tensor, k_off: int, v_off: int, out: torch
                            theta_scale: float, tok_pos: torch.Tensor, slots: torch.Tensor, page_table: torch.Tensor,
                            k_cache: torch.Tensor, v_cache: torch.Tensor, max_len: int,
                            items: Optional[torch.Tensor] = None, item_group: int = 0) -> torch.Tensor:
-    """The decode step's attention in one launch on tensor cores (attention_decode_tc.cu): rotary
+    """The decode step's attention in one launch on tensor cores (attention_decode_tc.cuh): rotary
     encoding of the raw queries and of the new key (``rotary_dims`` = 0: none), the new key and value
     written into the cache at ``tok_pos``, attention split over the keys, and the combination of
     the splits.  ``qkv`` holds one raw
@@ -1283,16 +1283,10 @@ def attention_decode_shared(qkv: torch.Tensor, k_off: int, v_off: int, out: torc
         global LAUNCHES
         LAUNCHES += 1  # the kernel that joins
         _check(_fn("attention_shared", "bn_attention_shared")(
-            _join_entry(), _ptr(qkv), row, k_off, v_off, _ptr(out), out.shape[1], n_seqs, n_heads, n_kv_heads, head_dim, c_float(scale), items, plan.n_items, members,
+            _ptr(qkv), row, k_off, v_off, _ptr(out), out.shape[1], n_seqs, n_heads, n_kv_heads, head_dim, c_float(scale), items, plan.n_items, members,
             plan.n_parts, sequences, _ptr(tok_pos), _ptr(slots), _ptr(page_table), page_table.shape[1], _ptr(k_cache), _ptr(v_cache), k_cache.shape[0],
             shared_o, shared_ml, n_splits, pages_per_block, _tc_status_arg(device), _stream()), "attention_decode_shared")
     return out
-
-
-@functools.lru_cache(maxsize=None)
-def _join_entry() -> c_void_p:
-    """``bn_attention_decode_tc_join``, which attention_shared.cu calls."""
-    return ctypes.cast(build.library("attention_decode_tc").bn_attention_decode_tc_join, c_void_p)
 
 
 SKINNY_MAX_ROWS = 16  # float32: warp-per-column kernel up to this many rows

@@ -1,5 +1,5 @@
 // Tensor-memory-accelerator loads and the mbarriers they complete on, shared by the kernels that
-// stream tiles from global memory (linear_tc.cu, attention_decode_tc.cu).
+// stream tiles from global memory (linear_tc.cu, attention_decode_tc.cuh).
 //
 // Every wait is bounded in time: a wait that gives up records a code in a status word of the
 // caller and returns false, so that the kernel can drain and return instead of spinning.
