@@ -307,13 +307,14 @@ static int as_launch(const CUtensorMap& mk, const CUtensorMap& mv, const AsArgs&
 
 // The kernel above and directly behind it the joining form of attention_decode_tc.cuh (one call from the host: two take it 3 us more; and that form relies on what is in front).  qkv: [n_seqs, q_stride] bfloat16 rows, rotated, query head h at
 // element h * head_dim, key heads at k_off, value heads at v_off, 16-byte aligned, q_stride a multiple of 8.  items [n_items], members [n_parts] and
-// sequences [n_seqs] (pages, first result, results, which sequence; those with the most pages of their own first) as above and there; part_o [n_parts, n_heads, head_dim] and part_ml [n_parts, n_heads, 2] are written where members say.  The caches are
+// sequences [n_seqs] (pages, first result, results, which sequence; those with the most pages of their own first) as above and there; part_o [n_parts, n_heads, head_dim] and part_ml [n_parts, n_heads, 2] are written where members say.  n_splits blocks, 8 at
+// most, share each sequence's own pages evenly.  The caches are
 // [n_cache_pages, n_kv_heads, 64, head_dim], contiguous and 16-byte aligned.  head_dim: a multiple of 16 up to 128; n_heads / n_kv_heads at
 // most 128.  status: one int, left as it is unless a wait gave up (then 9, or the other kernel's).
 extern "C" int bn_attention_shared(const void* qkv, int q_stride, int k_off, int v_off, void* out, int out_stride, int n_seqs, int n_heads,
                                    int n_kv_heads, int head_dim, float scale, const int* items, int n_items, const int* members, int n_parts,
                                    const int* sequences, const int* tok_pos, const int* slots, const int* page_table, int pt_stride, void* k_cache,
-                                   void* v_cache, int n_cache_pages, float* part_o, float* part_ml, int n_splits, int pages_per_block,
+                                   void* v_cache, int n_cache_pages, float* part_o, float* part_ml, int n_splits,
                                    int* status, cudaStream_t stream) {
   if (n_items <= 0 || n_seqs <= 0) return BN_OK;
   if (head_dim <= 0 || head_dim % 16 || head_dim > 128 || n_kv_heads <= 0 || n_heads % n_kv_heads || n_heads / n_kv_heads > AS_ROWS || !(scale > 0.f) ||
@@ -334,6 +335,6 @@ extern "C" int bn_attention_shared(const void* qkv, int q_stride, int k_off, int
   const int rc = head_dim <= 64 ? as_launch<64, 3, 3>(mk, mv, a, n_items, stream) : as_launch<128, 3, 2>(mk, mv, a, n_items, stream);
   if (rc != BN_OK) return rc;
   return dt_run<true>(qkv, q_stride, k_off, v_off, out, out_stride, n_seqs, n_heads, n_kv_heads, head_dim, scale, 0, 0, 1.0f, tok_pos, slots, page_table, pt_stride,
-                      k_cache, v_cache, n_cache_pages, status, nullptr, nullptr, n_splits, pages_per_block, nullptr, 0, nullptr, 0, 0, sequences, part_o, part_ml, n_parts,
+                      k_cache, v_cache, n_cache_pages, status, nullptr, nullptr, n_splits, 1, nullptr, 0, nullptr, 0, 0, sequences, part_o, part_ml, n_parts,
                       stream);
 }

@@ -1116,7 +1116,7 @@ class SharedPlan:
         self.lengths = [len(p) for p in pages]
         self.longest = max(self.lengths, default=0)
         self.deepest = max(self.first_own, default=0)
-        self._grid = None
+        self._splits = None
         self._lay_out(sms if sms is not None else n_sms(self.device))
         self.table = None
 
@@ -1136,12 +1136,11 @@ class SharedPlan:
         self.table = table
         self.pointers = tuple(c_void_p(table.data_ptr() + 4 * i) for i in self.at)  # items, members, sequences
 
-    def own_grid(self):
-        """``decode_grid`` of the sequences' own pages, at most 8 blocks a sequence: those are one cluster and share no workspace with other launches."""
-        if self._grid is None or self._grid[0] != self.own_pages:
-            splits, each = decode_grid(self.own_pages * PAGE, self.n_seqs, self.n_heads, self.n_kv_heads)
-            self._grid = self.own_pages, ((splits, each) if splits <= 8 else (8, -(-self.own_pages // 8)))
-        return self._grid[1]
+    def own_splits(self) -> int:
+        """How many blocks share a sequence's own pages: ``decode_grid``'s, at most 8 (those are one cluster and share no workspace with other launches)."""
+        if self._splits is None or self._splits[0] != self.own_pages:
+            self._splits = self.own_pages, min(8, decode_grid(self.own_pages * PAGE, self.n_seqs, self.n_heads, self.n_kv_heads)[0])
+        return self._splits[1]
 
     def pad(self, items: int, parts: int) -> "SharedPlan":
         """Bring the list of work to a size, for a recorded step whose list is data: so many items, and places for results."""
@@ -1274,7 +1273,6 @@ def attention_decode_shared(qkv: torch.Tensor, k_off: int, v_off: int, out: torc
         if not plan.n_items:
             return attention_decode_fused(qkv, k_off, v_off, out, n_seqs, n_heads, n_kv_heads, head_dim, scale, 0, 0, 1.0, tok_pos, slots, page_table,
                                           k_cache, v_cache, plan.own_pages * PAGE)
-        n_splits, pages_per_block = plan.own_grid()
         # results of the shared pages, values and then (maximum, sum); a sequence's own splits are one cluster and need no room
         results = plan.n_parts * n_heads
         room = torch.empty(results * (head_dim + 2), dtype=torch.float32, device=device)
@@ -1285,7 +1283,7 @@ def attention_decode_shared(qkv: torch.Tensor, k_off: int, v_off: int, out: torc
         _check(_fn("attention_shared", "bn_attention_shared")(
             _ptr(qkv), row, k_off, v_off, _ptr(out), out.shape[1], n_seqs, n_heads, n_kv_heads, head_dim, c_float(scale), items, plan.n_items, members,
             plan.n_parts, sequences, _ptr(tok_pos), _ptr(slots), _ptr(page_table), page_table.shape[1], _ptr(k_cache), _ptr(v_cache), k_cache.shape[0],
-            shared_o, shared_ml, n_splits, pages_per_block, _tc_status_arg(device), _stream()), "attention_decode_shared")
+            shared_o, shared_ml, plan.own_splits(), _tc_status_arg(device), _stream()), "attention_decode_shared")
     return out
 
 

@@ -61,12 +61,12 @@ class DecodeRunner:
         self.host_items: Optional[List[int]] = None  # what the device buffer holds
         self.items_for = None  # (bucket, page counts) that ``next_items`` was made for
         self.next_items: List[int] = []
-        # Sequences that share pages: what is shared is data (``ops.SharedPlan``), the length of its list and the longest run of own pages are
-        # buckets like that of the lengths.
+        # Sequences that share pages: what is shared is data (``ops.SharedPlan``); the length of its list is a bucket like that of the lengths, and so is
+        # the longest run of own pages, of which only the number of blocks that share a sequence's is part of the recording.
         self.can_share = model.shared_heads() is not None
         self.shared_tables = {}  # bucket -> its buffer, which its recordings point at, and what the buffer holds
         self.shared_for = None  # (slots, the cache's turns) that ``ctx.shared`` was made for
-        self.graphs = {}  # (length bucket, buckets of the shared pages' list and of own pages, or None) -> recorded graph
+        self.graphs = {}  # what ``_shape`` says -> recorded graph
         self.pool = pool
         self.warmed = set()  # whether a step with and without shared pages has run
         self.host_slots: Optional[List[int]] = None
@@ -109,7 +109,7 @@ class DecodeRunner:
             self.launches_per_step[kind] = ops.LAUNCHES - before
             self.warmed.add(kind)
         else:
-            key = (self.ctx.max_len, (self.ctx.shared.n_items, self.ctx.shared.n_parts, self.ctx.shared.own_pages) if kind else None)
+            key = self._shape()
             g = self.graphs.get(key)
             if g is None:
                 g = torch.cuda.CUDAGraph()
@@ -124,6 +124,11 @@ class DecodeRunner:
         self.host_pos = [p + 1 for p in positions]
         self.expect_tokens = None  # known once the caller has read ``sampled``
         return self.sampled
+
+    def _shape(self):
+        """What a recording of this step is good for: (length bucket, buckets of the shared pages' list and blocks of a sequence's own pages, or None)."""
+        plan = self.ctx.shared
+        return self.ctx.max_len, (plan.n_items, plan.n_parts, plan.own_splits()) if plan is not None else None
 
     def _shared_pages(self, slots: Sequence[int], positions: Sequence[int]) -> None:
         """Bring what the sequences share up to date: it changes when one is forked or ends.  (One that takes a new page of its own changes the longest run of

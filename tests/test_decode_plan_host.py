@@ -30,7 +30,7 @@ class TwoHeads:
 
 
 def cache_of(tokens, n):
-    cache = Cache([KvRequest(n_kv_heads=2, head_dim=64)], [None], [None], 64 * 64, 64 * 64, torch.bfloat16, "cpu", max_seqs=12, allocate=False)
+    cache = Cache([KvRequest(n_kv_heads=2, head_dim=64)], [None], [None], 64 * 800, 64 * 64, torch.bfloat16, "cpu", max_seqs=12, allocate=False)
     slot = cache.open()
     cache.reserve(slot, tokens)
     cache.advance(slot, tokens)
@@ -93,3 +93,20 @@ def test_an_upload_that_failed_is_issued_again(monkeypatch):
     runner._shared_pages(slots2, new_tokens(cache2, slots2))
     assert runner.ctx.shared.host == first and runner.ctx.shared.table[:len(first)].tolist() == first
     assert runner.ctx.shared.table is table
+
+
+@pytest.mark.parametrize("n", [2, 12])
+def test_recordings_of_growing_sequences(n):
+    # what a recording is good for changes with the blocks that share a sequence's own pages, not with every bucket of their number
+    cache, slots = cache_of(64 * 5 + 3, n)
+    runner = DecodeRunner(TwoHeads(), cache, None, n)
+    seen, buckets, splits = set(), set(), set()
+    for _ in range(40):
+        runner._shared_pages(slots, new_tokens(cache, slots))
+        seen.add(runner._shape())
+        buckets.add(runner.ctx.shared.own_pages)
+        splits.add(runner.ctx.shared.own_splits())
+        for s in slots:
+            cache.reserve(s, 64)
+            cache.advance(s, 64)
+    assert len(seen) == len(splits) < len(buckets)
