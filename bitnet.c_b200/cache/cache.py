@@ -250,8 +250,9 @@ class Cache:
                 if isinstance(i, tuple):
                     self._named.setdefault(i[0], {})[i[1]] = self.states[i]
         self.turns = 0  # goes up when a sequence is forked or ends: who shares what with whom may then be another
-        self._state_slots = None  # the same for copying a slot of all of them, made when a sequence is first forked
+        self.kept_plan = None  # what the sequences of the last decode step share, kept by the model (``Model.step``)
         self._state_rows = None  # where the states lie, for zeroing a slot of all of them in one launch
+        self._state_slots = None  # the same for copying a slot of all of them, made when a sequence is first forked
         if self.states and torch.device(device).type == "cuda":
             from ..csrc import ops
             self._state_rows = ops.slot_rows(self.states.values())

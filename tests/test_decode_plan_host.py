@@ -1,6 +1,4 @@
 """What a recorded decode step keeps of the pages that its sequences share, without a device."""
-import types
-
 import pytest
 import torch
 
@@ -8,6 +6,7 @@ import bitnet_c_b200  # noqa: F401
 from bitnet_c_b200.cache import Cache
 from bitnet_c_b200.csrc import ops
 from bitnet_c_b200.engine.decode import DecodeRunner
+from bitnet_c_b200.engine.model import Model
 from bitnet_c_b200.parts.base import KvRequest
 
 
@@ -110,3 +109,51 @@ def test_recordings_of_growing_sequences(n):
             cache.reserve(s, 64)
             cache.advance(s, 64)
     assert len(seen) == len(splits) < len(buckets)
+
+
+def test_unrecorded_steps_keep_their_plan(monkeypatch):
+    cache, slots = cache_of(64 * 5 + 3, 4)
+    model, made = TwoHeads(), []
+
+    class Asked(TwoHeads):
+        pays = True
+
+        def shared_pages(self, cache, slots, lengths):
+            made.append(list(slots))
+            plan = super().shared_pages(cache, slots, lengths)
+            return plan if self.pays else None
+
+    model = Asked()
+    step = lambda which=None: Model._plan_of_step(model, cache, list(which or slots), new_tokens(cache, which or slots))  # noqa: E731
+    grow = lambda n: [(cache.reserve(s, n), cache.advance(s, n)) for s in slots]  # noqa: E731
+    first = step()
+    assert first.own_pages == 1 and first.table[:len(first.host)].tolist() == first.host and len(made) == 1
+    for pages in (2, 3, 4):
+        grow(64)
+        assert step() is first and first.own_pages == pages and len(made) == 1
+    assert step(slots[:2]) is not first and step().own_pages == 4 and len(made) == 3  # other sequences, and these again
+    cache.close(slots.pop())
+    assert [r[0] for r in step().runs] == [[0, 1, 2]] and len(made) == 4
+    slots += cache.fork(slots[1])
+    assert [r[0] for r in step().runs] == [[0, 1, 2, 3], [1, 3]] and len(made) == 5
+    monkeypatch.setattr(ops, "USE_SHARED_PAGES", False)
+    step()
+    assert len(made) == 6
+    monkeypatch.undo()
+    # an answer of no is kept as well, an error is not
+    model.pays = False
+    cache.close(slots.pop())
+    assert step() is None and step() is None and len(made) == 7
+    cache.close(slots.pop())
+    model.fails = True
+    for _ in range(2):
+        with pytest.raises(RuntimeError):
+            step()
+    assert len(made) == 9
+    model.fails, model.pays = False, True
+    assert step().runs == [([0, 1], 0, 5)]
+    grow(1024)
+    step()
+    assert len(made) == 11 and step() and len(made) == 11  # asked again after a thousand tokens
+    cache.close(slots.pop())
+    assert step() is None and len(made) == 11  # nothing is shared any more
