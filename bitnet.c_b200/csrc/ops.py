@@ -1115,6 +1115,7 @@ class SharedPlan:
         self.own_pages = max((len(p) - f for p, f in zip(pages, self.first_own)), default=0)
         self.lengths = [len(p) for p in pages]
         self.longest = max(self.lengths, default=0)
+        self.native_layer = 0  # bytes of a layer's matrices if the step could else be launched from one native call (``shared_pays``)
         self.deepest = max(self.first_own, default=0)
         self._splits = None
         self._lay_out(sms if sms is not None else n_sms(self.device))
@@ -1225,7 +1226,14 @@ def shared_pays(plan: SharedPlan) -> bool:
     that are read fewer times and the longest run.  Measured (us, without and with; 32 query heads on 8 of 128, completions of one prompt, 100 tokens
     behind it): 4 of 4,096 tokens 12.6 / 12.9, 8 of 1,024 9.6 / 11.1, 8 of 2,048 14.2 / 13.2, 16 of 1,024 13.3 / 11.7, 64 of 256 16.6 / 17.7, 64 of 8,192 231 / 32;
     8 prompts by 2 of 1,024 13.7 / 14.1, of 2,048 21.3 / 18.1; 40 heads on 40: 16 of 256 17.3 / 18.3, 8 by 2 of 1,024 43 / 47, 64 of 8,192 817 / 76.  In a recorded step,
-    between the products (what is saved in a layer): 4 of 4,096 -0.5, 8 of 2,048 -1.0, 16 of 1,024 0.4, 8 of 3,000 1.4, 8 of 4,096 4, 16 of 2,048 5.7."""
+    between the products (what is saved in a layer): 4 of 4,096 -0.5, 8 of 2,048 -1.0, 16 of 1,024 0.4, 8 of 3,000 1.4, 8 of 4,096 4, 16 of 2,048 5.7.
+
+    A step that is not recorded and could be launched from one native call ends with the device there, which reads a layer's matrices (``plan.native_layer``) and every
+    sequence's keys and values; part by part it takes the host 115 to 130 us a layer, whatever there is to read.  Measured (ms a step, shared on two hosts and native): 32 layers of
+    width 4096 with 8 heads of 128, 16 sequences of 2,048 tokens 3.67 / 3.44, of 4,096 3.64, 4.1 / 3.91, 64 of 1,024 3.94, 4.3 / 4.35, of 2,048 4.0, 4.3 / 5.30; 16 layers of width 2048 with 8 heads
+    of 64, 64 of 4,096 2.07, 2.3 / 1.92, of 8,192 2.10, 2.3 / 2.95; 40 layers of width 5120 with 40 heads of 128, 2 of 8,192 6.0 / 6.16, 8 of 4,096 5.7 / 7.48."""
+    if plan.native_layer and plan.native_layer + sum(plan.lengths) * PAGE * plan.n_kv_heads * plan.head_dim * 4 < 720e6:
+        return False
     saved = sum((len(members) - 1) * n for members, _first, n in plan.runs)
     longest = max((n for _members, _first, n in plan.runs), default=0)
     return saved * plan.n_kv_heads >= 1900 and (longest >= 32 or (longest >= 8 and saved >= 0.6 * sum(plan.lengths)))

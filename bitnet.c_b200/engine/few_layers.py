@@ -112,6 +112,14 @@ class FewLayers:
         planes = cache.own_planes(len(layers[0]), m.spec.n_kv_heads, m.spec.head_dim, torch.bfloat16, m.w_qkv.device)
         return (*layers, planes) if planes is not None else None
 
+    @staticmethod
+    def layer_bytes(taken) -> int:
+        """Bytes of a layer's matrices, of what ``takes`` answered; 0 for None."""
+        if taken is None:
+            return 0
+        layer = taken[0][0]
+        return sum(2 * w.numel() for w in (layer.mixer.w_qkv, layer.mixer.w_o, layer.ffn.w_gate_up, layer.ffn.w_down))
+
     def run(self, taken, x, h, ctx, last_norm):
         """The layers on the residual x [T, width] from the first one's normed rows h; ``taken`` is what ``takes`` answered, ``last_norm`` the norm
         behind the last layer, if that layer's product is to prepare it.  Returns what is pending (as the last block would)."""

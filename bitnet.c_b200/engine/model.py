@@ -113,17 +113,18 @@ class Model:
                 return heads, i
         return None
 
-    def shared_pages(self, cache: Cache, slots: Sequence[int], lengths: Sequence[int]):
+    def shared_pages(self, cache: Cache, slots: Sequence[int], lengths: Sequence[int], native_layer: int = 0):
         """For a decode step of these sequences (``lengths``: before it): the plan of what they share, not yet on the device, or None if that is nothing, too
-        little to pay, or nothing that a mixer of this model can make use of."""
+        little to pay, or nothing that a mixer of this model can make use of.  ``native_layer``: as ``ops.shared_pays`` looks at it."""
         found = self.shared_heads() if cache.shares_pages() and ops.USE_SHARED_PAGES else None
         if found is None:
             return None
         heads, entry = found
         plan = ops.SharedPlan([cache.pages_of(entry, s, n // PAGE + 1) for s, n in zip(slots, lengths)], *heads, self.device)
+        plan.native_layer = native_layer
         return plan if ops.shared_pays(plan) else None
 
-    def _plan_of_step(self, cache: Cache, slots: List[int], lengths: Sequence[int]):
+    def _plan_of_step(self, cache: Cache, ctx: StepContext, slots: List[int], lengths: Sequence[int]):
         """The plan of an unrecorded decode step, on the device, or None.  Making it takes the host longer than a kernel (60 us for 16 sequences of 2,048 tokens, 170 for
         64 of 4,096), so the cache keeps it, or that there is none, until a sequence is forked or ends; what grows meanwhile is the sequences' own pages.  (Whether it
         pays is asked again every 1,024 tokens.)"""
@@ -132,7 +133,8 @@ class Model:
         now = (slots, cache.turns, max(lengths) // 1024, ops.USE_SHARED_PAGES)
         if cache.kept_plan is None or cache.kept_plan[0] != now:
             cache.kept_plan = None
-            plan = self.shared_pages(cache, slots, lengths)
+            native = self.few_layers.layer_bytes(self.few_layers.takes(self, cache, ctx)) if self.few_layers is not None else 0
+            plan = self.shared_pages(cache, slots, lengths, native)
             cache.kept_plan = now, plan.upload() if plan is not None else None
         plan = cache.kept_plan[1]
         if plan is not None:
@@ -282,7 +284,7 @@ class Model:
             cache.sync()
             ctx = pack_step(seqs, lengths, self.device)
             if ctx.decode:
-                ctx.shared = self._plan_of_step(cache, [s.slot for s in seqs], lengths)
+                ctx.shared = self._plan_of_step(cache, ctx, [s.slot for s in seqs], lengths)
             logits = self.forward(cache, ctx)
         except BaseException:
             for s in seqs:  # the step did not happen: its pages go back, the lengths stay

@@ -1,4 +1,6 @@
 """What a recorded decode step keeps of the pages that its sequences share, without a device."""
+import types
+
 import pytest
 import torch
 
@@ -6,6 +8,7 @@ import bitnet_c_b200  # noqa: F401
 from bitnet_c_b200.cache import Cache
 from bitnet_c_b200.csrc import ops
 from bitnet_c_b200.engine.decode import DecodeRunner
+from bitnet_c_b200.engine.few_layers import FewLayers
 from bitnet_c_b200.engine.model import Model
 from bitnet_c_b200.parts.base import KvRequest
 
@@ -15,6 +18,7 @@ class TwoHeads:
 
     device = torch.device("cpu")
     fails = False
+    few_layers = None
 
     def shared_heads(self):
         return (8, 2, 64), 0
@@ -22,7 +26,7 @@ class TwoHeads:
     def decode_blocks_per_sequence(self):
         return 0
 
-    def shared_pages(self, cache, slots, lengths):
+    def shared_pages(self, cache, slots, lengths, native_layer=0):
         if self.fails:
             raise RuntimeError("no room for the plan")
         return ops.SharedPlan([cache.pages_of(0, s, n // 64 + 1) for s, n in zip(slots, lengths)], 8, 2, 64, "cpu", sms=148)
@@ -118,13 +122,13 @@ def test_unrecorded_steps_keep_their_plan(monkeypatch):
     class Asked(TwoHeads):
         pays = True
 
-        def shared_pages(self, cache, slots, lengths):
+        def shared_pages(self, cache, slots, lengths, native_layer=0):
             made.append(list(slots))
-            plan = super().shared_pages(cache, slots, lengths)
+            plan = super().shared_pages(cache, slots, lengths, native_layer)
             return plan if self.pays else None
 
     model = Asked()
-    step = lambda which=None: Model._plan_of_step(model, cache, list(which or slots), new_tokens(cache, which or slots))  # noqa: E731
+    step = lambda which=None: Model._plan_of_step(model, cache, None, list(which or slots), new_tokens(cache, which or slots))  # noqa: E731
     grow = lambda n: [(cache.reserve(s, n), cache.advance(s, n)) for s in slots]  # noqa: E731
     first = step()
     assert first.own_pages == 1 and first.table[:len(first.host)].tolist() == first.host and len(made) == 1
@@ -157,3 +161,35 @@ def test_unrecorded_steps_keep_their_plan(monkeypatch):
     assert len(made) == 11 and step() and len(made) == 11  # asked again after a thousand tokens
     cache.close(slots.pop())
     assert step() is None and len(made) == 11  # nothing is shared any more
+
+
+def test_unrecorded_steps_that_one_native_call_runs_sooner():
+    weights = [torch.empty(shape, dtype=torch.bfloat16, device="meta") for shape in ((768, 1024), (1024, 512), (8192, 1024), (1024, 4096))]
+    part = types.SimpleNamespace(w_qkv=weights[0], w_o=weights[1], w_gate_up=weights[2], w_down=weights[3])
+    matrices = sum(2 * w.numel() for w in weights)
+
+    class Native(FewLayers):
+        def takes(self, model, cache, ctx):
+            return ([types.SimpleNamespace(mixer=part, ffn=part)], None, None) if ctx == "few" else None
+
+    class Model2(TwoHeads):
+        few_layers, told = Native(), []
+
+        def shared_pages(self, cache, slots, lengths, native_layer):
+            self.told.append(native_layer)
+
+    cache, slots = cache_of(64 * 5 + 3, 4)
+    positions, model = new_tokens(cache, slots), Model2()
+    for ctx in ("few", "few", "many"):  # (what was answered once is kept)
+        Model._plan_of_step(model, cache, ctx, slots, positions)
+    cache.kept_plan = None
+    Model._plan_of_step(model, cache, "many", slots, positions)
+    assert model.told == [matrices, 0]
+    # the rule: what the native call has the device read
+    pages = [list(range(400)) + [1000 + i, 2000 + i] for i in range(64)]
+    plan = ops.SharedPlan(pages, 32, 8, 128, "cpu", sms=148)
+    assert ops.shared_pays(plan)
+    for read, pays in ((720e6 - 1e6, False), (720e6 + 1e6, True)):
+        plan.lengths = [402 * 64 // 30]  # (so many pages that the matrices are a part of it)
+        plan.native_layer = int(read) - plan.lengths[0] * 64 * 8 * 128 * 4
+        assert ops.shared_pays(plan) == pays
