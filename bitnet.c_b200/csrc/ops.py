@@ -1179,7 +1179,7 @@ class SharedPlan:
         for c in count:
             place.append(at)
             at += c
-        self.n_parts, self.n_items = at, len(work)
+        self.n_parts, self.n_items, self.most_parts = at, len(work), max(count, default=0)
         order = sorted(range(self.n_seqs), key=lambda b: self.first_own[b] - self.lengths[b])
         items, entries, sequences = [], [], [x for b in order for x in (self.first_own[b], place[b], count[b], b)]
         for members, first, n in work:
@@ -1227,6 +1227,9 @@ def shared_pays(plan: SharedPlan) -> bool:
     behind it): 4 of 4,096 tokens 12.6 / 12.9, 8 of 1,024 9.6 / 11.1, 8 of 2,048 14.2 / 13.2, 16 of 1,024 13.3 / 11.7, 64 of 256 16.6 / 17.7, 64 of 8,192 231 / 32;
     8 prompts by 2 of 1,024 13.7 / 14.1, of 2,048 21.3 / 18.1; 40 heads on 40: 16 of 256 17.3 / 18.3, 8 by 2 of 1,024 43 / 47, 64 of 8,192 817 / 76.  In a recorded step,
     between the products (what is saved in a layer): 4 of 4,096 -0.5, 8 of 2,048 -1.0, 16 of 1,024 0.4, 8 of 3,000 1.4, 8 of 4,096 4, 16 of 2,048 5.7.
+    Few key/value heads (single calls): 16 heads of 128 on one, 64 of 2,048 18.2 / 22.7, of 8,192 38.2 / 27.8; 32 on two, 16 of 8,192 24.0 / 36.9 (its results of 40 places are
+    joined for as long as the rest takes), 64 of 2,048 27.8 / 20.7; 128 on one, where every sequence is a block of its own with sharing too, but reads a page once and not eight times, 4 of
+    8,192 24.0 / 38.7, 8 of 8,192 38.3 / 29.4, 64 of 8,192 238 / 68; 100 heads of 64 on one, 64 of 2,048 39.0 / 25.5.
 
     A step that is not recorded and could be launched from one native call ends with the device there, which reads a layer's matrices (``plan.native_layer``) and every
     sequence's keys and values; part by part it takes the host 115 to 130 us a layer, whatever there is to read.  Measured (ms a step, shared on two hosts and native): 32 layers of
@@ -1234,9 +1237,16 @@ def shared_pays(plan: SharedPlan) -> bool:
     of 64, 64 of 4,096 2.07, 2.3 / 1.92, of 8,192 2.10, 2.3 / 2.95; 40 layers of width 5120 with 40 heads of 128, 2 of 8,192 6.0 / 6.16, 8 of 4,096 5.7 / 7.48."""
     if plan.native_layer and plan.native_layer + sum(plan.lengths) * PAGE * plan.n_kv_heads * plan.head_dim * 4 < 720e6:
         return False
-    saved = sum((len(members) - 1) * n for members, _first, n in plan.runs)
+    # A sequence's own walk reads a page of one head once per 16 of its query heads, the second time and on from the L2 (each taken for half a page); with sharing each
+    # block of up to 128 rows reads it.
+    group = plan.n_heads // plan.n_kv_heads
+    walk, most = ((group + 15) // 16 + 1) / 2, SHARED_ROWS // group
+    saved = sum((len(members) * walk - -(-len(members) // most)) * n for members, _first, n in plan.runs)
     longest = max((n for _members, _first, n in plan.runs), default=0)
-    return saved * plan.n_kv_heads >= 1900 and (longest >= 32 or (longest >= 8 and saved >= 0.6 * sum(plan.lengths)))
+    # joining a sequence's results of the shared pages takes a block 0.12 us for each and for every 512 numbers of them
+    join = plan.most_parts * -(-min(16, group) * plan.head_dim // 512)
+    return (saved * plan.n_kv_heads >= max(1900, 50 * join)
+            and (longest >= 32 or (longest >= 8 and saved >= 0.6 * walk * sum(plan.lengths))))
 
 
 def attention_decode_shared(qkv: torch.Tensor, k_off: int, v_off: int, out: torch.Tensor, n_seqs: int, n_heads: int, n_kv_heads: int, head_dim: int,
