@@ -12,8 +12,9 @@
 // hundreds) and decides.  Where too many keys lie together (ties by the thousand, a huge temperature), borders are found by the bits of the keys
 // instead, 11, 11 and 10 at a time, the weights of the keys that agree with the bits found so far added into a histogram.
 // Weights are whole numbers of 64 bits: sums do not depend on the order of additions, and a running sum that lies next to a border falls on the
-// same side as in a sum of doubles (a float sum would move a token in a thousand).  2^-y is taken apart into 2^-(j/32) from a table, a shift, and
-// 1 - e of a remainder below 1/32, whose e is small enough for a float: y = (max - l) / T * log2(e) is carried in two floats.
+// same side as in a sum of doubles unless it is within 10^-9 of the sum (a float sum would move a token in a thousand).  exp(-y) is taken apart into 2^-(j/32) from a
+// table, a shift, and 1 - e of what is left of y behind multiples of ln 2 / 32 (in two parts, after Cody and Waite).  y = (max - l) / T and e are carried in two floats,
+// since one of them is off by up to 2^-30 of the weight by itself: weights are good to 2^-31, where this was measured on the CPU 2^-31.2.
 //
 // Measured: one row of 32,000 with top-k 11.3 us, 8 rows of 128,256 with top-p 17.9, 64 rows of 128,256 with parameters of their own 35.6, 200 flat
 // rows of 50,257 in bfloat16 53.5.  Few rows are bound by latency (the first block's plan takes 5.5 us, handing over and deciding 2.7, the cluster's barriers 2.5), many by some
@@ -29,6 +30,9 @@
 #define SF_COUNTED 65000 // keys of a block whose weights' halves add up in 32 bits whatever their steps
 #define SF_POINT 56      // a weight of 1 is 2^56 while a thread adds up its own (at most 2^7 of them)
 #define SF_MAX_CLUSTER 8
+#define SF_FAR 44.4f           // as far as there are steps: 64 octaves
+#define SF_32ND (5678.f / 262144.f)      // ln 2 / 32, 13 bits of it
+#define SF_32ND_REST 9.98318279e-7f      // and the rest
 
 struct SfArgs {
   const void* logits;
@@ -155,9 +159,9 @@ struct SfRow {
   int turn = 0;
   double top, per_t;     // the largest logit, 1 / temperature
   bool infinite;         // the largest logit is +inf: those share everything
-  float topf, c_hi, c_lo;  // the largest logit, log2(e) / temperature in two floats
+  float topf, t_hi, t_lo;  // the largest logit, 1 / temperature in two floats
   int fine;                // steps are 2^-fine of a 32nd of an octave: as fine as lets the smallest weight have a step in front of the last
-  float steps;             // to an octave
+  float steps;             // in 1 of y
 
   __device__ __forceinline__ unsigned key(int i) const { return sf_key(to_f32<T>(RESIDENT ? held[i] : row[i])); }
   __device__ __forceinline__ double weight(unsigned k) const {
@@ -277,29 +281,28 @@ struct SfRow {
   }
 
   // ---- by steps of weight ----
-  // The step of a logit (falling logits, rising steps: the nearest to y), and what its y is from the 32nd of an octave that the step lies in.  Conversions
-  // by adding 1.5 * 2^23: those of the conversion unit take four times the issue slots.  (Whatever the logit, the step is one of those that there are.)
-  __device__ __forceinline__ int step_of(float v, float* rest) const {
+  // The step of a logit (falling logits, rising steps: the nearest to y), and 1 - exp(-r), in two floats, of what is left (r) of y behind the 32nd of an octave that the
+  // step lies in.  Conversions by adding 1.5 * 2^23: those of the conversion unit take four times the issue slots.  (Whatever the logit, the step is one of those that
+  // there are.)  SF_32ND has 13 bits, so that its multiples and the first part of r are exact.
+  __device__ __forceinline__ int step_of(float v, float2* e) const {
     const float d = topf - v, bb = d - topf, dl = (topf - (d - bb)) - (v + bb);
-    const float y = d * c_hi, yl = fmaf(d, c_hi, -y) + fmaf(d, c_lo, dl * c_hi);
-    const int n = (int)min((unsigned)__float_as_int(fmaf(fminf(y, 64.f), steps, 12582912.f)) - 0x4B400000u, SF_STEPS - 1u);
-    *rest = fmaf(__int_as_float((n >> fine) + 0x4B400000) - 12582912.f, -1.f / 32.f, y) + yl;
+    const float y = d * t_hi, yl = fmaf(d, t_hi, -y) + fmaf(d, t_lo, dl * t_hi);
+    const int n = (int)min((unsigned)__float_as_int(fmaf(fminf(y, SF_FAR), steps, 12582912.f)) - 0x4B400000u, SF_STEPS - 1u);
+    const float at = __int_as_float((n >> fine) + 0x4B400000) - 12582912.f;
+    const float r = fmaf(at, -SF_32ND, y), rl = fmaf(at, -SF_32ND_REST, yl), s = r + rl;
+    // 1 - exp(-r) = r - r^2 / 2 + r^3 / 6 - r^4 / 24 and less than 2^-34
+    *e = make_float2(r, rl - s * (s * (0.5f - s * (0.16666667f - s * 0.041666668f))));
     return n;
   }
   __device__ __forceinline__ int step_of(float v) const {
-    return (int)min((unsigned)__float_as_int(fmaf(fminf((topf - v) * c_hi, 64.f), steps, 12582912.f)) - 0x4B400000u, SF_STEPS - 1u);
-  }
-  // 1 - 2^-rest
-  static __device__ __forceinline__ float short_of(float rest) {
-    const float g = rest * 0.69314718f;
-    return g * (1.f - g * (0.5f - g * (0.16666667f - g * 0.041666668f)));
+    return (int)min((unsigned)__float_as_int(fmaf(fminf((topf - v) * t_hi, SF_FAR), steps, 12582912.f)) - 0x4B400000u, SF_STEPS - 1u);
   }
   // The weight that a step's 32nd of an octave has its keys' weights from.
   __device__ __forceinline__ unsigned long long most_at(int n) const { return s.table[(n >> fine) & 31] >> (n >> fine >> 5); }
-  // 2^-y, 1 = 2^SF_POINT, to 2^-30 of itself
-  __device__ __forceinline__ unsigned long long weight_at(int n, float e) const {
-    const int whole = __float2int_rn(e * 4294967296.f), at = n >> fine;
-    const unsigned long long w = s.table[at & 31] - (((long long)s.small_table[at & 31] * whole) >> (62 - SF_POINT));
+  // exp(-y), 1 = 2^SF_POINT, to 2^-32 of itself
+  __device__ __forceinline__ unsigned long long weight_at(int n, float2 e) const {
+    const int whole = __float2int_rn(e.x * 17179869184.f) + __float2int_rn(e.y * 17179869184.f), at = n >> fine;  // (below 2^29)
+    const unsigned long long w = s.table[at & 31] - (((long long)s.small_table[at & 31] * whole) >> (64 - SF_POINT));
     return nothing(n) ? 0ull : w >> (at >> 5);
   }
   // Whether a step's keys weigh nothing: the last one's, where steps are as wide as they get (else no key lies there).
@@ -346,7 +349,7 @@ struct SfRow {
   }
 
   // All blocks: the keys by their steps.  With top-k their numbers (in one histogram: two, for fewer lanes that meet, cost the first block 0.6 us of loads); without it
-  // their weights, to 2^-31 of themselves.
+  // their weights, to 2^-31 of themselves (half of which is what is left behind 31 bits).
   __device__ __forceinline__ void count_steps(bool numbers) const {
     if (numbers) {
       each_value([&](const auto& v, int) {
@@ -360,10 +363,10 @@ struct SfRow {
       each_value([&](const auto& v, int) {
 #pragma unroll
         for (const float x : v) {
-          float rest;
-          const int n = step_of(x, &rest);
-          // 2^31 - e 2^31 in halves: e 2^15 is cut to a whole number, what is left of it has 16 bits more
-          const float e = short_of(rest), z = fmaf(e, 32768.f, -0.5f) + 12582912.f, left = fmaf(e, 32768.f, 12582912.f - z);
+          float2 e;
+          const int n = step_of(x, &e);
+          // 2^31 - e 2^31 in halves: e 2^15 is cut to a whole number, what is left of it (from -0.0003 to 1) has 16 bits more
+          const float z = fmaf(e.x + e.y, 32768.f, -0.4999f) + 12582912.f, left = fmaf(e.y, 32768.f, fmaf(e.x, 32768.f, 12582912.f - z));
           if (!nothing(n)) {
             atomicAdd(&s.one[n], (unsigned)(0x4B400000 + 32767 - __float_as_int(z)));
             atomicAdd(&s.two[n], (unsigned)(0x4B400000 + 65536 - __float_as_int(fmaf(left, 65536.f, 12582912.f))));
@@ -579,7 +582,7 @@ struct SfRow {
     float from[4], to[4];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const float y0 = topf - ((float)last[r] + 0.6f) / (steps * c_hi), y1 = topf - ((float)first[r] - 0.6f) / (steps * c_hi);
+      const float y0 = topf - ((float)last[r] + 0.6f) / (steps * t_hi), y1 = topf - ((float)first[r] - 0.6f) / (steps * t_hi);
       from[r] = fmaxf(y0 - fminf(fabsf(y0), 1e38f) * 1e-6f, -3.4028235e38f);
       to[r] = numbers ? INFINITY : y1 + fminf(fabsf(y1), 1e38f) * 1e-6f;
       if (first[r] < 0) from[r] = INFINITY, to[r] = -INFINITY;
@@ -591,13 +594,13 @@ struct SfRow {
     };
     const auto settle = [&](int i) {
       const float x = to_f32<T>(RESIDENT ? held[i] : row[i]);
-      float rest;
-      const int n = step_of(x, &rest);
+      float2 e;
+      const int n = step_of(x, &e);
       bool in = false;
 #pragma unroll
       for (int r = 0; r < 4; ++r) in |= n >= first[r] && n <= last[r] && !nothing(n);
       if (numbers) {
-        const unsigned long long w = weight_at(n, short_of(rest));
+        const unsigned long long w = weight_at(n, e);
 #pragma unroll
         for (int r = 0; r < 4; ++r)
           if (n < first[r]) add(over[r], w);
@@ -705,9 +708,9 @@ struct SfRow {
     int n[EACH];
 #pragma unroll
     for (int e = 0; e < EACH; ++e) {
-      float rest;
-      n[e] = step_of(sf_value(~(unsigned)(entry[e] >> 32)), &rest);
-      const unsigned long long w = tid + e * GROUP < m ? to_scale(weight_at(n[e], short_of(rest))) : 0ull;
+      float2 less;
+      n[e] = step_of(sf_value(~(unsigned)(entry[e] >> 32)), &less);
+      const unsigned long long w = tid + e * GROUP < m ? to_scale(weight_at(n[e], less)) : 0ull;
       run[e] = w;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -906,12 +909,12 @@ __global__ void __launch_bounds__(SF_THREADS, 1024 / SF_THREADS) sample_filtered
     row.infinite = row.topf == INFINITY;
     row.per_t = 1.0 / (double)temperature;
     const double c = 1.4426950408889634 * row.per_t;
-    row.c_hi = (float)c;
-    row.c_lo = (float)(c - (double)row.c_hi);
-    const float octaves = (row.topf - sf_value(0u - low)) * row.c_hi;
+    row.t_hi = (float)row.per_t;
+    row.t_lo = (float)(row.per_t - (double)row.t_hi);
+    const float octaves = (row.topf - sf_value(0u - low)) * (float)c;
     row.fine = 0;
     while (row.fine < 5 && octaves * (float)(64 << row.fine) < (float)(SF_STEPS - 2)) ++row.fine;
-    row.steps = (float)(32 << row.fine);
+    row.steps = (float)(32 << row.fine) * 1.442695f;
     const bool k_on = top_k > 0 && top_k < a.vocab, p_on = top_p > 0.f && top_p < 1.f, m_on = min_p > 0.f;
     bool by_bits = row.infinite || !(c > 1e-30 && c < 1e30) || a.per > SF_COUNTED;
     if (!by_bits) {
