@@ -2883,7 +2883,7 @@ def sample_filtered(logits: torch.Tensor, temperature, top_k=0, top_p=1.0, min_p
     temperature of 0 takes the first maximum; where there are logits of +inf, they share everything equally.
     Each parameter is a number or a tensor with one per row (``top_k`` int32, the others float32; numbers are rounded to float32).
     The random numbers are ``u`` [rows] in [0, 1), or row r draws from (and advances) the xorshift64* state ``rng_state[index[r]]`` (or [r]; no
-    two rows one state)."""
+    two rows one state; a row whose index names none gets -1)."""
     _need_rows(logits, "logits")
     n, vocab = logits.shape
     at = logits.get_device()
@@ -2923,7 +2923,7 @@ def sample_filtered(logits: torch.Tensor, temperature, top_k=0, top_p=1.0, min_p
     with _on(logits.device):
         _check(_fn("sampling_filtered", "bn_sample_filtered")(
             _ptr(logits), _code(logits), ctypes.c_longlong(logits.stride(0) if n > 1 else vocab), n, vocab, c_float(t), ts, k, ks, c_float(p), ps, c_float(m),
-            ms, us, states, indices, _ptr(out), _stream()), "sample_filtered")
+            ms, us, states, 0 if rng_state is None else min(rng_state.shape[0], 0x7fffffff), indices, _ptr(out), _stream()), "sample_filtered")
     return out
 
 

@@ -30,6 +30,7 @@
 #define SF_COUNTED 65000 // keys of a block whose weights' halves add up in 32 bits whatever their steps
 #define SF_POINT 56      // a weight of 1 is 2^56 while a thread adds up its own (at most 2^7 of them)
 #define SF_MAX_CLUSTER 8
+#define SF_NO_STATE 0xffffffffu  // in place of a random number: the row's index names no generator
 #define SF_FAR 44.4f           // as far as there are steps: 64 octaves
 #define SF_32ND (5678.f / 262144.f)      // ln 2 / 32, 13 bits of it
 #define SF_32ND_REST 9.98318279e-7f      // and the rest
@@ -45,8 +46,9 @@ struct SfArgs {
   const float* top_ps;
   const float* min_ps;
   const float* u;             // per row, or null: drawn from rng
-  unsigned long long* rng;
+  unsigned long long* rng;    // n_states of them
   const int* index;           // row -> its generator, or null
+  int n_states;
   int* out;
   int scale_bits;             // weights are multiples of 2^-scale_bits
   unsigned long long table[32];  // 2^-(j/32), 1 = 2^SF_POINT
@@ -881,11 +883,14 @@ __global__ void __launch_bounds__(SF_THREADS, 1024 / SF_THREADS) sample_filtered
   else __syncthreads();  // every block of the cluster runs: its shared memory may be written
   // the random number, drawn once for the whole cluster
   if (rank == 0 && threadIdx.x == 0) {
+    const int i = a.index ? a.index[r] : r;
     float u;
     if (a.u) {
       u = a.u[r];
+    } else if (i < 0 || i >= a.n_states) {
+      u = __uint_as_float(SF_NO_STATE);
     } else {  // xorshift64*, as in sampling.cu
-      unsigned long long* state = a.rng + (a.index ? a.index[r] : r);
+      unsigned long long* state = a.rng + i;
       unsigned long long x = *state;
       x ^= x >> 12; x ^= x << 25; x ^= x >> 27;
       *state = x;
@@ -901,6 +906,7 @@ __global__ void __launch_bounds__(SF_THREADS, 1024 / SF_THREADS) sample_filtered
   low = s.low;
   row.exchange_max(&high, &low);
   const float asked_u = __uint_as_float((unsigned)s.found[0]), u = asked_u > 0.f ? asked_u : 0.f;
+  if (a.u == nullptr && (unsigned)s.found[0] == SF_NO_STATE) high = 0u;  // as a row without a number above -inf
   unsigned chosen = high;
   unsigned long long tie = 0;
   if (high != 0u && temperature > 0.f) {
@@ -1018,11 +1024,11 @@ static int sf_run(SfArgs& a, int n_rows, cudaStream_t stream) {
 }
 
 // logits [n_rows, vocab] of `dtype`, rows ld numbers apart.  The four parameters hold for all rows where their array is null.  u: a number in
-// [0, 1) per row, or null: drawn from the generator rng[index ? index[r] : r], which is advanced.  out: the tokens, -1 for a row
-// without a number above -inf.
+// [0, 1) per row, or null: drawn from the generator rng[index ? index[r] : r] (of n_states), which is advanced.  out: the tokens, -1 for a row
+// without a number above -inf, or without a generator.
 extern "C" int bn_sample_filtered(const void* logits, int dtype, long long ld, int n_rows, int vocab, float temperature, const float* temperatures,
                                   int top_k, const int* top_ks, float top_p, const float* top_ps, float min_p, const float* min_ps, const float* u,
-                                  unsigned long long* rng, const int* index, int* out, cudaStream_t stream) {
+                                  unsigned long long* rng, int n_states, const int* index, int* out, cudaStream_t stream) {
   if (n_rows <= 0) return BN_OK;
   if (!logits || !out || vocab <= 0 || ld < vocab || (!u && !rng) || (dtype != BN_F32 && dtype != BN_BF16) || n_rows > 0x7fffffff / SF_MAX_CLUSTER)
     return BN_ERR_BAD_ARG;
@@ -1030,7 +1036,7 @@ extern "C" int bn_sample_filtered(const void* logits, int dtype, long long ld, i
   a.logits = logits; a.ld = ld; a.vocab = vocab;
   a.temperature = temperature; a.top_p = top_p; a.min_p = min_p; a.top_k = top_k;
   a.temperatures = temperatures; a.top_ks = top_ks; a.top_ps = top_ps; a.min_ps = min_ps;
-  a.u = u; a.rng = rng; a.index = index; a.out = out;
+  a.u = u; a.rng = rng; a.n_states = n_states; a.index = index; a.out = out;
   int bits = 0;
   while ((1ll << bits) < vocab) ++bits;
   a.scale_bits = 62 - bits < SF_POINT ? 62 - bits : SF_POINT;  // the sum of all weights stays below 2^62
