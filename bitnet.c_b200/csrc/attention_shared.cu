@@ -316,8 +316,8 @@ extern "C" int bn_attention_shared(const void* qkv, int q_stride, int k_off, int
                                    const int* sequences, const int* tok_pos, const int* slots, const int* page_table, int pt_stride, void* k_cache,
                                    void* v_cache, int n_cache_pages, float* part_o, float* part_ml, int n_splits,
                                    int* status, cudaStream_t stream) {
-  if (n_items <= 0 || n_seqs <= 0) return BN_OK;
-  if (head_dim <= 0 || head_dim % 16 || head_dim > 128 || n_kv_heads <= 0 || n_heads % n_kv_heads || n_heads / n_kv_heads > AS_ROWS || !(scale > 0.f) ||
+  if (n_seqs <= 0) return BN_OK;
+  if (n_items <= 0 || head_dim <= 0 || head_dim % 16 || head_dim > 128 || n_kv_heads <= 0 || n_heads % n_kv_heads || n_heads / n_kv_heads > AS_ROWS || !(scale > 0.f) ||
       q_stride % 8 || (long long)n_seqs * q_stride > 0x7fffffffll || n_items > 65535 || n_cache_pages <= 0 || n_parts <= 0 || !items || !members || !sequences || !part_o || !part_ml || !status ||
       (((uintptr_t)qkv | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)items | (uintptr_t)part_o) & 15) || ((uintptr_t)sequences & 15) || (((uintptr_t)members | (uintptr_t)part_ml) & 7))
     return BN_ERR_BAD_ARG;

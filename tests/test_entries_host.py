@@ -1,4 +1,5 @@
 """Entries of the compiled kernels, and the status codes of kernels that lie in headers (no device)."""
+import ctypes
 import glob
 import os
 import re
@@ -40,3 +41,16 @@ def test_every_code_names_its_kernel(monkeypatch, family, name, code):
     ops.tc_status(cpu).fill_(code)
     with pytest.raises(ops.KernelError, match=rf"^{family}: "):
         ops.check_tc_status(cpu)
+
+
+def test_sequences_without_anything_shared_are_refused_by_the_entry():
+    # (it would launch nothing, and the sequences' results would be those of the call before)
+    entry = build.library("attention_shared").bn_attention_shared
+    entry.restype = ctypes.c_int
+    p, i, f = ctypes.c_void_p, ctypes.c_int, ctypes.c_float
+    at = p(1 << 12)  # (16-byte aligned; refused before anything is read)
+    call = lambda n_seqs, n_items: entry(at, i(768), i(512), i(640), at, i(512), i(n_seqs), i(8), i(2), i(64), f(0.1), at, i(n_items), at, i(4), at, at, at, at, i(4),  # noqa: E731
+                                         at, at, i(9), at, at, i(1), at, p(0))
+    assert call(0, 0) == 0
+    for n_items in (0, -1, 65536):
+        assert call(3, n_items) == 1
