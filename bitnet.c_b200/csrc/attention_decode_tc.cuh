@@ -776,7 +776,7 @@ static int dt_run(const void* qkv, int q_stride, int k_off, int v_off, void* out
     return BN_ERR_BAD_ARG;
   if constexpr (JOIN) {
     if (head_dim > 128 || n_splits > 8 || out_stride % 4 || (((uintptr_t)out) & 7)) return BN_ERR_BAD_ARG;  // (splits are merged within a cluster)
-    // (always two stages: a third block an SM gains more beside the shared pages' blocks; 64 sequences of up to 9 pages of their own: 31.5 us, 36 with three)
+    // (always two stages: a third block an SM gains more beside the shared pages' blocks; 64 sequences of up to 9 pages of their own, when it was chosen: 31.5 us, 36 with three)
     if (head_dim <= 64) return launch_dt2<64, 2, true>(mk, mv, a, grid, cluster, stream);
     return launch_dt2<128, 2, true>(mk, mv, a, grid, cluster, stream);
   } else {

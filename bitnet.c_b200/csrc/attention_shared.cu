@@ -15,7 +15,7 @@
 //
 // The bytes bound it, the list of work spreads the pages over five blocks on four SMs, beside which the blocks of the sequences' own pages run: a page takes a
 // block about 0.9 us, the tensor cores' part of which is a sixth.  Both kernels together, 32 heads on 8 of 128: 64 sequences behind 8,192 tokens with 500 of
-// their own 31.8 us (231 where each reads all its pages), 8 prompts of 2,048 by 8 with 300 of their own 26.3 us.
+// their own 31.9 us (231 where each reads all its pages), 8 prompts of 2,048 by 8 with 300 of their own 27.0 us.
 #include "attention_decode_tc.cuh"
 #include "umma.cuh"
 
@@ -105,7 +105,7 @@ attention_shared_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
   const unsigned tmem_base = *tmem_slot;
 
   if (warp == 0) {
-    // (whatever filled the pages, or chose the slots, may still run before that: pages asked for in front of it gain 0.5 us of 26 for 64 sequences, less for others)
+    // (whatever filled the pages, or chose the slots, may still run before that: asking in front of it was worth 0.5 us of 27 for 64 sequences, less for others)
     pdl_wait();
     if (lane == 0) {
       const int* pt = a.page_table + (size_t)a.slots[item.y >> 8] * a.pt_stride + item.z;
@@ -330,8 +330,8 @@ extern "C" int bn_attention_shared(const void* qkv, int q_stride, int k_off, int
   a.per_group = n_heads / n_kv_heads; a.scale_log2e = scale * 1.4426950408889634f; a.items = (const int4*)items; a.members = (const int2*)members;
   a.n_members = n_parts; a.n_parts = n_parts; a.slots = slots; a.page_table = page_table; a.pt_stride = pt_stride; a.part_o = part_o;
   a.part_ml = part_ml; a.status = status;
-  // 64 KB and 112 KB: room for blocks of the sequences' own pages on the same SM, or for a second one of these (128 KB with rings of three and three: 36 us where it is
-  // 27; 96 KB with two and two: 27.9)
+  // 64 KB and 112 KB: room for blocks of the sequences' own pages on the same SM, or for a second one of these (64 behind 8,192 and 8 by 8: 31.9 and 27.0 us; 128 KB
+  // with rings of three and three: 32.4 and 36.0; 96 KB with two and two: 32.2 and 27.2)
   const int rc = head_dim <= 64 ? as_launch<64, 3, 3>(mk, mv, a, n_items, stream) : as_launch<128, 3, 2>(mk, mv, a, n_items, stream);
   if (rc != BN_OK) return rc;
   return dt_run<true>(qkv, q_stride, k_off, v_off, out, out_stride, n_seqs, n_heads, n_kv_heads, head_dim, scale, 0, 0, 1.0f, tok_pos, slots, page_table, pt_stride,

@@ -1160,7 +1160,7 @@ class SharedPlan:
         most = SHARED_ROWS // (self.n_heads // self.n_kv_heads)  # sequences of a block
         tiles = [(members[i:i + most], first, n) for members, first, n in self.runs for i in range(0, len(members), most)]
         # five blocks on four SMs, which share all pages evenly: with one an SM some wait longest for their pages, with two the sequences' own pages wait until they
-        # have ended (8 prompts of 2,048 tokens by 8 sequences: 25.9 us, 27.2 with one, 32.8 with two; 64 sequences behind one of 8,192: 31.7, 31.6 and 36.2)
+        # have ended (8 prompts of 2,048 tokens by 8 sequences: 27.0 us, 28.0 with one, 34.4 with two; 64 sequences behind one of 8,192: 31.8, 31.8 and 36.6)
         budget = max(1, 5 * sms // (4 * self.n_kv_heads))
         longest = max((n for _m, _f, n in tiles), default=1)
         each = min(longest, max(SHARED_MIN_PAGES, -(-sum(n for _m, _f, n in tiles) // budget)))
@@ -1224,9 +1224,10 @@ def shared_plan(pages, n_heads: int, n_kv_heads: int, head_dim: int, device) -> 
 def shared_pays(plan: SharedPlan) -> bool:
     """Whether ``attention_decode_shared`` (with the rotation in front of it) gains over every sequence reading its pages for itself, by the pages of single heads
     that are read fewer times and the longest run.  Measured (us, without and with; 32 query heads on 8 of 128, completions of one prompt, 100 tokens
-    behind it): 4 of 4,096 tokens 12.6 / 12.9, 8 of 1,024 9.6 / 11.1, 8 of 2,048 14.2 / 13.2, 16 of 1,024 13.3 / 11.7, 64 of 256 16.6 / 17.7, 64 of 8,192 231 / 32;
-    8 prompts by 2 of 1,024 13.7 / 14.1, of 2,048 21.3 / 18.1; 40 heads on 40: 16 of 256 17.3 / 18.3, 8 by 2 of 1,024 43 / 47, 64 of 8,192 817 / 76.  In a recorded step,
-    between the products (what is saved in a layer): 4 of 4,096 -0.5, 8 of 2,048 -1.0, 16 of 1,024 0.4, 8 of 3,000 1.4, 8 of 4,096 4, 16 of 2,048 5.7.
+    behind it): 4 of 4,096 tokens 12.7 / 12.7, 8 of 1,024 9.6 / 11.3, 8 of 2,048 14.2 / 13.7, 16 of 1,024 13.3 / 12.4, 64 of 256 16.6 / 18.0, 64 of 8,192 231 / 32;
+    8 prompts by 2 of 1,024 13.7 / 14.4, of 2,048 21.0 / 18.3; 40 heads on 40: 16 of 256 17.2 / 18.5, 64 of 2,048 241 / 64.  In a recorded step,
+    between the products (what is saved in a layer): 4 of 4,096 -0.5, 8 of 2,048 -1.4, 16 of 1,024 0, 8 of 3,000 0.3, 8 of 4,096 4, 4 of 8,192 2.3, 16 of 2,048 4.8.
+    It errs towards not sharing: 2 of 8,192 (18.9 / 15.7) and 64 of 256 with 40 heads on 40 (56.6 / 52.4) would gain.
     Few key/value heads (single calls): 16 heads of 128 on one, 64 of 2,048 18.2 / 22.7, of 8,192 38.2 / 27.8; 32 on two, 16 of 8,192 24.0 / 36.9 (its results of 40 places are
     joined for as long as the rest takes), 64 of 2,048 27.8 / 20.7; 128 on one, where every sequence is a block of its own with sharing too, but reads a page once and not eight times, 4 of
     8,192 24.0 / 38.7, 8 of 8,192 38.3 / 29.4, 64 of 8,192 238 / 68; 100 heads of 64 on one, 64 of 2,048 39.0 / 25.5.
@@ -1255,7 +1256,8 @@ def attention_decode_shared(qkv: torch.Tensor, k_off: int, v_off: int, out: torc
     """``attention_decode_fused`` for sequences that share pages: pages that several of them begin with are read once for all (``plan``, of
     ``shared_plan``), each sequence's own pages as ever, and the two are joined, in two launches.  ``qkv`` holds rotated q|k|v rows; the new key and
     value are written into the cache at ``tok_pos``.  No window; heads of at most 128.  ``max_len``: no sequence is longer, its new token included; it may be
-    left out, also where arguments go by their place (``..., v_cache, plan``): the plan knows it to a page."""
+    left out, also where arguments go by their place (``..., v_cache, plan``): the plan knows it to a page.
+    Where little is shared (``shared_pays``) every sequence for itself is faster (8 prompts of 256 tokens by 2: 9.0 us, 12.3 here): that is the caller's to choose."""
     if isinstance(max_len, SharedPlan):
         if plan is not None:
             raise KernelError("attention_decode_shared: two plans")

@@ -9,16 +9,20 @@
 // follow.  One pass adds up the keys' weights (with top-k: counts the keys) in steps of 2^(1/32) of the weight (finer ones
 // where the row's weights lie closer together: fewer keys meet in a step); from these sums the first block of the
 // cluster knows in which step each border lies.  A second pass hands the keys of those steps to it; it sorts them (some tens of keys, of a flat row
-// hundreds) and decides.  Where too many keys lie together (ties by the thousand, a huge temperature), borders are found by the bits of the keys
+// hundreds) and decides.  Where too many keys lie together (ties by the thousand, a huge temperature) or the border is not known well (a top-k of thousands), borders are found by the bits of the keys
 // instead, 11, 11 and 10 at a time, the weights of the keys that agree with the bits found so far added into a histogram.
 // Weights are whole numbers of 64 bits: sums do not depend on the order of additions, and a running sum that lies next to a border falls on the
 // same side as in a sum of doubles unless it is within 10^-9 of the sum (a float sum would move a token in a thousand).  exp(-y) is taken apart into 2^-(j/32) from a
 // table, a shift, and 1 - e of what is left of y behind multiples of ln 2 / 32 (in two parts, after Cody and Waite).  y = (max - l) / T and e are carried in two floats,
 // since one of them is off by up to 2^-30 of the weight by itself: weights are good to 2^-31, where this was measured on the CPU 2^-31.2.
 //
-// Measured: one row of 32,000 with top-k 11.3 us, 8 rows of 128,256 with top-p 17.9, 64 rows of 128,256 with parameters of their own 35.6, 200 flat
-// rows of 50,257 in bfloat16 53.5.  Few rows are bound by latency (the first block's plan takes 5.5 us, handing over and deciding 2.7, the cluster's barriers 2.5), many by some
-// 66 instructions a number, two additions in shared memory (2.8 cycles a warp's where no lanes meet) among them.
+// Measured: one row of 32,000 with top-k 11.4 us, 8 rows of 128,256 with top-p 17.6, 64 rows of 128,256 with parameters of their own 36.5, 200 flat
+// rows of 50,257 in bfloat16 54.5.  Few rows are bound by latency (the first block's plan takes 5.5 us, handing over and deciding 2.7, the cluster's barriers 2.5), many by some
+// 69 instructions a number, two additions in shared memory (2.8 cycles a warp's where no lanes meet) among them.
+//
+// Borders by bits are slow.  Ties: 64 rows of 128,256 equal numbers 4.2 ms.  Top-k of thousands: with top-k, steps are counted and not summed, so every mass is known to some 4.7 % only, and
+// the keys between the bounds may be more than the list holds.  64 rows of 128,256 normal logits of spread 3 with a top-k of 50 / 1,000 / 5,000 / 50,000: 24.6 / 41 / 307 / 327 us,
+// with top-p 0.95 behind it 26.2 / 47 / 525 / 535; one row 13.9 / 15.9 / 19.1 / 34.3 and 14.6 / 27.9 / 186 / 188.  A temperature of 10,000: 64 rows 290, one 98.
 #include "common.cuh"
 #include <math.h>
 
@@ -1007,17 +1011,17 @@ static int sf_run(SfArgs& a, int n_rows, cudaStream_t stream) {
   cudaError_t e = cudaGetDevice(&device);
   if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
   if (e != cudaSuccess) return BN_ERR_LAUNCH + (int)e;
-  // Blocks of a row: so many that each has 4,096 numbers (one row of 32,000: 16.2 us with one block, 14.1 with two, 12.4 with eight), but not
-  // more than 2.75 an SM in all, of which two run at once (64 rows of 128,256: 37 us with four blocks a row, 51 with eight; 200 of 50,257: 54 with two, 65 with
-  // four).  Clusters of eight only for some ten rows: more of them do not find their place at once (12 rows of 128,256: 22.0 us with eight, 20.3 with four; 10: 19.8 and 20.2;
-  // 40: 36.8 and 31.5).  No fewer blocks than add up a row's numbers.
+  // Blocks of a row: so many that each has 4,096 numbers (one row of 32,000: 14.9 us with one block, 13.2 with two, 11.3 with eight), but not
+  // more than 2.75 an SM in all, of which two run at once (64 rows of 128,256: 36.7 us with four blocks a row, 49.6 with eight; 200 of 50,257: 54 with two, 65 with
+  // four).  Clusters of eight only for some ten rows: more of them do not find their place at once (12 rows of 128,256: 22.6 us with eight, 19.8 with four; 10: 20.0 and 19.8;
+  // 40: 37.4 and 32.6).  No fewer blocks than add up a row's numbers.
   int blocks = SF_MAX_CLUSTER;
   while (blocks > 1 && a.vocab <= blocks / 2 * 4096) blocks /= 2;
   if (blocks == 8 && 64ll * n_rows > 5ll * sms && (a.vocab + 3) / 4 <= SF_COUNTED - 8) blocks = 4;
   while (blocks > 1 && 4ll * n_rows * blocks > 11ll * sms && (a.vocab + blocks / 2 - 1) / (blocks / 2) <= SF_COUNTED - 8) blocks /= 2;
   a.per = (((a.vocab + blocks - 1) / blocks) + 7) & ~7;
   // The row stays in shared memory where two blocks an SM still fit, or where there is one at most; else later passes find it in the L2 (256 rows of 32,000 in float32,
-  // one block each: 45 us from the L2, 53 held).
+  // one block each: 31.9 us from the L2, 39.9 held).
   const size_t base = (sizeof(SfShared) + 15) & ~(size_t)15, held = (((size_t)a.per * sizeof(T)) + 15) & ~(size_t)15;
   const bool resident = base + held <= ((long long)n_rows * blocks <= sms ? 220 : 112) * 1024 && a.per <= 128 * SF_THREADS;
   return resident ? sf_launch<T, true>(a, n_rows, blocks, base + held, stream) : sf_launch<T, false>(a, n_rows, blocks, base, stream);
